@@ -274,6 +274,119 @@ int pbs_prefill_fwd(const pbs_shape_t* shape,
                     void* out, const int64_t out_strides[4],
                     const pbs_options_t* options, const pbs_scratch_t* scratch, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * What follows a prompt: a paged cache of keys and values, the attention of new tokens over it, and the
+ * logits of a step.  No counterpart in the reference, which hands single tokens back to the model's own
+ * forward (pbs_attn/patch/huggingface.py:182-192).
+ *
+ * A cache is a pool of pages of page_size tokens.  The token at position p of sequence b lies in page
+ * block_table[b][p / page_size], slot p % page_size, for every KV head.
+ *   bits = 16: k and v are (pages, Hkv, page_size, D) of `dtype`.
+ *   bits = 4:  k and v are (pages, Hkv, page_size, D / 2) bytes, channel 2i in the low and 2i + 1 in the
+ *              high half of byte i; params are (pages, Hkv, page_size, D / group_size, 2) of `dtype`: step and
+ *              minimum of each group of group_size neighbouring channels of one token and head.  A code c
+ *              stands for minimum + c * step.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct {
+  void* k;
+  void* v;
+  void* k_params;          /* bits = 4 only (NULL otherwise)                                            */
+  void* v_params;
+  int64_t k_strides[3];    /* page, head, slot, in elements: of dtype for 16 bits, bytes for 4.  Rows   */
+  int64_t v_strides[3];    /* start on 16-byte boundaries                                               */
+  int64_t k_params_strides[3];   /* page, head, slot, in elements of dtype; a token's row of steps and  */
+  int64_t v_params_strides[3];   /* minima is dense and starts on a multiple of min(16, its size) bytes */
+  int32_t num_pages;
+  int32_t page_size;       /* a power of two, 16 .. 1024                                                */
+  int32_t kv_heads;
+  int32_t head_dim;        /* 64, 128 or 256                                                            */
+  int32_t dtype;           /* PBS_BF16 or PBS_FP16                                                      */
+  int32_t bits;            /* 16 or 4                                                                   */
+  int32_t group_size;      /* bits = 4: 32 or 64                                                        */
+  int32_t reserved;
+  int32_t* status;         /* one word that the device can write (pinned host memory will do); a call   */
+} pbs_paged_cache_t;       /* that finds one of the faults below stores it there and works around it    */
+
+#define PBS_PAGED_BAD_PAGE 1    /* a page number outside the pool: such a token is neither written nor attended  */
+#define PBS_PAGED_BAD_LENGTH 2  /* a sequence longer than its row of the block table: it ends with that row      */
+#define PBS_PAGED_BAD_ROTARY 3  /* a position behind the rotary tables: the token is neither rotated nor written */
+
+/* The sequences of a call.  seq_lens counts the new tokens in: token i of the new_lens[b] new ones of sequence b is at
+ * position seq_lens[b] - new_lens[b] + i.  Tokens at negative positions are left out (an unused row of a batch has length
+ * 0).  new_lens outside 0 .. new_tokens are taken as the nearer of the two. */
+typedef struct {
+  const int32_t* block_table;   /* (batch, max_pages); entries behind a sequence's last page are not read */
+  int64_t table_stride;         /* elements from row to row                                               */
+  const int32_t* seq_lens;      /* (batch)                                                                */
+  const int32_t* new_lens;      /* (batch), or NULL: new_tokens for all                                   */
+  int32_t max_pages;
+  int32_t batch;
+  int32_t new_tokens;           /* S: rows per sequence of the call's tensors                             */
+  int32_t reserved;
+} pbs_paged_batch_t;
+
+/* Writes the new tokens' keys and values, (B, Hkv, S, D), into the cache.  With rotary tables the keys are rotated on the
+ * way (x cos + rotate_half(x) sin in 32 bits), and the queries, if given: q (B, q_heads, S, D) -> q_out, which may be q; rows
+ * that are left out become 0.  cos and sin: (table_rows, D), indexed by position, with cs_strides = {0, row, 1}; or, with
+ * table_rows = 0, (B or 1, S, D) with cs_strides = {batch (0 to share), token, 1}.  NULL: no rotation, and no queries.
+ * 4 bits, per group, in 32 bits: step = (max / 2 - min / 2) * (2 / 15) and minimum, both rounded to dtype, and code =
+ * round((x - minimum) * (1 / step)) within 0 .. 15.  A group that holds an infinity or a NaN reads back as NaN. */
+int pbs_paged_append(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* batch,
+                     const void* k, const int64_t k_strides[4], const void* v, const int64_t v_strides[4],
+                     int32_t q_heads, const void* q, const int64_t q_strides[4], void* q_out, const int64_t q_out_strides[4],
+                     const void* cos_table, const void* sin_table, const int64_t cs_strides[3], int32_t table_rows, void* stream);
+
+/* The new tokens' keys and values as they are in the cache, back as (B, Hkv, S, D) of dtype; 0 for what was left out.
+ * A value of 4 bits beyond the finite numbers of dtype (its step was rounded up) becomes the nearest of them. */
+int pbs_paged_gather(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* batch, void* k, const int64_t k_strides[4],
+                     void* v, const int64_t v_strides[4], void* stream);
+
+/* Causal attention of the new tokens' queries, q (B, q_heads, S, D), over the cache: token i sees the positions up to its own.
+ * out has q's shape; rows that see nothing are 0.  Softmax and sums are held in 32 bits.
+ * workspace: pbs_paged_attn_workspace bytes, the first PBS_PAGED_COUNTER_BYTES of them 0 before the first call (each call leaves
+ * them so).  Calls that share one come after one another. */
+#define PBS_PAGED_COUNTER_BYTES 16384
+int pbs_paged_attn_workspace(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* batch, int32_t q_heads, int64_t* bytes);
+int pbs_paged_attn(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* batch, int32_t q_heads,
+                   const void* q, const int64_t q_strides[4], void* out, const int64_t out_strides[4],
+                   float scale, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Penalties, biases and a grammar mask on the logits of a step, (rows, vocab), rounded once:
+ *   seen in the row's history:        x > 0 ? x / repetition : x * repetition
+ *   c times in its written part:      x - frequency * c, then x - presence if c > 0
+ *   listed in the row's biases:       x + value (values of a token that is listed twice add up, in their order)
+ *   bit v % 32 of word v / 32 is 0:   -infinity
+ * The history of row b is tokens[b][0 .. token_lens[b]), its first prompt_lens[b] the prompt, the rest written.  Ids outside
+ * the vocabulary are skipped, in biases too.  NULL: without that part (NULL lengths: the whole row, no prompt).  A row of the
+ * bias's values is in the order of its ids; repetition is above 0. */
+typedef struct {
+  int32_t dtype;                  /* pbs_dtype_t of logits and out                              */
+  int32_t rows, vocab;
+  int32_t history;                /* entries a row of tokens                                    */
+  int32_t biases;                 /* entries a row of bias_ids and bias_values                  */
+  int32_t token_bytes;            /* 4 or 8: integers in tokens                                 */
+  int32_t bias_id_bytes;          /* 4 or 8: integers in bias_ids                               */
+  int32_t reserved;
+  const void* logits;
+  void* out;                      /* may be logits; must not overlap it otherwise               */
+  int64_t logits_stride, out_stride;   /* elements from row to row                              */
+  const void* tokens;
+  int64_t tokens_stride;
+  const int32_t* token_lens;      /* (rows)                                                     */
+  const int32_t* prompt_lens;     /* (rows)                                                     */
+  const float* repetition;        /* (rows), or NULL: repetition_all (1: none)                  */
+  const float* frequency;         /* (rows), or NULL: frequency_all (0: none)                   */
+  const float* presence;          /* (rows), or NULL: presence_all (0: none)                    */
+  float repetition_all, frequency_all, presence_all;
+  int32_t reserved2;
+  const void* bias_ids;
+  const float* bias_values;
+  int64_t bias_ids_stride, bias_values_stride;
+  const uint32_t* allowed;        /* (rows or 1, ceil(vocab / 32)) words                        */
+  int64_t allowed_stride;         /* words from row to row (0 to share)                         */
+} pbs_logits_t;
+int pbs_process_logits(const pbs_logits_t* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -54,9 +54,38 @@ class Options(C.Structure):
 
 
 Strides4 = C.c_int64 * 4
+
+
+class PagedCache(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("k", "v", "k_params", "v_params")]
+                + [(n, C.c_int64 * 3) for n in ("k_strides", "v_strides", "k_params_strides", "v_params_strides")]
+                + [(n, C.c_int32) for n in ("num_pages", "page_size", "kv_heads", "head_dim", "dtype", "bits", "group_size", "reserved")]
+                + [("status", C.c_void_p)])
+
+
+class PagedBatch(C.Structure):
+    _fields_ = [("block_table", C.c_void_p), ("table_stride", C.c_int64), ("seq_lens", C.c_void_p), ("new_lens", C.c_void_p),
+                ("max_pages", C.c_int32), ("batch", C.c_int32), ("new_tokens", C.c_int32), ("reserved", C.c_int32)]
+
+
+PAGED_COUNTER_BYTES = 16384
+
+
+class Logits(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "rows", "vocab", "history", "biases", "token_bytes", "bias_id_bytes", "reserved")]
+                + [("logits", C.c_void_p), ("out", C.c_void_p), ("logits_stride", C.c_int64), ("out_stride", C.c_int64),
+                   ("tokens", C.c_void_p), ("tokens_stride", C.c_int64)]
+                + [(n, C.c_void_p) for n in ("token_lens", "prompt_lens", "repetition", "frequency", "presence")]
+                + [(n, C.c_float) for n in ("repetition_all", "frequency_all", "presence_all")] + [("reserved2", C.c_int32)]
+                + [("bias_ids", C.c_void_p), ("bias_values", C.c_void_p), ("bias_ids_stride", C.c_int64),
+                   ("bias_values_stride", C.c_int64), ("allowed", C.c_void_p), ("allowed_stride", C.c_int64)])
+
+
 _P = C.c_void_p
 _SH = C.POINTER(Shape)
 _ST = C.POINTER(C.c_int64)
+_PC = C.POINTER(PagedCache)
+_PB = C.POINTER(PagedBatch)
 
 # name -> argument types; every function returns int except the two noted below
 SIGNATURES = {
@@ -77,6 +106,11 @@ SIGNATURES = {
     "pbs_ipc_import": [C.POINTER(C.c_ubyte * 64), C.POINTER(C.c_void_p)],
     "pbs_ipc_release": [_P],
     "pbs_prefill_fwd": [_SH, _P, _ST, _P, _ST, _P, _ST, _P, _ST, C.POINTER(Options), C.POINTER(Scratch), _P],
+    "pbs_paged_append": [_PC, _PB, _P, _ST, _P, _ST, C.c_int32, _P, _ST, _P, _ST, _P, _P, _ST, C.c_int32, _P],
+    "pbs_paged_gather": [_PC, _PB, _P, _ST, _P, _ST, _P],
+    "pbs_paged_attn_workspace": [_PC, _PB, C.c_int32, C.POINTER(C.c_int64)],
+    "pbs_paged_attn": [_PC, _PB, C.c_int32, _P, _ST, _P, _ST, C.c_float, _P, C.c_int64, _P],
+    "pbs_process_logits": [C.POINTER(Logits), _P],
 }
 EXPORTS = ["pbs_last_error_string", "pbs_version", "pbs_launch_count"] + list(SIGNATURES)
 

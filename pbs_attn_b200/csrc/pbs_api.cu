@@ -35,6 +35,19 @@ int device_sms() {
   return n;
 }
 
+int check_tensor(const char* name, const void* p, const int64_t* st, int dt, Strides* out) {
+  if (!p || !st) { set_error("%s: null pointer or strides", name); return PBS_ERR_ARG; }
+  const int e = elem_bytes(dt);
+  if (st[3] != 1) { set_error("%s: innermost (head_dim) stride is %lld, must be 1", name, (long long)st[3]); return PBS_ERR_LAYOUT; }
+  if (((uintptr_t)p & 15) || ((st[0] * e) & 15) || ((st[1] * e) & 15) || ((st[2] * e) & 15)) {
+    set_error("%s: base pointer and every row must be 16-byte aligned", name);
+    return PBS_ERR_LAYOUT;
+  }
+  if (st[0] < 0 || st[1] < 0 || st[2] <= 0) { set_error("%s: negative or zero-length row stride", name); return PBS_ERR_LAYOUT; }
+  out->b = st[0]; out->h = st[1]; out->s = st[2];
+  return PBS_OK;
+}
+
 namespace {
 
 // kv_in_place took the place of padding: structs of callers built without it keep their layout.
@@ -61,22 +74,6 @@ int check_shape(const pbs_shape_t* s) {
   }
   return PBS_OK;
 }
-
-int check_tensor(const char* name, const void* p, const int64_t* st, int dt, Strides* out) {
-  if (!p || !st) { set_error("%s: null pointer or strides", name); return PBS_ERR_ARG; }
-  const int e = elem_bytes(dt);
-  if (st[3] != 1) { set_error("%s: innermost (head_dim) stride is %lld, must be 1", name, (long long)st[3]); return PBS_ERR_LAYOUT; }
-  if (((uintptr_t)p & 15) || ((st[0] * e) & 15) || ((st[1] * e) & 15) || ((st[2] * e) & 15)) {
-    set_error("%s: base pointer and every row must be 16-byte aligned", name);
-    return PBS_ERR_LAYOUT;
-  }
-  if (st[0] < 0 || st[1] < 0 || st[2] <= 0) { set_error("%s: negative or zero-length row stride", name); return PBS_ERR_LAYOUT; }
-  out->b = st[0]; out->h = st[1]; out->s = st[2];
-  return PBS_OK;
-}
-
-#define PBS_TRY(x) do { int rc__ = (x); if (rc__ != PBS_OK) return rc__; } while (0)
-#define PBS_NONNULL(p) do { if (!(p)) { set_error(#p " is null"); return PBS_ERR_ARG; } } while (0)
 
 // A TMA descriptor cannot describe a broadcast (zero-stride) batch or head dimension.
 bool layout_fits_tc(const Dims& d, int heads, const Strides& st) {

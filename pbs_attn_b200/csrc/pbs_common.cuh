@@ -169,6 +169,11 @@ void count_launch();
     ::pbs::count_launch();                                            \
   } while (0)
 
+// Checks of arguments at the C entries (pbs_api.cu).
+int check_tensor(const char* name, const void* p, const int64_t* st, int dt, Strides* out);   // a (B, H, S, D) operand
+#define PBS_TRY(x) do { int rc__ = (x); if (rc__ != PBS_OK) return rc__; } while (0)
+#define PBS_NONNULL(p) do { if (!(p)) { set_error(#p " is null"); return PBS_ERR_ARG; } } while (0)
+
 // Stage launchers (defined one per .cu file).
 int device_sms();             // SMs of the current device, the one a launch goes to
 struct QueryPooling;                     // null, or what the first scoring pass pools beside its own work where it can
