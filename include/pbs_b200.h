@@ -320,7 +320,7 @@ typedef struct {
   const int32_t* seq_lens;      /* (batch)                                                                */
   const int32_t* new_lens;      /* (batch), or NULL: new_tokens for all                                   */
   int32_t max_pages;
-  int32_t batch;
+  int32_t batch;                /* at most 4096                                                           */
   int32_t new_tokens;           /* S: rows per sequence of the call's tensors                             */
   int32_t reserved;
 } pbs_paged_batch_t;

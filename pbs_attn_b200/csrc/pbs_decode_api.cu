@@ -29,6 +29,7 @@ int check_paged(const pbs_paged_cache_t* c, const pbs_paged_batch_t* b, PagedArg
   }
   if ((int64_t)b->max_pages * c->page_size > INT_MAX) { set_error("a row of the block table holds more than 2^31 tokens"); return PBS_ERR_SHAPE; }
   if (b->table_stride < 0) { set_error("block_table: negative stride"); return PBS_ERR_LAYOUT; }
+  if (b->batch > 4096) { set_error("%d sequences in a call, at most 4096", b->batch); return PBS_ERR_SHAPE; }
   PBS_NONNULL(b->block_table);
   PBS_NONNULL(b->seq_lens);
   PBS_NONNULL(c->status);
@@ -120,8 +121,7 @@ int pbs_paged_attn_workspace(const pbs_paged_cache_t* cache, const pbs_paged_bat
   PBS_NONNULL(bytes);
   PBS_TRY(check_paged(cache, batch, &a));
   PBS_TRY(check_q_heads(a, q_heads));
-  *bytes = paged_attn_workspace(a, q_heads);
-  return PBS_OK;
+  return paged_attn_workspace(a, q_heads, bytes);
 }
 
 int pbs_paged_attn(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* batch, int32_t q_heads, const void* q, const int64_t q_strides[4],
@@ -134,10 +134,9 @@ int pbs_paged_attn(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* batc
   PBS_TRY(check_rows("out", a, q_heads, out, out_strides, true, &ot));
   PBS_NONNULL(workspace);
   if ((uintptr_t)workspace % 16) { set_error("workspace: 16-byte alignment"); return PBS_ERR_LAYOUT; }
-  if (workspace_bytes < paged_attn_workspace(a, q_heads)) {
-    set_error("workspace: %lld bytes, need %lld", (long long)workspace_bytes, (long long)paged_attn_workspace(a, q_heads));
-    return PBS_ERR_SHAPE;
-  }
+  int64_t need;
+  PBS_TRY(paged_attn_workspace(a, q_heads, &need));
+  if (workspace_bytes < need) { set_error("workspace: %lld bytes, need %lld", (long long)workspace_bytes, (long long)need); return PBS_ERR_SHAPE; }
   return launch_paged_attn(a, q_heads, qt, ot, scale, workspace, (cudaStream_t)stream);
 }
 

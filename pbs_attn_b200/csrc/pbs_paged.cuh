@@ -49,7 +49,7 @@ __device__ __forceinline__ int64_t slot_offset(const int64_t (&st)[3], int page,
 int launch_paged_append(const PagedArgs& a, const RowTensor& k, const RowTensor& v, int q_heads, const RowTensor& q, const RowTensor& qo,
                         const void* cosp, const void* sinp, int64_t cs_b, int64_t cs_s, int table_rows, cudaStream_t st);
 int launch_paged_gather(const PagedArgs& a, const RowTensor& k, const RowTensor& v, cudaStream_t st);
-int64_t paged_attn_workspace(const PagedArgs& a, int q_heads);
+int paged_attn_workspace(const PagedArgs& a, int q_heads, int64_t* bytes);
 int launch_paged_attn(const PagedArgs& a, int q_heads, const RowTensor& q, const RowTensor& out, float scale, void* workspace, cudaStream_t st);
 int launch_process_logits(const pbs_logits_t& a, cudaStream_t st);
 

@@ -1,112 +1,901 @@
-// Causal attention of new tokens over a paged cache: out = softmax(scale q K^T) V with the running maximum and sum of one pass.
+// Causal attention of new tokens over a paged cache of 16 or 4 bits: out = softmax(scale q K^T) V in one pass over the cache.
 //
-// One CTA per row (sequence, query head, new token); its warps take every fourth token, a lane D / 32 channels, and meet at the end.
+// Mathematics.  With values of 4 bits K = lo + code * step (step and lo per token and group g of channels)
+//   q . k_t  =  sum_g  step_{t,g} (q_g . code_{t,g})  +  lo_{t,g} sum(q_g)
+//   o_d      =  sum_t (p_t step_{t,g}) code_{t,d}  +  sum_t p_t lo_{t,g},         g the group of channel d,
+// so the codes themselves go into the matrix products and steps and minima act on sums (K) or on the weights (V).  A code's four bits,
+// masked out of a word of eight, ARE an fp16 number: bits 0-3 of a half are code * 2^-24 and bits 4-7 code * 2^-20, subnormal numbers that the
+// tensor cores multiply exactly.  A word of eight codes costs four ANDs and a shift to become four operand registers, and the factors
+// 2^24 and 1/16 go into the queries and the final sums.
+//
+// What bounds it: the cache is read once, (D + 8 D / G) bytes a token and KV head in 4 bits, and a step of the batch has few queries a
+// head, so HBM bounds long caches and latency short ones.  Tokens are the rows (M) of both products and the queries of a KV head the
+// columns (N = 8 NT), because a group of 8 or fewer queries then fills an m16n8k16 product; with queries as rows half of it would be
+// padding.  mma.sync and not tcgen05: the operand that changes is unpacked in registers, tcgen05 would take it back through shared
+// memory (four times the bytes that came in), and the tensor cores are far from being the limit.
+//
+// Work is cut by tokens, not by sequences: all (sequence, row tile, KV head) items in a row, in units of kWarps tiles, are dealt
+// to the resident CTAs in equal contiguous shares, so lengths may differ at will and nothing about them has to be known on the host.
+// An item that several CTAs share is joined by whoever is last, from partial results in the order of the CTAs: same bits every time.
+//
+// Within a CTA every warp takes every kWarps-th tile of 16 or 32 tokens through its own ring of cp.async stages, with its own running
+// reference and sums; warps meet once an item.
+#include <climits>
+#include <type_traits>
+
 #include "pbs_paged.cuh"
 
 namespace pbs {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kMaxGrid = PBS_PAGED_COUNTER_BYTES / 4;
+
+template <int DT_, int D_, int BITS_, int G_, int NT_>
+struct Cfg {
+  static constexpr int DT = DT_, D = D_, BITS = BITS_, G = G_, NT = NT_;
+  using T = typename Elem<DT>::T;
+  static constexpr int COLS = 8 * NT;                              // queries of a tile
+  static constexpr int MT = BITS == 4 && NT <= 2 && NT * D <= 256 ? 2 : 1;   // 16-token products a tile, as registers allow
+  static constexpr int TILE = 16 * MT;
+  static constexpr int WARPS = BITS == 16 && D == 256 ? 4 : 8;
+  static constexpr int THREADS = 32 * WARPS;
+  static constexpr int UNIT = WARPS * TILE;                        // tokens that work is dealt in
+  static constexpr int ROW = BITS == 4 ? D / 2 : 2 * D;            // bytes of a token's row
+  static constexpr int CH = ROW / 16;
+  static constexpr int NG = BITS == 4 ? D / G : 1;
+  static constexpr int PROW = BITS == 4 ? 4 * NG : 0;
+  static constexpr int STAGE = TILE * 2 * (ROW + PROW);
+  static constexpr int OCC = BITS == 4 && NT == 1 && D <= 128 ? 2 : 1;       // CTAs a SM
+  static constexpr int BUDGET = (OCC == 2 ? 112 : 216) * 1024;
+  static constexpr int STAGES_FIT = BUDGET / (WARPS * STAGE);
+  static constexpr int STAGES = STAGES_FIT < 2 ? 2 : STAGES_FIT > 4 ? 4 : STAGES_FIT;
+  static constexpr int RING = WARPS * STAGES * STAGE;
+  static constexpr int OROW = D + 4;                               // floats of a row of partial sums: four on, so that stores spread over the banks
+  static constexpr int MERGE = WARPS * COLS * (OROW + 2) * 4;
+  static constexpr int JOIN = COLS * 2 * 148 * 2 * 4;              // references and sums of all CTAs that may share an item
+  static constexpr int POOL = RING > MERGE ? (RING > JOIN ? RING : JOIN) : (MERGE > JOIN ? MERGE : JOIN);
+  static constexpr int QFRAG = COLS * D * 2;
+  static constexpr int FIXED = POOL + QFRAG + COLS * NG * 4 + COLS * 8;      // then the batch's prefix sums
+};
 
 struct AttnArgs {
   PagedArgs a;
   RowTensor q, out;
-  int q_heads;
-  float scale;                                             // times log2(e)
+  int q_heads, group, row_tiles;
+  float scale;                                                     // times log2(e)
+  int* counters;
+  float* partials;                                                 // [CTA][2]: COLS x D sums, COLS references, COLS sums of weights
 };
 
-template <int DT, int D, int BITS>
-__device__ __forceinline__ void load_row(const pbs_paged_cache_t& c, bool is_v, int page, int head, int slot, int lane, float (&x)[D / 32]) {
-  using E = Elem<DT>;
-  using T = typename E::T;
-  constexpr int N = D / 32;
-  if constexpr (BITS == 16) {
-    const T* p = (const T*)(is_v ? c.v : c.k) + slot_offset(is_v ? c.v_strides : c.k_strides, page, head, slot) + N * lane;
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = E::ld(p + j);
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Copies N bytes, or fills them with zeros.
+template <int N>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool there) {
+  const int n = there ? N : 0;
+  if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void load_matrices_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+// kind: PBS_BF16 or PBS_FP16
+template <int KIND>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (KIND == PBS_BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <class T>
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+  if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) return pack_half(a, b);
+  else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+// Step (low half) and minimum (high half) of a word of params.
+template <class T>
+__device__ __forceinline__ float step_of(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)w));
+  else return __uint_as_float(w << 16);
+}
+template <class T>
+__device__ __forceinline__ float low_of(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)(w >> 16)));
+  else return __uint_as_float(w & 0xffff0000u);
+}
+
+// 16-byte piece `ch` of row `row` in shared memory: neighbouring rows' pieces lie in different banks, so eight rows are read at once.
+template <class C>
+__device__ __forceinline__ int piece(int row, int ch) {
+  constexpr int PER = C::CH >= 8 ? 1 : 8 / C::CH, MASK = (C::CH >= 8 ? 8 : C::CH) - 1;
+  return row * C::ROW + ((ch ^ ((row / PER) & MASK)) << 4);
+}
+
+// Params of one token, NG words.
+template <class C>
+__device__ __forceinline__ void load_params(uint32_t (&w)[C::NG], const uint8_t* p) {
+  if constexpr (C::NG == 1) w[0] = *reinterpret_cast<const uint32_t*>(p);
+  else if constexpr (C::NG == 2) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    w[0] = x.x; w[1] = x.y;
   } else {
-    const uint8_t* p = (const uint8_t*)(is_v ? c.v : c.k) + slot_offset(is_v ? c.v_strides : c.k_strides, page, head, slot) + N / 2 * lane;
-    const T* pp = (const T*)(is_v ? c.v_params : c.k_params) + slot_offset(is_v ? c.v_params_strides : c.k_params_strides, page, head, slot) +
-                  2 * (N * lane / c.group_size);
-    const float step = E::ld(pp), low = E::ld(pp + 1);
 #pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = fmaf((float)((p[j / 2] >> (4 * (j % 2))) & 15), step, low);
-  }
-}
-
-template <int DT, int D, int BITS>
-__global__ void __launch_bounds__(32 * kWarps) paged_attn_kernel(const __grid_constant__ AttnArgs p) {
-  using E = Elem<DT>;
-  using T = typename E::T;
-  constexpr int N = D / 32;
-  const pbs_paged_cache_t& c = p.a.c;
-  const int i = blockIdx.x % p.a.b.new_tokens, seq = blockIdx.x / p.a.b.new_tokens, qh = blockIdx.y, head = qh / (p.q_heads / c.kv_heads);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int last = new_position(p.a.b, seq, i);
-  float q[N], o[N] = {}, m = -CUDART_INF_F, l = 0.f;
-  const T* qp = (const T*)p.q.p + seq * p.q.st.b + qh * p.q.st.h + i * p.q.st.s + N * lane;
-#pragma unroll
-  for (int j = 0; j < N; ++j) q[j] = E::ld(qp + j) * p.scale;
-  for (int t = warp; t <= last; t += kWarps) {
-    const int page = page_of(p.a, seq, t);
-    if (page < 0) {
-      if ((t >> p.a.shift) >= p.a.b.max_pages) break;
-      continue;
+    for (int i = 0; i < C::NG; i += 4) {
+      const uint4 x = *reinterpret_cast<const uint4*>(p + 4 * i);
+      w[i] = x.x; w[i + 1] = x.y; w[i + 2] = x.z; w[i + 3] = x.w;
     }
-    float x[N], s = 0.f;
-    load_row<DT, D, BITS>(c, false, page, head, t & (c.page_size - 1), lane, x);
-#pragma unroll
-    for (int j = 0; j < N; ++j) s = fmaf(q[j], x[j], s);
-    s = warp_sum(s);
-    const float top = fmaxf(m, s), w = s == -CUDART_INF_F ? 0.f : exp2f(s - top), keep = m == -CUDART_INF_F ? 0.f : exp2f(m - top);
-    load_row<DT, D, BITS>(c, true, page, head, t & (c.page_size - 1), lane, x);
-    l = fmaf(l, keep, w);
-#pragma unroll
-    for (int j = 0; j < N; ++j) o[j] = fmaf(w, x[j], o[j] * keep);
-    m = top;
-  }
-  __shared__ float so[kWarps][D], sm[kWarps], sl[kWarps];
-#pragma unroll
-  for (int j = 0; j < N; ++j) so[warp][N * lane + j] = o[j];
-  if (lane == 0) { sm[warp] = m; sl[warp] = l; }
-  __syncthreads();
-  float top = -CUDART_INF_F, sum = 0.f;
-  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w]);
-  float wt[kWarps];
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    wt[w] = sm[w] == -CUDART_INF_F && sl[w] == 0.f ? 0.f : exp2f(sm[w] - top);
-    sum = fmaf(wt[w], sl[w], sum);
-  }
-  for (int d = threadIdx.x; d < D; d += 32 * kWarps) {
-    float x = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) x = fmaf(wt[w], so[w][d], x);
-    ((T*)p.out.p)[seq * p.out.st.b + qh * p.out.st.h + i * p.out.st.s + d] = E::cvt(sum == 0.f ? 0.f : x / sum);
   }
 }
 
-template <int DT, int D>
-int launch(const AttnArgs& p, cudaStream_t st) {
-  const dim3 grid((unsigned)(p.a.b.batch * p.a.b.new_tokens), (unsigned)p.q_heads);
-  if (p.a.c.bits == 16) paged_attn_kernel<DT, D, 16><<<grid, 32 * kWarps, 0, st>>>(p);
-  else paged_attn_kernel<DT, D, 4><<<grid, 32 * kWarps, 0, st>>>(p);
+// One warp's running attention of COLS queries.
+//
+// Weights are p = 2^(score - ref) with a reference per query that is raised only when a product p * step could leave fp16's range (above
+// 2^15), to where the largest is 2^7: so the maximum over the warp is taken once in a while and not every tile, and the products, which
+// are what the result is made of, keep 2^21 below the largest before they lose bits.
+template <class C>
+struct Warp {
+  using T = typename C::T;
+  float o[C::D / 16][C::NT][4];
+  float om[C::BITS == 4 ? C::NG : 1][C::NT][2];                    // sums of p * lo, this lane's tokens
+  float l[C::NT][2], ref[C::NT][2];
+  const uint4* qf;                                                 // this lane's query fragments, C::NT * 32 apart from chunk to chunk
+  const float* qsum;
+  const float* factor;
+  const int* limit;
+  int lane;
+
+  __device__ __forceinline__ void start() {
+#pragma unroll
+    for (int i = 0; i < C::D / 16; ++i)
+#pragma unroll
+      for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[i][n][c] = 0.f;
+#pragma unroll
+    for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        l[n][c] = 0.f;
+        ref[n][c] = -CUDART_INF_F;
+#pragma unroll
+        for (int g = 0; g < (C::BITS == 4 ? C::NG : 1); ++g) om[g][n][c] = 0.f;
+      }
+  }
+
+  // Scores of the tile (times 2^-k of the query's scaling: `factor` has the rest): tot[m][n] holds tokens lane / 4 and + 8, queries 2 (lane % 4) and + 1
+  __device__ __forceinline__ void scores(float (&tot)[C::MT][C::NT][4], const uint8_t* stage) const {
+    const uint32_t k_at = smem_addr(stage);
+#pragma unroll
+    for (int m = 0; m < C::MT; ++m) {
+      float acc[C::NT][4];
+#pragma unroll
+      for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tot[m][n][c] = acc[n][c] = 0.f;
+      const int row = 16 * m + (lane & 15), half = lane >> 4;
+      if constexpr (C::BITS == 16) {
+#pragma unroll
+        for (int ks = 0; ks < C::D / 16; ++ks) {
+          uint32_t r[4];
+          load_matrices(r, k_at + piece<C>(row, 2 * ks + half));
+#pragma unroll
+          for (int n = 0; n < C::NT; ++n) {
+            const uint4 q = qf[(ks / 2 * C::NT + n) * 32];
+            mma<C::DT>(tot[m][n], r[0], r[1], r[2], r[3], ks % 2 ? q.z : q.x, ks % 2 ? q.w : q.y);
+          }
+        }
+      } else {
+        uint32_t kp[2][C::NG];
+        const uint8_t* params = stage + 2 * C::TILE * C::ROW;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) load_params<C>(kp[h], params + (16 * m + lane / 4 + 8 * h) * C::PROW);
+#pragma unroll
+        for (int j2 = 0; j2 < C::CH / 2; ++j2) {
+          uint32_t r[4];
+          load_matrices(r, k_at + piece<C>(row, 2 * j2 + half));
+#pragma unroll
+          for (int jj = 0; jj < 2; ++jj) {
+            const int j = 2 * j2 + jj;
+            const uint32_t x = r[2 * jj], y = r[2 * jj + 1], x8 = x >> 8, y8 = y >> 8;
+            constexpr uint32_t M0 = 0x000f000fu, M1 = 0x00f000f0u;
+#pragma unroll
+            for (int n = 0; n < C::NT; ++n) {
+              const uint4 q = qf[(j * C::NT + n) * 32];
+              mma<PBS_FP16>(acc[n], x & M0, y & M0, x & M1, y & M1, q.x, q.y);
+              mma<PBS_FP16>(acc[n], x8 & M0, y8 & M0, x8 & M1, y8 & M1, q.z, q.w);
+            }
+            if ((j + 1) * 32 % C::G == 0) {
+              const int g = j * 32 / C::G;
+#pragma unroll
+              for (int n = 0; n < C::NT; ++n) {
+                const float2 s = *reinterpret_cast<const float2*>(qsum + g * C::COLS + 8 * n + 2 * (lane % 4));
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                  const float part = fmaf(low_of<T>(kp[c / 2][g]), c % 2 ? s.y : s.x, tot[m][n][c]);
+                  tot[m][n][c] = fmaf(acc[n][c], step_of<T>(kp[c / 2][g]), part);
+                  acc[n][c] = 0.f;
+                }
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+
+  static __device__ __forceinline__ bool too_large(float weight, float wide, float ref) {
+    return !(weight * wide <= 32768.f) || ref == -CUDART_INF_F;
+  }
+
+  // Raises the references of the queries that need it to this tile's scores (x, in powers of 2; wide: the largest step that a query
+  // sees), and weighs the tile anew.  A query's reference depends on what it sees alone, and so does every bit of its result.
+  __device__ __forceinline__ void raise(const float (&x)[C::MT][C::NT][4], float (&p)[C::MT][C::NT][4], const float (&wide)[C::NT][2]) {
+#pragma unroll
+    for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float most = -CUDART_INF_F, weight = 0.f, step = wide[n][c];
+#pragma unroll
+        for (int m = 0; m < C::MT; ++m) {
+          most = fmaxf(most, fmaxf(x[m][n][c], x[m][n][c + 2]));
+          weight = fmaxf(weight, fmaxf(p[m][n][c], p[m][n][c + 2]));
+        }
+        const uint32_t need = __ballot_sync(0xffffffffu, too_large(weight, step, ref[n][c]));
+#pragma unroll
+        for (int s = 4; s < 32; s <<= 1) {
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
+          step = fmaxf(step, __shfl_xor_sync(0xffffffffu, step, s));
+        }
+        const float old = ref[n][c];
+        if ((need & 0x11111111u << lane % 4) && most > -CUDART_INF_F) ref[n][c] = fmaxf(old, most + (C::BITS == 4 ? __log2f(step) : 0.f) - 7.f);
+        const float keep = ref[n][c] == old ? 1.f : exp2_fast(old - ref[n][c]);
+        l[n][c] *= keep;
+#pragma unroll
+        for (int i = 0; i < C::D / 16; ++i) {
+          o[i][n][c] *= keep;
+          o[i][n][c + 2] *= keep;
+        }
+#pragma unroll
+        for (int g = 0; g < (C::BITS == 4 ? C::NG : 1); ++g) om[g][n][c] *= keep;
+#pragma unroll
+        for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+          for (int h = 0; h < 4; h += 2) p[m][n][c + h] = x[m][n][c + h] == -CUDART_INF_F ? 0.f : exp2_fast(x[m][n][c + h] - ref[n][c]);
+      }
+  }
+
+  // Infinities and NaNs among the values of a tile that not all queries see: 0 for the product, and added where they are seen.
+  __device__ __forceinline__ void add_not_finite(const uint8_t* v, int t0) {
+    for (int t = 0; t < C::TILE; ++t)
+#pragma unroll
+      for (int i = 0; i < C::D / 16; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int d = 16 * i + lane / 4 + 8 * h;
+          const float x = Elem<C::DT>::ld(reinterpret_cast<const T*>(v + piece<C>(t, d / 8)) + d % 8);
+          if (fabsf(x) <= 3.402823466e38f) continue;
+#pragma unroll
+          for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              if (t0 + t < limit[8 * n + 2 * (lane % 4) + c]) o[i][n][2 * h + c] += x;
+        }
+  }
+
+  // Takes in the tile of tokens t0 .. in shared memory.  MASKED: some query does not see all of them, or 16 of them (a bit of hole) have no page.
+  template <bool MASKED>
+  __device__ __forceinline__ void tile(const uint8_t* stage, int t0, uint32_t hole) {
+    float x[C::MT][C::NT][4], p[C::MT][C::NT][4];
+    scores(x, stage);
+    bool seen[C::MT][C::NT][4];
+#pragma unroll
+    for (int n = 0; n < C::NT; ++n) {
+      const float2 f = *reinterpret_cast<const float2*>(factor + 8 * n + 2 * (lane % 4));
+      const int2 lim = MASKED ? *reinterpret_cast<const int2*>(limit + 8 * n + 2 * (lane % 4)) : make_int2(0, 0);
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          x[m][n][c] *= c % 2 ? f.y : f.x;
+          if (MASKED) {
+            seen[m][n][c] = t0 + 16 * m + lane / 4 + c / 2 * 8 < (c % 2 ? lim.y : lim.x) && !(hole >> m & 1);
+            if (!seen[m][n][c]) x[m][n][c] = -CUDART_INF_F;
+            p[m][n][c] = seen[m][n][c] ? exp2_fast(x[m][n][c] - ref[n][c % 2]) : 0.f;
+          } else {
+            p[m][n][c] = exp2_fast(x[m][n][c] - ref[n][c % 2]);
+          }
+        }
+    }
+    uint32_t vp[C::MT][2][C::NG];
+    float wide[C::NT][2];
+    float widest = 1.f;
+    if constexpr (C::BITS == 4) {
+      constexpr float kLeast = 0x1p-40f;                           // (weights stay below 2^55, their sum within 32 bits' range)
+      widest = kLeast;
+      float steps[C::MT][2];
+      const uint8_t* params = stage + 2 * C::TILE * C::ROW + C::TILE * C::PROW;
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          load_params<C>(vp[m][h], params + (16 * m + lane / 4 + 8 * h) * C::PROW);
+          steps[m][h] = kLeast;
+#pragma unroll
+          for (int g = 0; g < C::NG; ++g) steps[m][h] = fmaxf(steps[m][h], step_of<T>(vp[m][h][g]));
+          widest = fmaxf(widest, steps[m][h]);
+        }
+      if constexpr (MASKED) {
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            wide[n][c] = kLeast;
+#pragma unroll
+            for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                if (seen[m][n][2 * h + c]) wide[n][c] = fmaxf(wide[n][c], steps[m][h]);
+          }
+      }
+    }
+    bool need = false;
+#pragma unroll
+    for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        if (!MASKED || C::BITS == 16) wide[n][c] = widest;
+        float weight = 0.f;
+#pragma unroll
+        for (int m = 0; m < C::MT; ++m) weight = fmaxf(weight, fmaxf(p[m][n][c], p[m][n][c + 2]));
+        need = need || too_large(weight, wide[n][c], ref[n][c]);
+      }
+    if (__any_sync(0xffffffffu, need)) raise(x, p, wide);
+#pragma unroll
+    for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m) {
+        l[n][0] += p[m][n][0] + p[m][n][2];
+        l[n][1] += p[m][n][1] + p[m][n][3];
+      }
+    const uint8_t* v = stage + C::TILE * C::ROW;
+    const uint32_t v_at = smem_addr(v);
+    if constexpr (C::BITS == 16) {
+      bool clean = true;
+      if constexpr (MASKED) {
+        constexpr uint32_t E = C::DT == PBS_BF16 ? 0x7f80u : 0x7c00u;
+        for (int i = lane; i < C::TILE * C::CH; i += 32) {
+          const uint4 w = *reinterpret_cast<const uint4*>(v + 16 * i);
+          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) clean = clean && (u[e] & E) != E && ((u[e] >> 16) & E) != E;
+        }
+        clean = __all_sync(0xffffffffu, clean);
+      }
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m) {
+        uint32_t b[C::NT][2];
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) b[n][h] = transpose8(pack<T>(p[m][n][2 * h], p[m][n][2 * h + 1]));
+#pragma unroll
+        for (int i = 0; i < C::D / 16; ++i) {
+          uint32_t r[4];
+          load_matrices_t(r, v_at + piece<C>(16 * m + (lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)));
+          if constexpr (MASKED) {
+            if (!clean) {
+              constexpr uint32_t E = C::DT == PBS_BF16 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if ((r[e] & E) == E) r[e] &= 0xffff0000u;
+                if (((r[e] >> 16) & E) == E) r[e] &= 0xffffu;
+              }
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < C::NT; ++n) mma<C::DT>(o[i][n], r[0], r[1], r[2], r[3], b[n][0], b[n][1]);
+        }
+      }
+      if constexpr (MASKED) {
+        if (!clean) add_not_finite(v, t0);
+      }
+    } else {
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m) {
+        uint32_t b[C::NT][2];
+#pragma unroll
+        for (int j2 = 0; j2 < C::CH / 2; ++j2) {
+          uint32_t r[4];
+          load_matrices_t(r, v_at + piece<C>(16 * m + (lane & 15), 2 * j2 + (lane >> 4)));
+#pragma unroll
+          for (int jj = 0; jj < 2; ++jj) {
+            const int j = 2 * j2 + jj;
+            if (j * 32 % C::G == 0) {                              // a group's weights
+              const int g = j * 32 / C::G;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float s = step_of<T>(vp[m][h][g]), low = low_of<T>(vp[m][h][g]);
+#pragma unroll
+                for (int n = 0; n < C::NT; ++n) {
+                  // a weight of 0 must not meet a step or minimum that is not finite, of a token that this query does not see
+                  const float p0 = p[m][n][2 * h], p1 = p[m][n][2 * h + 1];
+                  const bool s0 = !MASKED || seen[m][n][2 * h], s1 = !MASKED || seen[m][n][2 * h + 1];
+                  om[g][n][0] = s0 ? fmaf(p0, low, om[g][n][0]) : om[g][n][0];
+                  om[g][n][1] = s1 ? fmaf(p1, low, om[g][n][1]) : om[g][n][1];
+                  // rounded to fp16, 11 bits: the codes have 4, the result 8 or 11
+                  b[n][h] = transpose8(pack_half(s0 ? p0 * s : 0.f, s1 ? p1 * s : 0.f));
+                }
+              }
+            }
+            const uint32_t y = r[2 * jj], z = r[2 * jj + 1], y8 = y >> 8, z8 = z >> 8;
+            constexpr uint32_t M0 = 0x000f000fu, M1 = 0x00f000f0u;
+#pragma unroll
+            for (int n = 0; n < C::NT; ++n) {
+              mma<PBS_FP16>(o[2 * j][n], y & M0, y & M1, z & M0, z & M1, b[n][0], b[n][1]);
+              mma<PBS_FP16>(o[2 * j + 1][n], y8 & M0, y8 & M1, z8 & M0, z8 & M1, b[n][0], b[n][1]);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // Sums, reference and weights' sum of this warp's tokens to shared memory, query by query.
+  __device__ __forceinline__ void put(float* sums, float* refs, float* weights) {
+#pragma unroll
+    for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int col = 8 * n + 2 * (lane % 4) + c;
+#pragma unroll
+        for (int s = 4; s < 32; s <<= 1) {
+          l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], s);
+          if constexpr (C::BITS == 4) {
+#pragma unroll
+            for (int g = 0; g < C::NG; ++g) om[g][n][c] += __shfl_xor_sync(0xffffffffu, om[g][n][c], s);
+          }
+        }
+        if (lane < 4) {
+          refs[col] = ref[n][c];
+          weights[col] = l[n][c];
+        }
+        float* row = sums + col * C::OROW;
+        if constexpr (C::BITS == 4) {
+#pragma unroll
+          for (int j = 0; j < C::CH; ++j) {
+            const float low = om[j * 32 / C::G][n][c];
+            *reinterpret_cast<float4*>(row + 32 * j + 4 * (lane / 4)) =
+                make_float4(fmaf(o[2 * j][n][c], 0x1p24f, low), fmaf(o[2 * j][n][c + 2], 0x1p20f, low),
+                            fmaf(o[2 * j + 1][n][c], 0x1p24f, low), fmaf(o[2 * j + 1][n][c + 2], 0x1p20f, low));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < C::D / 16; ++i) {
+            row[16 * i + lane / 4] = o[i][n][c];
+            row[16 * i + lane / 4 + 8] = o[i][n][c + 2];
+          }
+        }
+      }
+  }
+};
+
+// The part of an item that a CTA works on.
+struct Item {
+  int seq, head, row0;                                             // row = new token * group + query head within the KV head
+  int len, full, n;                                                // tokens of the sequence that its row of the table holds, all of them, new ones
+  int first, end;                                                  // tokens that the first of the rows sees, and the last
+};
+
+// Brings the queries of an item into the order of the product's second operand (in 4 bits scaled by a power of two to a maximum in
+// [2^14, 2^15), which fp16 holds to 2^-38 of it), and what belongs to each.
+template <class C>
+__device__ __forceinline__ void load_queries(const AttnArgs& p, const Item& it, uint8_t* frag, float* qsum, float* factor, int* limit) {
+  using T = typename C::T;
+  constexpr int PIECES = C::D / 8;
+  for (int e = threadIdx.x; e < C::COLS * PIECES; e += C::THREADS) {
+    const int col = e / PIECES, pc = e % PIECES, r = it.row0 + col, i = r / p.group;
+    const bool valid = i < it.n;
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (valid) raw = *reinterpret_cast<const uint4*>((const T*)p.q.p + it.seq * p.q.st.b + (it.head * p.group + r % p.group) * p.q.st.h + i * p.q.st.s + 8 * pc);
+    float f = p.scale;
+    if constexpr (C::BITS == 16) {
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        *reinterpret_cast<uint32_t*>(frag + (((pc / 4) * C::NT + col / 8) * 32 + (col % 8) * 4 + t) * 16 + (pc / 2 % 2 * 2 + pc % 2) * 4) = w[t];
+    } else {
+      const T* raw8 = reinterpret_cast<const T*>(&raw);
+      float x[8], most = 0.f, sum = 0.f;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        x[t] = Elem<C::DT>::ld(raw8 + t);
+        most = fmaxf(most, fabsf(x[t]));
+      }
+#pragma unroll
+      for (int s = PIECES / 2; s > 0; s >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
+      // most = 2^e * [1, 2): scaled by 2^k, k = 14 - e, kept where 2^k and the factor 2^(24 - k) are ordinary numbers
+      int k = most > 0.f ? 14 - ((int)(__float_as_uint(most) >> 23) - 127) : 0;
+      k = min(max(k, -90), 120);
+      const float up = __uint_as_float((uint32_t)(k + 127) << 23);
+      f *= __uint_as_float((uint32_t)(24 - k + 127) << 23);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        x[t] = __half2float(__float2half_rn(x[t] * up));
+        sum += x[t];
+      }
+#pragma unroll
+      for (int s = C::G / 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+      if (pc % (C::G / 8) == 0) qsum[pc / (C::G / 8) * C::COLS + col] = sum * 0x1p-24f;
+      // codes i and i + 4 of a word meet in one register; those of bits 4-7 are 16 times too large
+      *reinterpret_cast<uint4*>(frag + (((pc / 4) * C::NT + col / 8) * 32 + (col % 8) * 4 + pc % 4) * 16) =
+          make_uint4(pack_half(x[0], x[4]), pack_half(x[1] * 0.0625f, x[5] * 0.0625f), pack_half(x[2], x[6]), pack_half(x[3] * 0.0625f, x[7] * 0.0625f));
+    }
+    if (pc == 0) {
+      factor[col] = f;
+      limit[col] = valid ? max(0, min(it.len, it.full - it.n + i + 1)) : INT_MAX;
+    }
+  }
+}
+
+template <class C>
+__global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __grid_constant__ AttnArgs p) {
+  using T = typename C::T;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* frag = smem + C::POOL;
+  float* qsum = reinterpret_cast<float*>(frag + C::QFRAG);
+  float* factor = qsum + C::COLS * C::NG;
+  int* limit = reinterpret_cast<int*>(factor + C::COLS);
+  int* prefix = limit + C::COLS;                                   // units before sequence b
+  __shared__ int scan[C::WARPS];
+  __shared__ int is_last;
+  const pbs_paged_cache_t& c = p.a.c;
+  const pbs_paged_batch_t& bt = p.a.b;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int table_tokens = bt.max_pages << p.a.shift;
+
+  // units of all sequences (an empty one has a unit too: its rows are written)
+  const int per = p.row_tiles * c.kv_heads;
+  int total = 0;
+  for (int b0 = 0; b0 < bt.batch; b0 += C::THREADS) {
+    const int b = b0 + tid;
+    int u = 0;
+    if (b < bt.batch) {
+      const int len = bt.seq_lens[b];
+      if (len > table_tokens) paged_fault(p.a, PBS_PAGED_BAD_LENGTH);
+      u = max(1, (max(0, min(len, table_tokens)) + C::UNIT - 1) / C::UNIT) * per;
+    }
+    int sum = u;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, sum, s);
+      if (lane >= s) sum += y;
+    }
+    if (lane == 31) scan[warp] = sum;
+    __syncthreads();
+    int before = total;
+#pragma unroll
+    for (int w = 0; w < C::WARPS; ++w) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+    }
+    if (b < bt.batch) prefix[b] = before + sum - u;
+    __syncthreads();
+  }
+  const int share = (total + gridDim.x - 1) / gridDim.x;
+  int unit = min(total, (int)blockIdx.x * share);
+  const int unit_end = min(total, unit + share);
+
+  Warp<C> w;
+  w.lane = lane;
+  w.qf = reinterpret_cast<const uint4*>(frag) + lane;
+  w.qsum = qsum;
+  w.factor = factor;
+  w.limit = limit;
+  uint8_t* const ring = smem + warp * C::STAGES * C::STAGE;
+
+  while (unit < unit_end) {
+    // the item of this unit
+    int lo = 0, hi = bt.batch - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (prefix[mid] <= unit) lo = mid;
+      else hi = mid - 1;
+    }
+    Item it;
+    it.seq = lo;
+    it.full = bt.seq_lens[lo];
+    it.len = max(0, min(it.full, table_tokens));
+    const int units = max(1, (it.len + C::UNIT - 1) / C::UNIT);
+    const int within = unit - prefix[lo], index = within / units, start = within % units;
+    const int item_first = unit - start, item_end = item_first + units, stop = min(unit_end, item_end);
+    it.head = index % c.kv_heads;
+    it.row0 = index / c.kv_heads * C::COLS;
+    it.n = bt.new_lens ? min(max(bt.new_lens[lo], 0), bt.new_tokens) : bt.new_tokens;
+    {
+      const int i0 = it.row0 / p.group, i1 = min((it.row0 + C::COLS - 1) / p.group, it.n - 1);
+      it.first = max(0, min(it.len, it.full - it.n + i0 + 1));
+      it.end = i0 <= i1 ? max(0, min(it.len, it.full - it.n + i1 + 1)) : 0;
+    }
+    const int tok0 = start * C::UNIT, tok1 = min(it.end, (start + stop - unit) * C::UNIT);
+    const int tiles = tok1 > tok0 ? (tok1 - tok0 + C::TILE - 1) / C::TILE : 0;
+    const int mine = max(0, (tiles - warp + C::WARPS - 1) / C::WARPS);
+
+    const uint8_t* const kb = (const uint8_t*)c.k + it.head * c.k_strides[1] * (C::BITS == 16 ? 2 : 1);
+    const uint8_t* const vb = (const uint8_t*)c.v + it.head * c.v_strides[1] * (C::BITS == 16 ? 2 : 1);
+    const int* const table = bt.block_table + it.seq * bt.table_stride;
+    int page[C::MT];
+    uint32_t holes = 0;                                            // 16 tokens without a page: bit (tile % STAGES) * MT + m
+    auto fetch = [&](int i) {                                      // pages of this warp's tile i
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m) {
+        const int t = tok0 + (i * C::WARPS + warp) * C::TILE + 16 * m;
+        page[m] = -1;
+        if (i < mine && t < tok1) {
+          const int x = table[t >> p.a.shift];
+          if ((unsigned)x < (unsigned)c.num_pages) page[m] = x;
+          else paged_fault(p.a, PBS_PAGED_BAD_PAGE);
+        }
+      }
+    };
+    auto issue = [&](int i) {                                      // its copies, of the pages fetched last
+      const int t0 = tok0 + (i * C::WARPS + warp) * C::TILE;
+      uint8_t* const stage = ring + i % C::STAGES * C::STAGE;
+      const uint32_t at = smem_addr(stage);
+      constexpr int ES = C::BITS == 16 ? 2 : 1;
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m) {
+        const int t = t0 + 16 * m;
+        const bool there = page[m] >= 0;
+        const uint32_t hole = 1u << (i % C::STAGES * C::MT + m);
+        holes = there ? holes & ~hole : holes | hole;
+        const int64_t pg = there ? page[m] : 0;
+        const int slot = t & (c.page_size - 1);
+#pragma unroll
+        for (int s = 0; s < C::CH / 2; ++s) {
+          const int row = lane / C::CH + s * (32 / C::CH), ch = lane % C::CH;
+          const bool copy = there && t + row < tok1;
+          const int64_t r = copy ? slot + row : 0;
+          const int dst = piece<C>(16 * m + row, ch);
+          copy_async<16>(at + dst, kb + (pg * c.k_strides[0] + r * c.k_strides[2]) * ES + 16 * ch, copy);
+          copy_async<16>(at + C::TILE * C::ROW + dst, vb + (pg * c.v_strides[0] + r * c.v_strides[2]) * ES + 16 * ch, copy);
+        }
+      }
+      if constexpr (C::BITS == 4) {
+        constexpr int N = C::PROW < 16 ? C::PROW : 16;
+        const int row = lane % C::TILE, m = row / 16, t = t0 + row;
+        const int pgm = C::MT == 2 && m ? page[C::MT - 1] : page[0];
+        const bool copy = pgm >= 0 && t < tok1;
+        const int64_t pg = copy ? pgm : 0, slot = copy ? t & (c.page_size - 1) : 0;
+        const uint32_t dst = at + 2 * C::TILE * C::ROW + row * C::PROW;
+        const uint8_t* ks = (const uint8_t*)c.k_params + 2 * (pg * c.k_params_strides[0] + it.head * c.k_params_strides[1] + slot * c.k_params_strides[2]);
+        const uint8_t* vs = (const uint8_t*)c.v_params + 2 * (pg * c.v_params_strides[0] + it.head * c.v_params_strides[1] + slot * c.v_params_strides[2]);
+#pragma unroll
+        for (int o = 0; o < C::PROW; o += N) {
+          if (C::TILE == 32 || lane < 16) copy_async<N>(dst + o, ks + o, copy);
+          if (C::TILE == 32 || lane >= 16) copy_async<N>(dst + C::TILE * C::PROW + o, vs + o, copy);
+        }
+      }
+    };
+    fetch(0);
+#pragma unroll
+    for (int s = 0; s < C::STAGES - 1; ++s) {
+      if (s < mine) issue(s);
+      fetch(s + 1);
+      copy_commit();
+    }
+    load_queries<C>(p, it, frag, qsum, factor, limit);
+    w.start();
+    __syncthreads();
+    for (int i = 0; i < mine; ++i) {
+      copy_wait<C::STAGES - 2>();
+      __syncwarp();
+      if (i + C::STAGES - 1 < mine) issue(i + C::STAGES - 1);
+      fetch(i + C::STAGES);
+      copy_commit();
+      const int t0 = tok0 + (i * C::WARPS + warp) * C::TILE;
+      const uint8_t* stage = ring + i % C::STAGES * C::STAGE;
+      const uint32_t hole = holes >> (i % C::STAGES * C::MT) & ((1u << C::MT) - 1);
+      if (t0 + C::TILE > min(it.first, tok1) || hole) w.template tile<true>(stage, t0, hole);
+      else w.template tile<false>(stage, t0, 0);
+    }
+    copy_wait<0>();
+    __syncthreads();                                               // the ring is free: partial sums take its place
+    float* sums = reinterpret_cast<float*>(smem);
+    float* refs = sums + C::WARPS * C::COLS * C::OROW;
+    float* weights = refs + C::WARPS * C::COLS;
+    w.put(sums + warp * C::COLS * C::OROW, refs + warp * C::COLS, weights + warp * C::COLS);
+    __syncthreads();
+
+    const int cols = min(C::COLS, bt.new_tokens * p.group - it.row0);
+    auto write = [&](int col, int d, float4 x, float sum) {        // a piece of a row of the result
+      const int r = it.row0 + col, i = r / p.group;
+      const bool empty = i >= it.n || sum == 0.f;
+      const float inv = empty ? 0.f : 1.f / sum;
+      uint2 y = make_uint2(pack<T>(x.x * inv, x.y * inv), pack<T>(x.z * inv, x.w * inv));
+      if (empty) y = make_uint2(0, 0);
+      *reinterpret_cast<uint2*>((T*)p.out.p + it.seq * p.out.st.b + (it.head * p.group + r % p.group) * p.out.st.h + i * p.out.st.s + d) = y;
+    };
+    constexpr int Q4 = C::D / 4;
+    constexpr int PART = C::COLS * (C::D + 2);                     // floats of a partial result
+    const int i0 = item_first / share, i1 = (item_end - 1) / share;
+    float* const part = p.partials + ((int64_t)blockIdx.x * 2 + ((int)blockIdx.x == i0)) * PART;
+    for (int e = tid; e < cols * Q4; e += C::THREADS) {
+      const int col = e / Q4, d = e % Q4 * 4;
+      float top = -CUDART_INF_F, sum = 0.f;
+#pragma unroll
+      for (int v = 0; v < C::WARPS; ++v) top = fmaxf(top, refs[v * C::COLS + col]);
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int v = 0; v < C::WARPS; ++v) {
+        const float rv = refs[v * C::COLS + col], wt = rv == top ? 1.f : exp2_fast(rv - top);
+        const float4 y = *reinterpret_cast<const float4*>(sums + (v * C::COLS + col) * C::OROW + d);
+        sum = fmaf(wt, weights[v * C::COLS + col], sum);
+        x.x = fmaf(wt, y.x, x.x);
+        x.y = fmaf(wt, y.y, x.y);
+        x.z = fmaf(wt, y.z, x.z);
+        x.w = fmaf(wt, y.w, x.w);
+      }
+      if (i0 == i1) {
+        write(col, d, x, sum);
+      } else {
+        __stcg(reinterpret_cast<float4*>(part + col * C::D + d), x);
+        if (d == 0) {
+          __stcg(part + C::COLS * C::D + col, top);
+          __stcg(part + C::COLS * (C::D + 1) + col, sum);
+        }
+      }
+    }
+    if (i0 != i1) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) is_last = atomicAdd(p.counters + i0, 1) == i1 - i0;
+      __syncthreads();
+      if (is_last) {
+        __threadfence();
+        if (tid == 0) p.counters[i0] = 0;
+        const int n = i1 - i0 + 1;
+        auto from = [&](int k) { return p.partials + ((int64_t)(i0 + k) * 2 + (k == 0)) * PART; };
+        float* tops = reinterpret_cast<float*>(smem);              // [n][COLS], then weights
+        float* lsum = tops + n * C::COLS;
+        for (int e = tid; e < n * C::COLS; e += C::THREADS) {
+          const float* f = from(e / C::COLS) + C::COLS * C::D + e % C::COLS;
+          tops[e] = __ldcg(f);
+          lsum[e] = __ldcg(f + C::COLS);
+        }
+        __syncthreads();
+        for (int col = warp; col < cols; col += C::WARPS) {        // a warp a query: weights of the parts, and their sum
+          float top = -CUDART_INF_F, sum = 0.f;
+          for (int k = lane; k < n; k += 32) top = fmaxf(top, tops[k * C::COLS + col]);
+          top = warp_max(top);
+          for (int k = lane; k < n; k += 32) {
+            const float rv = tops[k * C::COLS + col], wt = rv == top ? 1.f : exp2_fast(rv - top);
+            tops[k * C::COLS + col] = wt;
+            sum = fmaf(wt, lsum[k * C::COLS + col], sum);
+          }
+          sum = warp_sum(sum);
+          __syncwarp();
+          if (lane == 0) lsum[col] = sum;                          // (part 0's place, read already)
+        }
+        __syncthreads();
+        for (int e = tid; e < cols * Q4; e += C::THREADS) {
+          const int col = e / Q4, d = e % Q4 * 4;
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+          for (int k = 0; k < n; ++k) {
+            const float wt = tops[k * C::COLS + col];
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(from(k) + col * C::D + d));
+            x.x = fmaf(wt, y.x, x.x);
+            x.y = fmaf(wt, y.y, x.y);
+            x.z = fmaf(wt, y.z, x.z);
+            x.w = fmaf(wt, y.w, x.w);
+          }
+          write(col, d, x, lsum[col]);
+        }
+      }
+    }
+    __syncthreads();
+    unit = stop;
+  }
+}
+
+int query_tiles(const PagedArgs& a, int q_heads) {                 // NT: the narrowest that holds all queries of a KV head, or the widest
+  const int64_t rows = (int64_t)q_heads / a.c.kv_heads * a.b.new_tokens;
+  return rows <= 8 ? 1 : rows <= 16 || a.c.head_dim == 256 ? 2 : 4;
+}
+
+template <class C>
+int launch(AttnArgs p, void* workspace, bool measure, int64_t* bytes, cudaStream_t st) {
+  const int64_t rows = (int64_t)p.group * p.a.b.new_tokens;
+  p.row_tiles = (int)((rows + C::COLS - 1) / C::COLS);
+  const int64_t most = ((int64_t)p.a.b.max_pages * p.a.c.page_size / C::UNIT + 1) * p.row_tiles * p.a.c.kv_heads * p.a.b.batch;
+  if (most > INT_MAX) { set_error("paged attention: sequences x heads x tokens beyond what a call can count"); return PBS_ERR_SHAPE; }
+  int grid = C::OCC * device_sms();
+  grid = grid < 2 * 148 ? grid : 2 * 148;
+  grid = grid < kMaxGrid ? grid : kMaxGrid;
+  if (most < grid) grid = (int)most;
+  if (measure) {
+    *bytes = PBS_PAGED_COUNTER_BYTES + (int64_t)grid * 2 * C::COLS * (C::D + 2) * 4;
+    return PBS_OK;
+  }
+  const int bytes_smem = C::FIXED + p.a.b.batch * 4;
+  p.counters = (int*)workspace;
+  p.partials = (float*)((uint8_t*)workspace + PBS_PAGED_COUNTER_BYTES);
+  const cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes_smem);
+  if (e != cudaSuccess) return cuda_fail(e, "paged_attn_kernel shared memory");
+  paged_attn_kernel<C><<<grid, C::THREADS, bytes_smem, st>>>(p);
   PBS_CUDA_CHECK_LAUNCH("paged_attn_kernel");
   return PBS_OK;
 }
 
+template <int DT, int D, int BITS, int G>
+int by_queries(const AttnArgs& p, void* w, bool measure, int64_t* bytes, cudaStream_t st) {
+  const int nt = query_tiles(p.a, p.q_heads);
+  if (nt == 1) return launch<Cfg<DT, D, BITS, G, 1>>(p, w, measure, bytes, st);
+  if constexpr (D != 256)
+    if (nt == 4) return launch<Cfg<DT, D, BITS, G, 4>>(p, w, measure, bytes, st);
+  return launch<Cfg<DT, D, BITS, G, 2>>(p, w, measure, bytes, st);
+}
+
+template <int DT, int D>
+int by_bits(const AttnArgs& p, void* w, bool measure, int64_t* bytes, cudaStream_t st) {
+  if (p.a.c.bits == 16) return by_queries<DT, D, 16, D>(p, w, measure, bytes, st);
+  return p.a.c.group_size == 32 ? by_queries<DT, D, 4, 32>(p, w, measure, bytes, st) : by_queries<DT, D, 4, 64>(p, w, measure, bytes, st);
+}
+
 template <int DT>
-int by_dim(const AttnArgs& p, cudaStream_t st) {
-  return p.a.c.head_dim == 64 ? launch<DT, 64>(p, st) : p.a.c.head_dim == 128 ? launch<DT, 128>(p, st) : launch<DT, 256>(p, st);
+int by_dim(const AttnArgs& p, void* w, bool measure, int64_t* bytes, cudaStream_t st) {
+  return p.a.c.head_dim == 64 ? by_bits<DT, 64>(p, w, measure, bytes, st)
+         : p.a.c.head_dim == 128 ? by_bits<DT, 128>(p, w, measure, bytes, st) : by_bits<DT, 256>(p, w, measure, bytes, st);
+}
+
+int by_type(const AttnArgs& p, void* w, bool measure, int64_t* bytes, cudaStream_t st) {
+  return p.a.c.dtype == PBS_BF16 ? by_dim<PBS_BF16>(p, w, measure, bytes, st) : by_dim<PBS_FP16>(p, w, measure, bytes, st);
 }
 
 }  // namespace
 
-int64_t paged_attn_workspace(const PagedArgs&, int) { return PBS_PAGED_COUNTER_BYTES; }
+int paged_attn_workspace(const PagedArgs& a, int q_heads, int64_t* bytes) {
+  AttnArgs p{};
+  p.a = a;
+  p.q_heads = q_heads;
+  p.group = q_heads / a.c.kv_heads;
+  return by_type(p, nullptr, true, bytes, nullptr);
+}
 
-int launch_paged_attn(const PagedArgs& a, int q_heads, const RowTensor& q, const RowTensor& out, float scale, void*, cudaStream_t st) {
-  const AttnArgs p{a, q, out, q_heads, scale * 1.44269504f};
-  return a.c.dtype == PBS_BF16 ? by_dim<PBS_BF16>(p, st) : by_dim<PBS_FP16>(p, st);
+int launch_paged_attn(const PagedArgs& a, int q_heads, const RowTensor& q, const RowTensor& out, float scale, void* workspace, cudaStream_t st) {
+  AttnArgs p{};
+  p.a = a;
+  p.q = q;
+  p.out = out;
+  p.q_heads = q_heads;
+  p.group = q_heads / a.c.kv_heads;
+  p.scale = scale * 1.44269504f;
+  return by_type(p, workspace, false, nullptr, st);
 }
 
 }  // namespace pbs
