@@ -27,7 +27,7 @@ int check_paged(const pbs_paged_cache_t* c, const pbs_paged_batch_t* b, PagedArg
     set_error("batch, new_tokens and max_pages must be positive (got %d, %d, %d)", b->batch, b->new_tokens, b->max_pages);
     return PBS_ERR_SHAPE;
   }
-  if ((int64_t)b->max_pages * c->page_size > INT_MAX) { set_error("a row of the block table holds more than 2^31 tokens"); return PBS_ERR_SHAPE; }
+  if ((int64_t)b->max_pages * c->page_size > INT_MAX - (1 << 20)) { set_error("a row of the block table holds 2^31 tokens or more"); return PBS_ERR_SHAPE; }
   if (b->table_stride < 0) { set_error("block_table: negative stride"); return PBS_ERR_LAYOUT; }
   if (b->batch > 4096) { set_error("%d sequences in a call, at most 4096", b->batch); return PBS_ERR_SHAPE; }
   PBS_NONNULL(b->block_table);

@@ -61,6 +61,9 @@ struct Cfg {
 struct AttnArgs {
   PagedArgs a;
   RowTensor q, out;
+  // steps from page to page and from slot to slot: rows in 16 bytes, params in 4, so that 32 bits hold every offset in a pool
+  uint32_t k_page, k_slot, v_page, v_slot, kp_page, kp_slot, vp_page, vp_slot;
+  int dense;                                                       // a page's rows of a head lie together, its params too
   int q_heads, group, row_tiles;
   float scale;                                                     // times log2(e)
   int* counters;
@@ -79,6 +82,11 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool t
   const int n = there ? N : 0;
   if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
   else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(n) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -190,57 +198,71 @@ struct Warp {
   // Scores of the tile (times 2^-k of the query's scaling: `factor` has the rest): tot[m][n] holds tokens lane / 4 and + 8, queries 2 (lane % 4) and + 1
   __device__ __forceinline__ void scores(float (&tot)[C::MT][C::NT][4], const uint8_t* stage) const {
     const uint32_t k_at = smem_addr(stage);
+    const int row = lane & 15, half = lane >> 4;
 #pragma unroll
-    for (int m = 0; m < C::MT; ++m) {
-      float acc[C::NT][4];
+    for (int m = 0; m < C::MT; ++m)
 #pragma unroll
       for (int n = 0; n < C::NT; ++n)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tot[m][n][c] = acc[n][c] = 0.f;
-      const int row = 16 * m + (lane & 15), half = lane >> 4;
-      if constexpr (C::BITS == 16) {
+        for (int c = 0; c < 4; ++c) tot[m][n][c] = 0.f;
+    if constexpr (C::BITS == 16) {
 #pragma unroll
-        for (int ks = 0; ks < C::D / 16; ++ks) {
-          uint32_t r[4];
-          load_matrices(r, k_at + piece<C>(row, 2 * ks + half));
+      for (int ks = 0; ks < C::D / 16; ++ks) {
+        uint32_t r[C::MT][4];
+#pragma unroll
+        for (int m = 0; m < C::MT; ++m) load_matrices(r[m], k_at + piece<C>(16 * m + row, 2 * ks + half));
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n) {
+          const uint4 q = qf[(ks / 2 * C::NT + n) * 32];
+#pragma unroll
+          for (int m = 0; m < C::MT; ++m) mma<C::DT>(tot[m][n], r[m][0], r[m][1], r[m][2], r[m][3], ks % 2 ? q.z : q.x, ks % 2 ? q.w : q.y);
+        }
+      }
+    } else {
+      uint32_t kp[C::MT][2][C::NG];
+      const uint8_t* params = stage + 2 * C::TILE * C::ROW;
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) load_params<C>(kp[m][h], params + (16 * m + lane / 4 + 8 * h) * C::PROW);
+      float acc[C::MT][C::NT][4];
+#pragma unroll
+      for (int j2 = 0; j2 < C::CH / 2; ++j2) {
+        uint32_t r[C::MT][4];
+#pragma unroll
+        for (int m = 0; m < C::MT; ++m) load_matrices(r[m], k_at + piece<C>(16 * m + row, 2 * j2 + half));
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          const int j = 2 * j2 + jj;
+          if (j * 32 % C::G == 0) {
+#pragma unroll
+            for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+              for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[m][n][c] = 0.f;
+          }
+          constexpr uint32_t M0 = 0x000f000fu, M1 = 0x00f000f0u;
 #pragma unroll
           for (int n = 0; n < C::NT; ++n) {
-            const uint4 q = qf[(ks / 2 * C::NT + n) * 32];
-            mma<C::DT>(tot[m][n], r[0], r[1], r[2], r[3], ks % 2 ? q.z : q.x, ks % 2 ? q.w : q.y);
+            const uint4 q = qf[(j * C::NT + n) * 32];
+#pragma unroll
+            for (int m = 0; m < C::MT; ++m) {
+              const uint32_t x = r[m][2 * jj], y = r[m][2 * jj + 1], x8 = x >> 8, y8 = y >> 8;
+              mma<PBS_FP16>(acc[m][n], x & M0, y & M0, x & M1, y & M1, q.x, q.y);
+              mma<PBS_FP16>(acc[m][n], x8 & M0, y8 & M0, x8 & M1, y8 & M1, q.z, q.w);
+            }
           }
-        }
-      } else {
-        uint32_t kp[2][C::NG];
-        const uint8_t* params = stage + 2 * C::TILE * C::ROW;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) load_params<C>(kp[h], params + (16 * m + lane / 4 + 8 * h) * C::PROW);
-#pragma unroll
-        for (int j2 = 0; j2 < C::CH / 2; ++j2) {
-          uint32_t r[4];
-          load_matrices(r, k_at + piece<C>(row, 2 * j2 + half));
-#pragma unroll
-          for (int jj = 0; jj < 2; ++jj) {
-            const int j = 2 * j2 + jj;
-            const uint32_t x = r[2 * jj], y = r[2 * jj + 1], x8 = x >> 8, y8 = y >> 8;
-            constexpr uint32_t M0 = 0x000f000fu, M1 = 0x00f000f0u;
+          if ((j + 1) * 32 % C::G == 0) {
+            const int g = j * 32 / C::G;
 #pragma unroll
             for (int n = 0; n < C::NT; ++n) {
-              const uint4 q = qf[(j * C::NT + n) * 32];
-              mma<PBS_FP16>(acc[n], x & M0, y & M0, x & M1, y & M1, q.x, q.y);
-              mma<PBS_FP16>(acc[n], x8 & M0, y8 & M0, x8 & M1, y8 & M1, q.z, q.w);
-            }
-            if ((j + 1) * 32 % C::G == 0) {
-              const int g = j * 32 / C::G;
+              const float2 s = *reinterpret_cast<const float2*>(qsum + g * C::COLS + 8 * n + 2 * (lane % 4));
 #pragma unroll
-              for (int n = 0; n < C::NT; ++n) {
-                const float2 s = *reinterpret_cast<const float2*>(qsum + g * C::COLS + 8 * n + 2 * (lane % 4));
+              for (int m = 0; m < C::MT; ++m)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                  const float part = fmaf(low_of<T>(kp[c / 2][g]), c % 2 ? s.y : s.x, tot[m][n][c]);
-                  tot[m][n][c] = fmaf(acc[n][c], step_of<T>(kp[c / 2][g]), part);
-                  acc[n][c] = 0.f;
-                }
-              }
+                for (int c = 0; c < 4; ++c)
+                  tot[m][n][c] = fmaf(acc[m][n][c], step_of<T>(kp[m][c / 2][g]), fmaf(low_of<T>(kp[m][c / 2][g]), c % 2 ? s.y : s.x, tot[m][n][c]));
             }
           }
         }
@@ -271,8 +293,9 @@ struct Warp {
           most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
           step = fmaxf(step, __shfl_xor_sync(0xffffffffu, step, s));
         }
+        if (!(need & 0x11111111u << lane % 4)) continue;           // (whole columns of lanes agree)
         const float old = ref[n][c];
-        if ((need & 0x11111111u << lane % 4) && most > -CUDART_INF_F) ref[n][c] = fmaxf(old, most + (C::BITS == 4 ? __log2f(step) : 0.f) - 7.f);
+        if (most > -CUDART_INF_F) ref[n][c] = fmaxf(old, most + (C::BITS == 4 ? __log2f(step) : 0.f) - 7.f);
         const float keep = ref[n][c] == old ? 1.f : exp2_fast(old - ref[n][c]);
         l[n][c] *= keep;
 #pragma unroll
@@ -321,13 +344,13 @@ struct Warp {
       for (int m = 0; m < C::MT; ++m)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          x[m][n][c] *= c % 2 ? f.y : f.x;
           if (MASKED) {
+            x[m][n][c] *= c % 2 ? f.y : f.x;
             seen[m][n][c] = t0 + 16 * m + lane / 4 + c / 2 * 8 < (c % 2 ? lim.y : lim.x) && !(hole >> m & 1);
             if (!seen[m][n][c]) x[m][n][c] = -CUDART_INF_F;
             p[m][n][c] = seen[m][n][c] ? exp2_fast(x[m][n][c] - ref[n][c % 2]) : 0.f;
           } else {
-            p[m][n][c] = exp2_fast(x[m][n][c] - ref[n][c % 2]);
+            p[m][n][c] = exp2_fast(fmaf(x[m][n][c], c % 2 ? f.y : f.x, -ref[n][c % 2]));
           }
         }
     }
@@ -374,7 +397,19 @@ struct Warp {
         for (int m = 0; m < C::MT; ++m) weight = fmaxf(weight, fmaxf(p[m][n][c], p[m][n][c + 2]));
         need = need || too_large(weight, wide[n][c], ref[n][c]);
       }
-    if (__any_sync(0xffffffffu, need)) raise(x, p, wide);
+    if (__any_sync(0xffffffffu, need)) {
+      if (!MASKED) {
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n) {
+          const float2 f = *reinterpret_cast<const float2*>(factor + 8 * n + 2 * (lane % 4));
+#pragma unroll
+          for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x[m][n][c] *= c % 2 ? f.y : f.x;
+        }
+      }
+      raise(x, p, wide);
+    }
 #pragma unroll
     for (int n = 0; n < C::NT; ++n)
 #pragma unroll
@@ -452,12 +487,14 @@ struct Warp {
                 }
               }
             }
-            const uint32_t y = r[2 * jj], z = r[2 * jj + 1], y8 = y >> 8, z8 = z >> 8;
-            constexpr uint32_t M0 = 0x000f000fu, M1 = 0x00f000f0u;
+            // rows of the product: the low code of a byte, and the byte (low + 16 high, eight bits that fp16 holds as well): four
+            // operations for eight codes, where masking the high ones out takes five
+            constexpr uint32_t M0 = 0x000f000fu, M = 0x00ff00ffu;
+            const uint32_t y = r[2 * jj] & M, z = r[2 * jj + 1] & M, y8 = __byte_perm(r[2 * jj], 0, 0x4341), z8 = __byte_perm(r[2 * jj + 1], 0, 0x4341);
 #pragma unroll
             for (int n = 0; n < C::NT; ++n) {
-              mma<PBS_FP16>(o[2 * j][n], y & M0, y & M1, z & M0, z & M1, b[n][0], b[n][1]);
-              mma<PBS_FP16>(o[2 * j + 1][n], y8 & M0, y8 & M1, z8 & M0, z8 & M1, b[n][0], b[n][1]);
+              mma<PBS_FP16>(o[2 * j][n], y & M0, y, z & M0, z, b[n][0], b[n][1]);
+              mma<PBS_FP16>(o[2 * j + 1][n], y8 & M0, y8, z8 & M0, z8, b[n][0], b[n][1]);
             }
           }
         }
@@ -490,8 +527,8 @@ struct Warp {
           for (int j = 0; j < C::CH; ++j) {
             const float low = om[j * 32 / C::G][n][c];
             *reinterpret_cast<float4*>(row + 32 * j + 4 * (lane / 4)) =
-                make_float4(fmaf(o[2 * j][n][c], 0x1p24f, low), fmaf(o[2 * j][n][c + 2], 0x1p20f, low),
-                            fmaf(o[2 * j + 1][n][c], 0x1p24f, low), fmaf(o[2 * j + 1][n][c + 2], 0x1p20f, low));
+                make_float4(fmaf(o[2 * j][n][c], 0x1p24f, low), fmaf(o[2 * j][n][c + 2] - o[2 * j][n][c], 0x1p20f, low),
+                            fmaf(o[2 * j + 1][n][c], 0x1p24f, low), fmaf(o[2 * j + 1][n][c + 2] - o[2 * j + 1][n][c], 0x1p20f, low));
           }
         } else {
 #pragma unroll
@@ -617,6 +654,7 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
   w.factor = factor;
   w.limit = limit;
   uint8_t* const ring = smem + warp * C::STAGES * C::STAGE;
+  const uint32_t ring_at = smem_addr(ring);
 
   while (unit < unit_end) {
     // the item of this unit
@@ -645,55 +683,80 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
     const int tiles = tok1 > tok0 ? (tok1 - tok0 + C::TILE - 1) / C::TILE : 0;
     const int mine = max(0, (tiles - warp + C::WARPS - 1) / C::WARPS);
 
-    const uint8_t* const kb = (const uint8_t*)c.k + it.head * c.k_strides[1] * (C::BITS == 16 ? 2 : 1);
-    const uint8_t* const vb = (const uint8_t*)c.v + it.head * c.v_strides[1] * (C::BITS == 16 ? 2 : 1);
+    constexpr int ES = C::BITS == 16 ? 2 : 1;
+    const uint8_t* const kb = (const uint8_t*)c.k + it.head * c.k_strides[1] * ES + lane % C::CH * 16;
+    const uint8_t* const vb = (const uint8_t*)c.v + it.head * c.v_strides[1] * ES + lane % C::CH * 16;
+    const uint8_t* const kpb = (const uint8_t*)c.k_params + 2 * it.head * c.k_params_strides[1];
+    const uint8_t* const vpb = (const uint8_t*)c.v_params + 2 * it.head * c.v_params_strides[1];
     const int* const table = bt.block_table + it.seq * bt.table_stride;
     int page[C::MT];
-    uint32_t holes = 0;                                            // 16 tokens without a page: bit (tile % STAGES) * MT + m
-    auto fetch = [&](int i) {                                      // pages of this warp's tile i
-#pragma unroll
-      for (int m = 0; m < C::MT; ++m) {
-        const int t = tok0 + (i * C::WARPS + warp) * C::TILE + 16 * m;
-        page[m] = -1;
-        if (i < mine && t < tok1) {
-          const int x = table[t >> p.a.shift];
-          if ((unsigned)x < (unsigned)c.num_pages) page[m] = x;
-          else paged_fault(p.a, PBS_PAGED_BAD_PAGE);
-        }
-      }
+    uint32_t holes = 0;                                            // 16 tokens without a page: bit (place in the ring) * MT + m
+    int next = tok0 + warp * C::TILE;                              // first token of the tile whose pages are fetched next
+    auto lookup = [&](int t) {
+      if (t >= tok1) return -1;
+      const int x = table[t >> p.a.shift];
+      if ((unsigned)x < (unsigned)c.num_pages) return x;
+      paged_fault(p.a, PBS_PAGED_BAD_PAGE);
+      return -1;
     };
-    auto issue = [&](int i) {                                      // its copies, of the pages fetched last
-      const int t0 = tok0 + (i * C::WARPS + warp) * C::TILE;
-      uint8_t* const stage = ring + i % C::STAGES * C::STAGE;
-      const uint32_t at = smem_addr(stage);
-      constexpr int ES = C::BITS == 16 ? 2 : 1;
+    auto fetch = [&] {                                             // pages of the next tile
+      page[0] = lookup(next);
+      if constexpr (C::MT == 2) page[1] = p.a.shift > 4 ? page[0] : lookup(next + 16);   // (tiles start at multiples of 32)
+      next += C::UNIT;
+    };
+    auto issue = [&](int slot) {                                   // its copies, to this place in the ring, once its pages are here
+      const int t0 = next - C::UNIT;
+      const uint32_t at = ring_at + slot * C::STAGE;
+      if (p.dense && t0 + C::TILE <= tok1 && page[0] >= 0 && page[C::MT - 1] >= 0) {
+        // the common case, whose copies are a few constants away from one another: half the instructions of the one below
+        holes &= ~(((1u << C::MT) - 1) << slot * C::MT);
+#pragma unroll
+        for (int m = 0; m < C::MT; ++m) {
+          const uint32_t sl = (t0 + 16 * m) & (c.page_size - 1);
+          const uint8_t* const ks = kb + 16 * (uint64_t)(page[m] * p.k_page + sl * (uint32_t)C::CH + lane / C::CH * C::CH);
+          const uint8_t* const vs = vb + 16 * (uint64_t)(page[m] * p.v_page + sl * (uint32_t)C::CH + lane / C::CH * C::CH);
+#pragma unroll
+          for (int s = 0; s < C::CH / 2; ++s) {
+            const int dst = piece<C>(16 * m + lane / C::CH + s * (32 / C::CH), lane % C::CH);
+            copy_async<16>(at + dst, ks + s * 512);
+            copy_async<16>(at + C::TILE * C::ROW + dst, vs + s * 512);
+          }
+        }
+        if constexpr (C::BITS == 4) {
+          constexpr int N = C::PROW < 16 ? C::PROW : 16;
+          const int row = lane % C::TILE, pg = C::MT == 2 && row >= 16 ? page[C::MT - 1] : page[0];
+          const uint32_t sl = (t0 + row) & (c.page_size - 1), dst = at + 2 * C::TILE * C::ROW + row * C::PROW;
+          const uint8_t* const ks = kpb + 4 * (uint64_t)(pg * p.kp_page + sl * (uint32_t)C::NG);
+          const uint8_t* const vs = vpb + 4 * (uint64_t)(pg * p.vp_page + sl * (uint32_t)C::NG);
+#pragma unroll
+          for (int o = 0; o < C::PROW; o += N) {
+            if (C::TILE == 32 || lane < 16) copy_async<N>(dst + o, ks + o);
+            if (C::TILE == 32 || lane >= 16) copy_async<N>(dst + C::TILE * C::PROW + o, vs + o);
+          }
+        }
+        return;
+      }
 #pragma unroll
       for (int m = 0; m < C::MT; ++m) {
-        const int t = t0 + 16 * m;
         const bool there = page[m] >= 0;
-        const uint32_t hole = 1u << (i % C::STAGES * C::MT + m);
+        const uint32_t hole = 1u << (slot * C::MT + m), pg = there ? page[m] : 0, sl = (t0 + 16 * m) & (c.page_size - 1);
         holes = there ? holes & ~hole : holes | hole;
-        const int64_t pg = there ? page[m] : 0;
-        const int slot = t & (c.page_size - 1);
+        const int rows = there ? tok1 - t0 - 16 * m : 0;           // (offsets stay within the page also for those that are only filled)
+        const uint32_t ko = pg * p.k_page + (sl + lane / C::CH) * p.k_slot, vo = pg * p.v_page + (sl + lane / C::CH) * p.v_slot;
 #pragma unroll
         for (int s = 0; s < C::CH / 2; ++s) {
-          const int row = lane / C::CH + s * (32 / C::CH), ch = lane % C::CH;
-          const bool copy = there && t + row < tok1;
-          const int64_t r = copy ? slot + row : 0;
-          const int dst = piece<C>(16 * m + row, ch);
-          copy_async<16>(at + dst, kb + (pg * c.k_strides[0] + r * c.k_strides[2]) * ES + 16 * ch, copy);
-          copy_async<16>(at + C::TILE * C::ROW + dst, vb + (pg * c.v_strides[0] + r * c.v_strides[2]) * ES + 16 * ch, copy);
+          const int row = lane / C::CH + s * (32 / C::CH), dst = piece<C>(16 * m + row, lane % C::CH);
+          copy_async<16>(at + dst, kb + 16 * (uint64_t)(ko + s * (32 / C::CH) * p.k_slot), row < rows);
+          copy_async<16>(at + C::TILE * C::ROW + dst, vb + 16 * (uint64_t)(vo + s * (32 / C::CH) * p.v_slot), row < rows);
         }
       }
       if constexpr (C::BITS == 4) {
         constexpr int N = C::PROW < 16 ? C::PROW : 16;
-        const int row = lane % C::TILE, m = row / 16, t = t0 + row;
-        const int pgm = C::MT == 2 && m ? page[C::MT - 1] : page[0];
-        const bool copy = pgm >= 0 && t < tok1;
-        const int64_t pg = copy ? pgm : 0, slot = copy ? t & (c.page_size - 1) : 0;
-        const uint32_t dst = at + 2 * C::TILE * C::ROW + row * C::PROW;
-        const uint8_t* ks = (const uint8_t*)c.k_params + 2 * (pg * c.k_params_strides[0] + it.head * c.k_params_strides[1] + slot * c.k_params_strides[2]);
-        const uint8_t* vs = (const uint8_t*)c.v_params + 2 * (pg * c.v_params_strides[0] + it.head * c.v_params_strides[1] + slot * c.v_params_strides[2]);
+        const int row = lane % C::TILE, pgm = C::MT == 2 && row >= 16 ? page[C::MT - 1] : page[0];
+        const bool copy = pgm >= 0 && t0 + row < tok1;
+        const uint32_t pg = pgm >= 0 ? pgm : 0, sl = (t0 + row) & (c.page_size - 1), dst = at + 2 * C::TILE * C::ROW + row * C::PROW;
+        const uint8_t* const ks = kpb + 4 * (uint64_t)(pg * p.kp_page + sl * p.kp_slot);
+        const uint8_t* const vs = vpb + 4 * (uint64_t)(pg * p.vp_page + sl * p.vp_slot);
 #pragma unroll
         for (int o = 0; o < C::PROW; o += N) {
           if (C::TILE == 32 || lane < 16) copy_async<N>(dst + o, ks + o, copy);
@@ -701,27 +764,29 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
         }
       }
     };
-    fetch(0);
+    fetch();
 #pragma unroll
     for (int s = 0; s < C::STAGES - 1; ++s) {
       if (s < mine) issue(s);
-      fetch(s + 1);
+      fetch();
       copy_commit();
     }
     load_queries<C>(p, it, frag, qsum, factor, limit);
     w.start();
     __syncthreads();
-    for (int i = 0; i < mine; ++i) {
+    int slot = 0, t0 = tok0 + warp * C::TILE;
+    const int plain = min(it.first, tok1) - C::TILE;               // tiles up to here are seen whole by all queries
+    for (int i = 0; i < mine; ++i, t0 += C::UNIT) {
       copy_wait<C::STAGES - 2>();
-      __syncwarp();
-      if (i + C::STAGES - 1 < mine) issue(i + C::STAGES - 1);
-      fetch(i + C::STAGES);
+      __syncwarp();                                                // (the place read last is free in all lanes, too)
+      if (i + C::STAGES - 1 < mine) issue(slot == 0 ? C::STAGES - 1 : slot - 1);
+      fetch();
       copy_commit();
-      const int t0 = tok0 + (i * C::WARPS + warp) * C::TILE;
-      const uint8_t* stage = ring + i % C::STAGES * C::STAGE;
-      const uint32_t hole = holes >> (i % C::STAGES * C::MT) & ((1u << C::MT) - 1);
-      if (t0 + C::TILE > min(it.first, tok1) || hole) w.template tile<true>(stage, t0, hole);
+      const uint8_t* stage = ring + slot * C::STAGE;
+      const uint32_t hole = holes >> slot * C::MT & ((1u << C::MT) - 1);
+      if (t0 > plain || hole) w.template tile<true>(stage, t0, hole);
       else w.template tile<false>(stage, t0, 0);
+      slot = slot == C::STAGES - 1 ? 0 : slot + 1;
     }
     copy_wait<0>();
     __syncthreads();                                               // the ring is free: partial sums take its place
@@ -805,7 +870,7 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
         for (int e = tid; e < cols * Q4; e += C::THREADS) {
           const int col = e / Q4, d = e % Q4 * 4;
           float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 16
           for (int k = 0; k < n; ++k) {
             const float wt = tops[k * C::COLS + col];
             const float4 y = __ldcg(reinterpret_cast<const float4*>(from(k) + col * C::D + d));
@@ -842,6 +907,23 @@ int launch(AttnArgs p, void* workspace, bool measure, int64_t* bytes, cudaStream
     *bytes = PBS_PAGED_COUNTER_BYTES + (int64_t)grid * 2 * C::COLS * (C::D + 2) * 4;
     return PBS_OK;
   }
+  const pbs_paged_cache_t& c = p.a.c;
+  bool fits = true;
+  auto steps = [&](const int64_t (&st)[3], int bytes, int unit, uint32_t& page, uint32_t& slot) {
+    const int64_t a = st[0] * bytes / unit, b = st[2] * bytes / unit;
+    fits = fits && a <= UINT32_MAX && b <= UINT32_MAX && (__int128)(c.num_pages - 1) * a + (__int128)(c.page_size - 1) * b <= UINT32_MAX;
+    page = (uint32_t)a;
+    slot = (uint32_t)b;
+  };
+  p.dense = c.k_strides[2] * (C::BITS == 16 ? 2 : 1) == C::ROW && c.v_strides[2] * (C::BITS == 16 ? 2 : 1) == C::ROW &&
+            (C::BITS == 16 || (c.k_params_strides[2] == 2 * C::NG && c.v_params_strides[2] == 2 * C::NG));
+  steps(c.k_strides, C::BITS == 16 ? 2 : 1, 16, p.k_page, p.k_slot);
+  steps(c.v_strides, C::BITS == 16 ? 2 : 1, 16, p.v_page, p.v_slot);
+  if (C::BITS == 4) {
+    steps(c.k_params_strides, 2, 4, p.kp_page, p.kp_slot);
+    steps(c.v_params_strides, 2, 4, p.vp_page, p.vp_slot);
+  }
+  if (!fits) { set_error("paged attention: a pool of more than 64 GiB (params: 16 GiB)"); return PBS_ERR_SHAPE; }
   const int bytes_smem = C::FIXED + p.a.b.batch * 4;
   p.counters = (int*)workspace;
   p.partials = (float*)((uint8_t*)workspace + PBS_PAGED_COUNTER_BYTES);
