@@ -2,7 +2,7 @@
 
     python -m pbs_attn_b200.build [--force] [--verbose]
 
-Beside it pbs_host.<torch>.<python>.so, the native host side of the Python call (csrc/host_call.cpp), which fits the torch and Python
+Beside it pbs_host.<torch>.<python>.so, the native host side of the Python calls (csrc/host_*.cpp), which fits the torch and Python
 in its name alone.  Where it could not be built or was built for others calls go through Python.
 Objects and the libraries land in pbs_attn_b200/lib/ (git-ignored).  nvcc cross-compiles
 without a GPU.  The library links the static CUDA runtime only, so it also loads on a
@@ -21,7 +21,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "lib")
 LIB = os.path.join(OUT, "libpbs_b200.so")
-HOST_SRC = os.path.join(CSRC, "host_call.cpp")
+HOST_SRCS = [os.path.join(CSRC, f) for f in ("host_call.cpp", "host_decode.cpp")]
+HOST_HEADER = os.path.join(CSRC, "host_common.h")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 NVCC_FLAGS = [
@@ -62,14 +63,14 @@ def _host_command(target: str):
     includes = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
     libdir = os.path.join(os.path.dirname(torch.__file__), "lib")
     return (["g++", "-O2", "-shared", "-fPIC", "-std=c++17", "-Wno-attributes", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-            + [f for d in includes for f in ("-isystem", d)] + [HOST_SRC, "-o", target, "-L" + libdir, "-L" + os.path.join(cuda, "lib64"),
+            + [f for d in includes for f in ("-isystem", d)] + HOST_SRCS + ["-o", target, "-L" + libdir, "-L" + os.path.join(cuda, "lib64"),
                "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10", f"-l:libcudart.so.{torch.version.cuda.split('.')[0]}"])
 
 
 def _build_host(run, force: bool):
     try:
         target = host_path()
-        if force or _stale(target, [HOST_SRC, os.path.join(INCLUDE, "pbs_b200.h")]):
+        if force or _stale(target, HOST_SRCS + [HOST_HEADER, os.path.join(INCLUDE, "pbs_b200.h")]):
             for f in os.listdir(OUT):
                 if f.startswith("pbs_host."):
                     os.remove(os.path.join(OUT, f))        # for another torch or Python
@@ -80,7 +81,7 @@ def _build_host(run, force: bool):
 
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OUT, exist_ok=True)
-    headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
+    headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h")) and not f.startswith("host_")]
     headers.append(os.path.join(INCLUDE, "pbs_b200.h"))
     nvcc = _nvcc()
     jobs = []

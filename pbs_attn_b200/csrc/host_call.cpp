@@ -2,21 +2,10 @@
 // deferred status check of prefill.py, for plain CUDA tensors that the kernels can read in place and the default options.  Whatever it
 // does not cover it leaves, untouched, to the Python code (returns None), which also raises all errors.
 // A call of 187 tokens keeps the GPU busy for 14 us, and its Python took 36: here 14 (calls back to back 36.7 -> 21.5 us).
-#include <Python.h>
-
-#include <torch/csrc/autograd/python_variable.h>
-#include <ATen/PythonTorchFunctionTLS.h>
-#include <ATen/ops/empty_like.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/DynamicTypes.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/utils/object_ptr.h>
-
 #include <cstdlib>
 #include <vector>
 
-#include "../../include/pbs_b200.h"
+#include "host_common.h"
 
 namespace {
 
@@ -71,11 +60,6 @@ void sweep() {
 }
 
 void destroy(PyObject* capsule) { leaving.push_back(static_cast<Call*>(PyCapsule_GetPointer(capsule, kName))); }
-
-bool capturing(cudaStream_t st) {
-  cudaStreamCaptureStatus s;
-  return cudaStreamIsCapturing(st, &s) != cudaSuccess || s != cudaStreamCaptureStatusNone;
-}
 
 // Sends the status words of the call just enqueued to its slot of the ring.  Not those of a captured call: it is replayed at times unknown
 // here, perhaps after the plan is gone (check_status reads the device's words).  by_copy: for calls that go through Python, the
@@ -226,14 +210,6 @@ bool plain_int(PyObject* o, int64_t* v) {
   return !over && *v > 0 && *v < (1ll << 31);
 }
 
-// prefill.py's _readable
-bool readable(const at::Tensor& t, bool distinct_heads) {
-  const auto st = t.strides(), sz = t.sizes();
-  if (st[3] != 1 || st[2] <= 0 || st[0] < 0 || st[1] < 0) return false;
-  if (((st[0] | st[1] | st[2]) * t.element_size()) % 16 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
-  return !distinct_heads || ((st[0] > 0 || sz[0] == 1) && (st[1] > 0 || sz[1] == 1));
-}
-
 // A call's turn for as long as this lives, if nobody has it.
 struct TryTurn {
   Call* c;
@@ -325,4 +301,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "pbs_host", nullptr, -1, methods};
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_pbs_host(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit_pbs_host(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddFunctions(m, pbs_decode_methods) < 0) Py_CLEAR(m);
+  return m;
+}

@@ -20,6 +20,7 @@
 //
 // Within a CTA every warp takes every kWarps-th tile of 16 or 32 tokens through its own ring of cp.async stages, with its own running
 // reference and sums; warps meet once an item.
+#include <atomic>
 #include <climits>
 #include <type_traits>
 
@@ -28,7 +29,7 @@
 namespace pbs {
 namespace {
 
-constexpr int kMaxGrid = PBS_PAGED_COUNTER_BYTES / 4;
+constexpr int kMaxGrid = PBS_PAGED_COUNTER_BYTES / 4, kMaxBatch = 4096;
 
 template <int DT_, int D_, int BITS_, int G_, int NT_>
 struct Cfg {
@@ -46,7 +47,7 @@ struct Cfg {
   static constexpr int PROW = BITS == 4 ? 4 * NG : 0;
   static constexpr int STAGE = TILE * 2 * (ROW + PROW);
   static constexpr int OCC = BITS == 4 && NT == 1 && D <= 128 ? 2 : 1;       // CTAs a SM
-  static constexpr int BUDGET = (OCC == 2 ? 112 : 216) * 1024;
+  static constexpr int BUDGET = (OCC == 2 ? 112 : 200) * 1024;
   static constexpr int STAGES_FIT = BUDGET / (WARPS * STAGE);
   static constexpr int STAGES = STAGES_FIT < 2 ? 2 : STAGES_FIT > 4 ? 4 : STAGES_FIT;
   static constexpr int RING = WARPS * STAGES * STAGE;
@@ -56,6 +57,7 @@ struct Cfg {
   static constexpr int POOL = RING > MERGE ? (RING > JOIN ? RING : JOIN) : (MERGE > JOIN ? MERGE : JOIN);
   static constexpr int QFRAG = COLS * D * 2;
   static constexpr int FIXED = POOL + QFRAG + COLS * NG * 4 + COLS * 8;      // then the batch's prefix sums
+  static_assert(FIXED + kMaxBatch * 4 + 256 <= 227 * 1024, "shared memory");
 };
 
 struct AttnArgs {
@@ -927,7 +929,14 @@ int launch(AttnArgs p, void* workspace, bool measure, int64_t* bytes, cudaStream
   const int bytes_smem = C::FIXED + p.a.b.batch * 4;
   p.counters = (int*)workspace;
   p.partials = (float*)((uint8_t*)workspace + PBS_PAGED_COUNTER_BYTES);
-  const cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes_smem);
+  // the limit that holds for any batch, set once a device
+  static std::atomic<uint64_t> allowed{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !(allowed.load(std::memory_order_relaxed) >> dev & 1))) {
+    e = cudaFuncSetAttribute(paged_attn_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::FIXED + kMaxBatch * 4);
+    if (e == cudaSuccess && dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   if (e != cudaSuccess) return cuda_fail(e, "paged_attn_kernel shared memory");
   paged_attn_kernel<C><<<grid, C::THREADS, bytes_smem, st>>>(p);
   PBS_CUDA_CHECK_LAUNCH("paged_attn_kernel");

@@ -82,6 +82,8 @@ class PagedKVCache:
         self.lib = _cabi.load()
         self.bits = 4 if k.dtype == torch.uint8 else 16
         pages, heads, page_size, row = k.shape
+        if self.bits == 4 and (k_params is None or v_params is None):
+            raise ValueError("pages of 4 bits need k_params and v_params")
         self.dtype = k.dtype if self.bits == 16 else k_params.dtype
         if self.dtype not in _DTYPES:
             raise TypeError(f"unsupported dtype {self.dtype}: need bfloat16 or float16")
@@ -117,6 +119,13 @@ class PagedKVCache:
         bytes_ = C.c_int64()
         probe = _cabi.PagedBatch(16, 1, 16, None, 1, 1, 1, 0)
         _cabi.check(self.lib.pbs_paged_attn_workspace(C.byref(self._c), C.byref(probe), heads, C.byref(bytes_)), "paged cache")
+        # the common calls without Python (csrc/host_decode.cpp); None where that was not built
+        self._host, self._native = _cabi.load_host(), None
+        if self._host is not None:
+            address = lambda f: C.cast(f, C.c_void_p).value  # noqa: E731
+            lib = self.lib
+            self._native = self._host.paged_attach(C.addressof(self._c), self.device.index, address(lib.pbs_paged_append), address(lib.pbs_paged_gather),
+                                                   address(lib.pbs_paged_attn), address(lib.pbs_paged_attn_workspace))
 
     def check_status(self):
         """Synchronises and raises if a call on this device met a fault (see the module)."""
@@ -167,6 +176,10 @@ def paged_kv_append(cache: PagedKVCache, key_states: torch.Tensor, value_states:
     are (positions, D), looked up by position, or (B or 1, S, D), one row per token as a model hands them over; of the cache's
     dtype.  Without them keys are taken as they are and None is returned.  Padding rows of ``query_out`` are 0.
     One kernel on the current stream, without synchronising."""
+    if cache._native is not None:
+        done = cache._host.paged_append(cache._native, key_states, value_states, block_table, seq_lens, new_lens, cos, sin, query_states, query_out)
+        if done is not None:
+            return None if done is True else done
     B, _, S, _ = key_states.shape
     _check_rows(cache, "key_states", key_states, B, cache.kv_heads, S)
     _check_rows(cache, "value_states", value_states, B, cache.kv_heads, S)
@@ -216,6 +229,10 @@ def paged_kv_gather(cache: PagedKVCache, block_table: torch.Tensor, seq_lens: to
     """The last ``count`` tokens of each sequence (or the last ``new_lens[b]``, in the first rows) as the cache holds them: keys and values,
     (B, Hkv, count, D) of the cache's dtype, 0 where a sequence has no such token.  ``count`` = the longest sequence with ``new_lens`` =
     ``seq_lens`` reads everything."""
+    if cache._native is not None:
+        done = cache._host.paged_gather(cache._native, block_table, seq_lens, count, new_lens)
+        if done is not None:
+            return done
     B = seq_lens.shape[0]
     batch = _batch(cache, B, count, block_table, seq_lens, new_lens)
     # (B, S, H, D) memory: rows of one token lie together, as a projection's do
@@ -253,6 +270,10 @@ def paged_attn_fwd(query_states: torch.Tensor, cache: PagedKVCache, block_table:
     head h // (Hq // Hkv).  The result has the queries' shape, dtype and memory layout; rows that see no token (padding, or a sequence of
     length 0) are 0.  ``scale`` defaults to 1 / sqrt(D).  Made for one token a sequence or a few; any number works.
     One kernel on the current stream, without synchronising."""
+    if cache._native is not None:
+        done = cache._host.paged_attn(cache._native, query_states, block_table, seq_lens, new_lens, scale, out)
+        if done is not None:
+            return done
     B, Hq, S, D = query_states.shape
     _check_rows(cache, "query_states", query_states, B, None, S)
     batch = _batch(cache, B, S, block_table, seq_lens, new_lens)

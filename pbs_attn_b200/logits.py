@@ -10,6 +10,7 @@ from . import _cabi
 from .prefill import _DTYPES
 
 Penalty = Optional[Union[float, torch.Tensor]]
+_host = _address = None
 
 
 def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, token_lens: Optional[torch.Tensor] = None,
@@ -28,6 +29,14 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     whole row, no prompt).  ``tokens`` and ``bias_ids`` are int32 or int64; ids outside 0 .. V - 1 are skipped.  Penalties are
     numbers or (B,) float32 tensors.  All in 32 bits, rounded once.  Runs on the current stream without synchronising; tokens are
     counted anew in every call, so nothing has to be kept in step when rows move, leave or take back tokens."""
+    global _host, _address
+    if _host is None:
+        _host, _address = _cabi.load_host() or False, C.cast(_cabi.load().pbs_process_logits, C.c_void_p).value
+    if _host:                                              # without Python in between (csrc/host_decode.cpp), where it can be
+        done = _host.process_logits(_address, logits, tokens, token_lens, prompt_lens, repetition_penalty, frequency_penalty, presence_penalty,
+                                    bias_ids, bias_values, allowed, out)
+        if done is not None:
+            return done
     if not logits.is_cuda:
         raise RuntimeError("pbs_attn_b200 runs on CUDA devices only; there is no CPU path")
     if logits.dtype not in _DTYPES:
