@@ -55,7 +55,7 @@ int check_rows(const char* name, const PagedArgs& a, int heads, const void* p, c
 }
 
 int check_count(const PagedArgs& a, int64_t heads) {
-  if ((int64_t)a.b.batch * a.b.new_tokens * heads > INT_MAX) { set_error("more than 2^31 rows in a call"); return PBS_ERR_SHAPE; }
+  if ((int64_t)a.b.batch * a.b.new_tokens * heads > INT_MAX || heads > 65535) { set_error("more than 2^31 rows in a call, or 65535 heads"); return PBS_ERR_SHAPE; }
   return PBS_OK;
 }
 
