@@ -18,6 +18,8 @@ Under ``torch.distributed.run`` the model is tensor-parallel the way the referen
 ``down_proj`` are summed over the ranks (one NCCL all-reduce each).  Random weights need no loading, so each rank
 simply builds the architecture with its share of the heads; the attention kernels see exactly a rank's heads.
 
+``--decode N`` goes on from the prompt: N tokens through the paged cache (``generate``), whose time per token is reported.
+
 ``--parallel dp`` is multi-sequence prefill instead: every rank holds the WHOLE model and its share of a batch
 of ``--batch`` sequences (default: one per rank; ``sharding.shard_batch``), nothing is exchanged while
 computing, a step ends when the slowest rank ends.  ``--attention-share`` times the same model a second
@@ -144,6 +146,24 @@ def measure_prefill_latency(model, input_ids) -> float:
     return a.elapsed_time(b) / 1000.0
 
 
+def measure_decode(model, input_ids, tokens: int, bits: int) -> float:
+    """Milliseconds per token of ``generate``: what ``tokens`` more of them add to the time (model patched)."""
+    from .generate import generate
+
+    def seconds(n):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        torch.cuda.synchronize()
+        a.record()
+        generate(model, input_ids, n, bits=bits, repetition_penalty=1.1)
+        b.record()
+        torch.cuda.synchronize()
+        return a.elapsed_time(b) / 1000.0
+
+    seconds(4)
+    few, more = seconds(4), seconds(4 + tokens)
+    return (more - few) / tokens * 1000.0
+
+
 def last_density():
     """Selected fraction of the causal block triangle in the most recent sparse call (last layer)."""
     from . import prefill
@@ -175,6 +195,9 @@ def main(argv=None):
     ap.add_argument("--batch", type=int, default=None, help="sequences per step (data parallel: default one per rank)")
     ap.add_argument("--attention-share", action="store_true",
                     help="time the model a second time with attention replaced by a no-op and report the share")
+    ap.add_argument("--decode", type=int, default=0, metavar="N",
+                    help="also generate N tokens through the paged cache (generate.py) and report the time of one")
+    ap.add_argument("--cache-bits", type=int, default=4, choices=[4, 16], help="what the paged cache holds keys and values in")
     ap.add_argument("--out", default=None, help="append the JSON lines to this file (rank 0)")
     args = ap.parse_args(argv)
     if not torch.cuda.is_available():
@@ -188,6 +211,8 @@ def main(argv=None):
     if world > 1:
         dist.init_process_group("nccl", device_id=torch.device("cuda", local_rank))
     from .hf_patch import apply_patch_with_prefill, remove_patch
+    if args.decode and (world > 1 or args.method == "unpatched"):
+        raise SystemExit("--decode is for single-process runs of a patched model")
     if args.slice_of > 1 and world > 1:
         raise SystemExit("--slice-of is for single-process runs")
     tp = world if args.parallel == "tp" else 1
@@ -238,6 +263,11 @@ def main(argv=None):
         if "noattn" in results and args.method != "noattn":
             rest = sum(results["noattn"]) / len(results["noattn"])
             rec.update(without_attention_s=rest, attention_s=mean_s - rest, attention_share=(mean_s - rest) / mean_s)
+        if args.decode:
+            remove_patch(model)                                  # (the no-op arm came last)
+            apply_patch_with_prefill(model, prefill_function(args.method, args.block_size, args.segment_size, args.threshold))
+            rec.update(decode_tokens=args.decode, cache_bits=args.cache_bits,
+                       decode_ms_per_token=measure_decode(model, ids, args.decode, args.cache_bits))
         line = json.dumps(rec)
         print(line, flush=True)
         if args.out:

@@ -102,6 +102,17 @@ def _takes_grouped_kv(prefill_fn) -> bool:
     return kern in (permuted_block_sparse_attn_fwd, MeanPooling_prefill) or bool(getattr(kern, "takes_grouped_kv", False))
 
 
+def _grouped(prefill_fn):
+    """``prefill_fn`` as a function of queries and un-repeated keys and values."""
+    if _takes_grouped_kv(prefill_fn):
+        return prefill_fn
+
+    def call(q, k, v):
+        n_rep = max(1, q.shape[1] // k.shape[1])
+        return prefill_fn(q, repeat_kv(k, n_rep), repeat_kv(v, n_rep))
+    return call
+
+
 def patched_attention_forward(
     self,
     hidden_states: torch.Tensor,
@@ -116,10 +127,14 @@ def patched_attention_forward(
 
     Prompts (q_len > 1) go through ``prefill_fn(query, key, value)`` on (B, H, S, D) tensors after
     projection, RoPE and the KV-cache update; single-token decode goes to the layer's original
-    forward.  Head counts are derived from the projection widths, so a tensor-parallel shard works
+    forward, or with a ``PagedModelCache`` for ``past_key_values`` (``generate``) through that.  Head counts are derived from the projection widths, so a tensor-parallel shard works
     unchanged.  Returns ``(attn_output, None)``.
     """
     bsz, q_len, _ = hidden_states.size()
+    if hasattr(past_key_values, "attend"):                 # a paged cache (generate.PagedModelCache) takes prompts and single tokens
+        if prefill_fn is None:
+            raise RuntimeError("prefill_fn required.")
+        return past_key_values.attend(self, hidden_states, _grouped(prefill_fn)), None
     if q_len <= 1:
         return self.original_forward(hidden_states=hidden_states, position_embeddings=position_embeddings,
                                      attention_mask=attention_mask, past_key_values=past_key_values,
