@@ -147,21 +147,11 @@ def measure_prefill_latency(model, input_ids) -> float:
 
 
 def measure_decode(model, input_ids, tokens: int, bits: int) -> float:
-    """Milliseconds per token of ``generate``: what ``tokens`` more of them add to the time (model patched)."""
+    """Milliseconds per token of ``generate`` behind the prompt, one graph replay each (model patched)."""
     from .generate import generate
-
-    def seconds(n):
-        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-        torch.cuda.synchronize()
-        a.record()
-        generate(model, input_ids, n, bits=bits, repetition_penalty=1.1)
-        b.record()
-        torch.cuda.synchronize()
-        return a.elapsed_time(b) / 1000.0
-
-    seconds(4)
-    few, more = seconds(4), seconds(4 + tokens)
-    return (more - few) / tokens * 1000.0
+    timings = {}
+    generate(model, input_ids, tokens + 2, bits=bits, repetition_penalty=1.1, timings=timings)
+    return timings["ms_per_token"]
 
 
 def last_density():

@@ -78,14 +78,14 @@ def _run_layers(model, ids: torch.Tensor, cache: PagedModelCache) -> torch.Tenso
 def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, bits: int = 16, page_size: int = 64, group_size: int = 64,
              repetition_penalty=None, frequency_penalty=None, presence_penalty=None, bias_ids: Optional[torch.Tensor] = None,
              bias_values: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None, cuda_graph: bool = True,
-             step_logits: Optional[list] = None) -> torch.Tensor:
+             step_logits: Optional[list] = None, timings: Optional[dict] = None) -> torch.Tensor:
     """(B, S) prompts of one length -> (B, S + max_new_tokens): the token with the largest logit after penalties, biases and mask
     (the lowest of equals), step by step.
 
     ``model`` is a patched bfloat16 or float16 model with every layer patched (``apply_patch_with_prefill``).  ``bits``: what the cache
     holds keys and values in, 16 or 4.  The arguments after it are those of ``process_logits``; the history is the whole sequence, its
     prompt part the prompt.  ``cuda_graph=False`` runs every step eagerly; ``step_logits``, a list, receives each step's logits before
-    the penalties (eager steps only)."""
+    the penalties (eager steps only); ``timings``, a dict, receives ``ms_per_token`` of the steps behind the second new token."""
     if not is_model_supported(model) or any("original_forward" not in layer.self_attn.__dict__ for layer in model.model.layers):
         raise ValueError("generate needs a model whose layers are all patched (apply_patch_with_prefill)")
     B, S = input_ids.shape
@@ -125,11 +125,18 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, bits: int =
             with torch.cuda.graph(graph):
                 cache.seq_lens += 1
                 step()
-            for _ in range(max_new_tokens - 2):
-                graph.replay()
+            more = graph.replay
         else:
-            for _ in range(max_new_tokens - 2):
+            def more():
                 cache.add(1)
                 step()
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        for _ in range(max_new_tokens - 2):
+            more()
+        end.record()
+        if timings is not None:
+            end.synchronize()
+            timings["ms_per_token"] = start.elapsed_time(end) / (max_new_tokens - 2)
     cache.check_status()
     return history
