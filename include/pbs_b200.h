@@ -135,10 +135,10 @@ int pbs_version(void);
 /* Number of kernels this library has launched in the calling process so far. */
 int64_t pbs_launch_count(void);
 
-/* Diagnostic.  Every device-side wait of the tcgen05 attention kernel is bounded; wait_ns sets the
+/* Diagnostic.  Every device-side wait of the tcgen05 attention kernel and of the paged one is bounded; wait_ns sets the
  * bound for later launches of this process (0 restores the default of 2 s).  drop_arrive = n makes
- * the first softmax warpgroup of CTA 0 (pbs_attn_fwd: of each of the first n CTAs) withhold one barrier arrive, so that one wait
- * runs out there: the kernel then returns with status[0] != 0 instead of a result.  The failure-path tests use
+ * the first softmax warpgroup of CTA 0 (pbs_attn_fwd: of each of the first n CTAs; pbs_paged_attn: CTA 0, status 4) withhold one barrier
+ * arrive, so that one wait runs out there: the kernel then returns with status[0] != 0 instead of a result.  The failure-path tests use
  * this (with a bound of a few milliseconds) to exercise the abort path without faulting or hanging
  * the GPU.  No counterpart in the reference. */
 int pbs_debug_set_attn_wait(int64_t wait_ns, int32_t drop_arrive);
@@ -310,6 +310,7 @@ typedef struct {
 #define PBS_PAGED_BAD_PAGE 1    /* a page number outside the pool: such a token is neither written nor attended  */
 #define PBS_PAGED_BAD_LENGTH 2  /* a sequence longer than its row of the block table: it ends with that row      */
 #define PBS_PAGED_BAD_ROTARY 3  /* a position behind the rotary tables: the token is neither rotated nor written */
+#define PBS_PAGED_TIMEOUT 4     /* pbs_paged_attn: a bounded wait ran out; the output is invalid, and the workspace has to be cleared */
 
 /* The sequences of a call.  seq_lens counts the new tokens in: token i of the new_lens[b] new ones of sequence b is at
  * position seq_lens[b] - new_lens[b] + i.  Tokens at negative positions are left out (an unused row of a batch has length
@@ -343,9 +344,10 @@ int pbs_paged_gather(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* ba
 
 /* Causal attention of the new tokens' queries, q (B, q_heads, S, D), over the cache: token i sees the positions up to its own.
  * out has q's shape; rows that see nothing are 0.  Softmax and sums are held in 32 bits.
+ * The blocks of the kernel wait for one another (it is launched cooperatively) where a sequence may be worked on by several.
  * workspace: pbs_paged_attn_workspace bytes, the first PBS_PAGED_COUNTER_BYTES of them 0 before the first call (each call leaves
  * them so).  Calls that share one come after one another. */
-#define PBS_PAGED_COUNTER_BYTES 16384
+#define PBS_PAGED_COUNTER_BYTES 4096
 int pbs_paged_attn_workspace(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* batch, int32_t q_heads, int64_t* bytes);
 int pbs_paged_attn(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* batch, int32_t q_heads,
                    const void* q, const int64_t q_strides[4], void* out, const int64_t out_strides[4],

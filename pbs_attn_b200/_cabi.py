@@ -68,7 +68,7 @@ class PagedBatch(C.Structure):
                 ("max_pages", C.c_int32), ("batch", C.c_int32), ("new_tokens", C.c_int32), ("reserved", C.c_int32)]
 
 
-PAGED_COUNTER_BYTES = 16384
+PAGED_COUNTER_BYTES = 4096
 
 
 class Logits(C.Structure):

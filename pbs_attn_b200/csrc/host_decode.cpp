@@ -1,5 +1,4 @@
-// The calls of decode.py and logits.py without Python in between, for plain CUDA tensors that the kernels can read in place and outside of
-// stream captures.  Whatever they do not cover they leave, untouched, to the Python code (they return None), which also raises all errors.
+// The calls of decode.py and logits.py without Python in between, for plain CUDA tensors that the kernels can read in place.  Whatever they do not cover they leave, untouched, to the Python code (they return None), which also raises all errors.
 // A step's kernels take a few us; through Python and ctypes a call of the attention took 24 us, one of the logits 30, here 6 and 6.
 #include "host_common.h"
 
@@ -9,7 +8,7 @@
 
 #include <cmath>
 #include <map>
-#include <utility>
+#include <tuple>
 
 namespace {
 
@@ -79,17 +78,18 @@ bool batch_of(const Cache* c, PyObject* table, PyObject* lens, PyObject* new_len
   return true;
 }
 
-// Memory for partial results, one piece a stream: calls on a stream come after one another.  (Never destroyed: the interpreter ends after
-// the allocator that it would go back to.)
-using Spaces = std::map<std::pair<int, cudaStream_t>, at::Tensor>;
+// Memory for partial results, one piece a stream, or a stream of a capture: calls there come after one another.  A capture's comes from
+// its graph's own pool and is cleared by the graph, once for all its calls.  (Never destroyed: the interpreter ends after the allocator
+// that it would go back to.)
+using Spaces = std::map<std::tuple<int, cudaStream_t, unsigned long long>, at::Tensor>;
 Spaces& spaces() {
   static Spaces* s = new Spaces;
   return *s;
 }
 
-at::Tensor& space_of(int device, cudaStream_t st, int64_t need) {
+at::Tensor& space_of(int device, cudaStream_t st, unsigned long long capture, int64_t need) {
   Spaces& s = spaces();
-  const auto key = std::make_pair(device, st);
+  const auto key = std::make_tuple(device, st, capture);
   auto it = s.find(key);
   if (it == s.end() && s.size() >= 8) s.erase(s.begin());
   at::Tensor& t = s[key];
@@ -117,16 +117,19 @@ PyObject* py_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (a[6] != Py_None && !rows_of(c, a[6], q.size(0), q.size(1), q.size(2))) Py_RETURN_NONE;
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)c->device);
   const cudaStream_t st = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)c->device).stream();
-  if (capturing(st)) Py_RETURN_NONE;
+  cudaStreamCaptureStatus status;
+  unsigned long long capture = 0;
+  if (cudaStreamGetCaptureInfo(st, &status, &capture) != cudaSuccess || status == cudaStreamCaptureStatusInvalidated) Py_RETURN_NONE;
+  if (status == cudaStreamCaptureStatusNone) capture = 0;
   at::Tensor out = a[6] == Py_None ? at::empty_like(q) : THPVariable_Unpack(a[6]);
   if (!readable(out, false)) Py_RETURN_NONE;
   int rc = PBS_ERR_SHAPE;
-  at::Tensor* space = &space_of(c->device, st, PBS_PAGED_COUNTER_BYTES);
+  at::Tensor* space = &space_of(c->device, st, capture, PBS_PAGED_COUNTER_BYTES);
   for (int round = 0; rc == PBS_ERR_SHAPE && round < 2; ++round) {
     if (round == 1) {                                              // too small, perhaps
       int64_t need = 0;
       if (c->workspace(c->c, &batch, (int32_t)q.size(1), &need) != PBS_OK || need <= space->numel()) Py_RETURN_NONE;
-      space = &space_of(c->device, st, need);
+      space = &space_of(c->device, st, capture, need);
     }
     const int64_t bytes = space->numel();
     void* const at = space->data_ptr();
@@ -299,6 +302,12 @@ PyObject* py_logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// paged_forget(): the next calls make new workspaces
+PyObject* py_forget(PyObject*, PyObject*) {
+  spaces().clear();
+  Py_RETURN_NONE;
+}
+
 template <class F>
 PyCFunction fast(F f) { return reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f)); }
 
@@ -306,6 +315,7 @@ PyCFunction fast(F f) { return reinterpret_cast<PyCFunction>(reinterpret_cast<vo
 
 PyMethodDef pbs_decode_methods[] = {
     {"paged_attach", py_attach, METH_VARARGS, "paged_attach(struct, device, append, gather, attn, workspace): addresses -> the cache's object here"},
+    {"paged_forget", py_forget, METH_NOARGS, "paged_forget(): workspaces are made anew"},
     {"paged_append", fast(py_append), METH_FASTCALL, "paged_append(cache, k, v, table, lens, new_lens, cos, sin, q, q_out): the rotated queries, True, or None where Python has to do it"},
     {"paged_gather", fast(py_gather), METH_FASTCALL, "paged_gather(cache, table, lens, count, new_lens): (keys, values), or None where Python has to do it"},
     {"paged_attn", fast(py_attn), METH_FASTCALL, "paged_attn(cache, q, table, lens, new_lens, scale, out): the result, or None where Python has to do it"},

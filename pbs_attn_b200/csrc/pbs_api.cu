@@ -146,6 +146,7 @@ int64_t pbs_launch_count(void) { return (int64_t)g_launches.load(); }
 int pbs_debug_set_attn_wait(int64_t wait_ns, int32_t drop_arrive) {
   if (wait_ns < 0) { set_error("wait_ns must be >= 0 (0 restores the default)"); return PBS_ERR_ARG; }
   set_attn_wait((unsigned long long)wait_ns, drop_arrive);
+  set_paged_wait((unsigned long long)wait_ns, drop_arrive);
   return PBS_OK;
 }
 

@@ -201,6 +201,7 @@ int launch_attn_fp32(const Dims& d, const void* q, Strides qs, const void* pk, c
                      const uint8_t* mask, void* out, Strides os, cudaStream_t st);
 bool attn_tc_supported(const Dims& d, int dt);
 void set_attn_wait(unsigned long long wait_ns, int drop_arrive);
+void set_paged_wait(unsigned long long wait_ns, int drop_arrive);
 // Keys and values as the attention reads them: (B, Hq / group, S, D) with any strides, query head h uses head h / group.
 struct KvSource {
   const void* k;

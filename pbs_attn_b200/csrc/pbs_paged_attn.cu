@@ -16,7 +16,9 @@
 //
 // Work is cut by tokens, not by sequences: all (sequence, row tile, KV head) items in a row, in units of kWarps tiles, are dealt
 // to the resident CTAs in equal contiguous shares, so lengths may differ at will and nothing about them has to be known on the host.
-// An item that several CTAs share is joined by whoever is last, from partial results in the order of the CTAs: same bits every time.
+// Items that several CTAs share are joined by all of them together, once each has written its partial result (they wait for one another, so
+// the grid is launched cooperatively): each joins its part of the rows, from the partial results in the order of the CTAs: same bits every time.
+// (With the last CTA of an item joining all of it, one SM read up to 256 KB while the others were done: 5 us instead of 2.)
 //
 // Within a CTA every warp takes every kWarps-th tile of 16 or 32 tokens through its own ring of cp.async stages, with its own running
 // reference and sums; warps meet once an item.
@@ -29,7 +31,11 @@
 namespace pbs {
 namespace {
 
-constexpr int kMaxGrid = PBS_PAGED_COUNTER_BYTES / 4, kMaxBatch = 4096;
+constexpr int kMaxBatch = 4096, kMaxGrid = PBS_PAGED_COUNTER_BYTES / 8;
+
+// Limit of the wait for an item's parts, and the hook that makes it run out (pbs_debug_set_attn_wait).
+std::atomic<unsigned long long> g_wait_ns{2000000000ull};
+std::atomic<int> g_drop_arrive{0};
 
 template <int DT_, int D_, int BITS_, int G_, int NT_>
 struct Cfg {
@@ -53,8 +59,7 @@ struct Cfg {
   static constexpr int RING = WARPS * STAGES * STAGE;
   static constexpr int OROW = D + 4;                               // floats of a row of partial sums: four on, so that stores spread over the banks
   static constexpr int MERGE = WARPS * COLS * (OROW + 2) * 4;
-  static constexpr int JOIN = COLS * 2 * 148 * 2 * 4;              // references and sums of all CTAs that may share an item
-  static constexpr int POOL = RING > MERGE ? (RING > JOIN ? RING : JOIN) : (MERGE > JOIN ? MERGE : JOIN);
+  static constexpr int POOL = RING > MERGE ? RING : MERGE;
   static constexpr int QFRAG = COLS * D * 2;
   static constexpr int FIXED = POOL + QFRAG + COLS * NG * 4 + COLS * 8;      // then the batch's prefix sums
   static_assert(FIXED + kMaxBatch * 4 + 256 <= 227 * 1024, "shared memory");
@@ -68,7 +73,9 @@ struct AttnArgs {
   int dense;                                                       // a page's rows of a head lie together, its params too
   int q_heads, group, row_tiles;
   float scale;                                                     // times log2(e)
-  int* counters;
+  int drop_arrive;                                                 // diagnostic: CTA 0 does not count its part
+  unsigned long long wait_ns;
+  unsigned* counters;                                              // by the first CTA of an item: parts written, and CTAs that have seen all of them
   float* partials;                                                 // [CTA][2]: COLS x D sums, COLS references, COLS sums of weights
 };
 
@@ -548,6 +555,7 @@ struct Item {
   int seq, head, row0;                                             // row = new token * group + query head within the KV head
   int len, full, n;                                                // tokens of the sequence that its row of the table holds, all of them, new ones
   int first, end;                                                  // tokens that the first of the rows sees, and the last
+  int unit1;                                                       // the unit behind the item
 };
 
 // Brings the queries of an item into the order of the product's second operand (in 4 bits scaled by a power of two to a maximum in
@@ -611,7 +619,7 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
   int* limit = reinterpret_cast<int*>(factor + C::COLS);
   int* prefix = limit + C::COLS;                                   // units before sequence b
   __shared__ int scan[C::WARPS];
-  __shared__ int is_last;
+  __shared__ int arrived;
   const pbs_paged_cache_t& c = p.a.c;
   const pbs_paged_batch_t& bt = p.a.b;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -658,6 +666,18 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
   uint8_t* const ring = smem + warp * C::STAGES * C::STAGE;
   const uint32_t ring_at = smem_addr(ring);
 
+  Item it{};
+  constexpr int Q4 = C::D / 4;
+  constexpr int PART = C::COLS * (C::D + 2);                       // floats of a partial result
+  auto write = [&](int col, int d, float4 x, float sum) {          // a piece of a row of the result
+    const int r = it.row0 + col, i = r / p.group;
+    const bool empty = i >= it.n || sum == 0.f;
+    const float inv = empty ? 0.f : 1.f / sum;
+    uint2 y = make_uint2(pack<T>(x.x * inv, x.y * inv), pack<T>(x.z * inv, x.w * inv));
+    if (empty) y = make_uint2(0, 0);
+    *reinterpret_cast<uint2*>((T*)p.out.p + it.seq * p.out.st.b + (it.head * p.group + r % p.group) * p.out.st.h + i * p.out.st.s + d) = y;
+  };
+  int i0 = 0, i1 = 0;                                              // CTAs that share the item
   while (unit < unit_end) {
     // the item of this unit
     int lo = 0, hi = bt.batch - 1;
@@ -666,13 +686,14 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
       if (prefix[mid] <= unit) lo = mid;
       else hi = mid - 1;
     }
-    Item it;
     it.seq = lo;
     it.full = bt.seq_lens[lo];
     it.len = max(0, min(it.full, table_tokens));
     const int units = max(1, (it.len + C::UNIT - 1) / C::UNIT);
     const int within = unit - prefix[lo], index = within / units, start = within % units;
-    const int item_first = unit - start, item_end = item_first + units, stop = min(unit_end, item_end);
+    const int item_first = unit - start;
+    it.unit1 = item_first + units;
+    const int stop = min(unit_end, it.unit1);
     it.head = index % c.kv_heads;
     it.row0 = index / c.kv_heads * C::COLS;
     it.n = bt.new_lens ? min(max(bt.new_lens[lo], 0), bt.new_tokens) : bt.new_tokens;
@@ -798,18 +819,9 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
     w.put(sums + warp * C::COLS * C::OROW, refs + warp * C::COLS, weights + warp * C::COLS);
     __syncthreads();
 
+    i0 = item_first / share;
+    i1 = (it.unit1 - 1) / share;
     const int cols = min(C::COLS, bt.new_tokens * p.group - it.row0);
-    auto write = [&](int col, int d, float4 x, float sum) {        // a piece of a row of the result
-      const int r = it.row0 + col, i = r / p.group;
-      const bool empty = i >= it.n || sum == 0.f;
-      const float inv = empty ? 0.f : 1.f / sum;
-      uint2 y = make_uint2(pack<T>(x.x * inv, x.y * inv), pack<T>(x.z * inv, x.w * inv));
-      if (empty) y = make_uint2(0, 0);
-      *reinterpret_cast<uint2*>((T*)p.out.p + it.seq * p.out.st.b + (it.head * p.group + r % p.group) * p.out.st.h + i * p.out.st.s + d) = y;
-    };
-    constexpr int Q4 = C::D / 4;
-    constexpr int PART = C::COLS * (C::D + 2);                     // floats of a partial result
-    const int i0 = item_first / share, i1 = (item_end - 1) / share;
     float* const part = p.partials + ((int64_t)blockIdx.x * 2 + ((int)blockIdx.x == i0)) * PART;
     for (int e = tid; e < cols * Q4; e += C::THREADS) {
       const int col = e / Q4, d = e % Q4 * 4;
@@ -837,58 +849,108 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
         }
       }
     }
-    if (i0 != i1) {
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) is_last = atomicAdd(p.counters + i0, 1) == i1 - i0;
-      __syncthreads();
-      if (is_last) {
-        __threadfence();
-        if (tid == 0) p.counters[i0] = 0;
-        const int n = i1 - i0 + 1;
-        auto from = [&](int k) { return p.partials + ((int64_t)(i0 + k) * 2 + (k == 0)) * PART; };
-        float* tops = reinterpret_cast<float*>(smem);              // [n][COLS], then weights
-        float* lsum = tops + n * C::COLS;
-        for (int e = tid; e < n * C::COLS; e += C::THREADS) {
-          const float* f = from(e / C::COLS) + C::COLS * C::D + e % C::COLS;
-          tops[e] = __ldcg(f);
-          lsum[e] = __ldcg(f + C::COLS);
-        }
-        __syncthreads();
-        for (int col = warp; col < cols; col += C::WARPS) {        // a warp a query: weights of the parts, and their sum
-          float top = -CUDART_INF_F, sum = 0.f;
-          for (int k = lane; k < n; k += 32) top = fmaxf(top, tops[k * C::COLS + col]);
-          top = warp_max(top);
-          for (int k = lane; k < n; k += 32) {
-            const float rv = tops[k * C::COLS + col], wt = rv == top ? 1.f : exp2_fast(rv - top);
-            tops[k * C::COLS + col] = wt;
-            sum = fmaf(wt, lsum[k * C::COLS + col], sum);
-          }
-          sum = warp_sum(sum);
-          __syncwarp();
-          if (lane == 0) lsum[col] = sum;                          // (part 0's place, read already)
-        }
-        __syncthreads();
-        for (int e = tid; e < cols * Q4; e += C::THREADS) {
-          const int col = e / Q4, d = e % Q4 * 4;
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 16
-          for (int k = 0; k < n; ++k) {
-            const float wt = tops[k * C::COLS + col];
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(from(k) + col * C::D + d));
-            x.x = fmaf(wt, y.x, x.x);
-            x.y = fmaf(wt, y.y, x.y);
-            x.z = fmaf(wt, y.z, x.z);
-            x.w = fmaf(wt, y.w, x.w);
-          }
-          write(col, d, x, lsum[col]);
-        }
-      }
-    }
     __syncthreads();
+    if (i0 != i1 && tid == 0 && !(p.drop_arrive && blockIdx.x == 0)) {
+      __threadfence();                                             // (after the barrier above: for the whole CTA's stores)
+      atomicAdd(p.counters + 2 * i0, 1u);
+    }
     unit = stop;
   }
+  if (i0 == i1) return;
+
+  // The CTAs whose last item this is (the one behind its end may have gone on to another) wait for all parts and join a share of the pieces each
+  const int n = i1 - i0 + 1, joiners = min(total, (i1 + 1) * share) > it.unit1 ? n - 1 : n;
+  if (tid == 0) {
+    volatile unsigned* const parts = p.counters + 2 * i0;
+    unsigned long long start, now;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
+    do {
+      arrived = *parts == (unsigned)n;
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+    } while (!arrived && now - start < p.wait_ns);
+    __threadfence();
+    if (!arrived) {
+      paged_fault(p.a, PBS_PAGED_TIMEOUT);
+    } else if (atomicAdd(p.counters + 2 * i0 + 1, 1u) == (unsigned)joiners - 1) {        // all have seen it: for the next call
+      p.counters[2 * i0] = 0;
+      p.counters[2 * i0 + 1] = 0;
+    }
+  }
+  __syncthreads();
+  if (!arrived) return;
+  const int pieces = min(C::COLS, bt.new_tokens * p.group - it.row0) * Q4, per_cta = (pieces + joiners - 1) / joiners;
+  const int e0 = ((int)blockIdx.x - i0) * per_cta, e1 = min(pieces, e0 + per_cta);
+  auto from = [&](int k) { return p.partials + ((int64_t)(i0 + k) * 2 + (k == 0)) * PART; };
+  if (n <= 8) {                                                    // few parts: a thread a piece
+    for (int e = e0 + tid; e < e1; e += C::THREADS) {
+      const int col = e / Q4, d = e % Q4 * 4;
+      float top = -CUDART_INF_F, sum = 0.f, rv[8], lv[8];
+      float4 y[8], x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        rv[k] = -CUDART_INF_F;
+        lv[k] = 0.f;
+        y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k >= n) continue;
+        rv[k] = __ldcg(from(k) + C::COLS * C::D + col);
+        lv[k] = __ldcg(from(k) + C::COLS * (C::D + 1) + col);
+        y[k] = __ldcg(reinterpret_cast<const float4*>(from(k) + col * C::D + d));
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, rv[k]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float wt = rv[k] == top ? 1.f : exp2_fast(rv[k] - top);
+        sum = fmaf(wt, lv[k], sum);
+        x.x = fmaf(wt, y[k].x, x.x);
+        x.y = fmaf(wt, y[k].y, x.y);
+        x.z = fmaf(wt, y[k].z, x.z);
+        x.w = fmaf(wt, y[k].w, x.w);
+      }
+      write(col, d, x, sum);
+    }
+    return;
+  }
+  for (int e = e0 + warp; e < e1; e += C::WARPS) {                 // many: a warp a piece
+    const int col = e / Q4, d = e % Q4 * 4;
+    float top = -CUDART_INF_F, sum = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = lane; k0 - lane < n; k0 += 128) {
+      float rv[4], lv[4];
+      float4 y[4];
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        rv[a] = -CUDART_INF_F;
+        lv[a] = 0.f;
+        y[a] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int k = k0 + 32 * a;
+        if (k >= n) continue;
+        rv[a] = __ldcg(from(k) + C::COLS * C::D + col);
+        lv[a] = __ldcg(from(k) + C::COLS * (C::D + 1) + col);
+        y[a] = __ldcg(reinterpret_cast<const float4*>(from(k) + col * C::D + d));
+      }
+      const float most = fmaxf(top, warp_max(fmaxf(fmaxf(rv[0], rv[1]), fmaxf(rv[2], rv[3])))), keep = top == most ? 1.f : exp2_fast(top - most);
+      top = most;
+      sum *= keep;
+      x = make_float4(x.x * keep, x.y * keep, x.z * keep, x.w * keep);
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const float wt = rv[a] == top ? 1.f : exp2_fast(rv[a] - top);
+        sum = fmaf(wt, lv[a], sum);
+        x.x = fmaf(wt, y[a].x, x.x);
+        x.y = fmaf(wt, y[a].y, x.y);
+        x.z = fmaf(wt, y[a].z, x.z);
+        x.w = fmaf(wt, y[a].w, x.w);
+      }
+    }
+    x = make_float4(warp_sum(x.x), warp_sum(x.y), warp_sum(x.z), warp_sum(x.w));
+    sum = warp_sum(sum);
+    if (lane == 0) write(col, d, x, sum);
+  }
 }
+
+// Shared memory of a SM, and what a CTA takes of it beyond its dynamic part.
+constexpr int kSmemPerSm = 228 * 1024, kOverhead = 1024 + 256;
 
 int query_tiles(const PagedArgs& a, int q_heads) {                 // NT: the narrowest that holds all queries of a KV head, or the widest
   const int64_t rows = (int64_t)q_heads / a.c.kv_heads * a.b.new_tokens;
@@ -907,8 +969,9 @@ int launch(AttnArgs p, void* workspace, bool measure, int64_t* bytes, cudaStream
   constexpr int kShort = 8;
   const int sms = device_sms();
   int grid = most <= (int64_t)kShort * sms ? sms : C::OCC * sms;
-  grid = grid < 2 * 148 ? grid : 2 * 148;
-  grid = grid < kMaxGrid ? grid : kMaxGrid;
+  const int bytes_smem = C::FIXED + p.a.b.batch * 4;
+  if (2 * (bytes_smem + kOverhead) > kSmemPerSm && grid > sms) grid = sms;     // (all CTAs have to be resident)
+  if (grid > kMaxGrid) grid = kMaxGrid;
   if (most < grid) grid = (int)most;
   if (measure) {
     *bytes = PBS_PAGED_COUNTER_BYTES + (int64_t)grid * 2 * C::COLS * (C::D + 2) * 4;
@@ -931,8 +994,10 @@ int launch(AttnArgs p, void* workspace, bool measure, int64_t* bytes, cudaStream
     steps(c.v_params_strides, 2, 4, p.vp_page, p.vp_slot);
   }
   if (!fits) { set_error("paged attention: a pool of more than 64 GiB (params: 16 GiB)"); return PBS_ERR_SHAPE; }
-  const int bytes_smem = C::FIXED + p.a.b.batch * 4;
-  p.counters = (int*)workspace;
+  p.counters = (unsigned*)workspace;
+  const bool splits = (int64_t)p.a.b.max_pages * p.a.c.page_size > C::UNIT;    // an item may be long enough for several CTAs
+  p.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
+  p.drop_arrive = g_drop_arrive.load(std::memory_order_relaxed);
   p.partials = (float*)((uint8_t*)workspace + PBS_PAGED_COUNTER_BYTES);
   // the limit that holds for any batch, set once a device
   static std::atomic<uint64_t> allowed{0};
@@ -943,7 +1008,18 @@ int launch(AttnArgs p, void* workspace, bool measure, int64_t* bytes, cudaStream
     if (e == cudaSuccess && dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   if (e != cudaSuccess) return cuda_fail(e, "paged_attn_kernel shared memory");
-  paged_attn_kernel<C><<<grid, C::THREADS, bytes_smem, st>>>(p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = bytes_smem;
+  cfg.stream = st;
+  cudaLaunchAttribute together = {};
+  together.id = cudaLaunchAttributeCooperative;
+  together.val.cooperative = 1;
+  cfg.attrs = &together;
+  cfg.numAttrs = splits ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, paged_attn_kernel<C>, p);
+  if (e != cudaSuccess) return cuda_fail(e, "paged_attn_kernel");
   PBS_CUDA_CHECK_LAUNCH("paged_attn_kernel");
   return PBS_OK;
 }
@@ -992,6 +1068,11 @@ int launch_paged_attn(const PagedArgs& a, int q_heads, const RowTensor& q, const
   p.group = q_heads / a.c.kv_heads;
   p.scale = scale * 1.44269504f;
   return by_type(p, workspace, false, nullptr, st);
+}
+
+void set_paged_wait(unsigned long long wait_ns, int drop_arrive) {
+  g_wait_ns.store(wait_ns ? wait_ns : 2000000000ull, std::memory_order_relaxed);
+  g_drop_arrive.store(drop_arrive, std::memory_order_relaxed);
 }
 
 }  // namespace pbs

@@ -27,6 +27,7 @@ from .prefill import _ptr, _readable, _strides
 _DTYPES = {torch.bfloat16: _cabi.BF16, torch.float16: _cabi.FP16}
 _FAULTS = {1: "a page number in block_table is outside the pool", 2: "a sequence is longer than its row of block_table",
            3: "a position is behind the rotary tables"}
+_TIMEOUT = 4
 
 # One word a device that kernels report a fault in: pinned host memory, looked at without a copy, and never given back, since a kernel
 # may still be on its way when the cache it works on is gone.
@@ -46,6 +47,12 @@ def _status_word(device: torch.device) -> C.c_int32:
 
 def _raise_fault(word: C.c_int32):
     code, word.value = word.value, 0
+    if code == _TIMEOUT:                                   # what the blocks meet at is out of step
+        _WORKSPACES.clear()
+        host = _cabi.load_host()
+        if host is not None:
+            host.paged_forget()
+        raise _cabi.PbsError("paged attention: a bounded wait ran out in an earlier call on this device; its output is invalid")
     raise _cabi.PbsError(f"paged cache: {_FAULTS.get(code, code)} (in an earlier call on this device, which left the tokens concerned out)")
 
 

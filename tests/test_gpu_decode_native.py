@@ -113,3 +113,32 @@ def test_logits_same_bits_as_through_python(monkeypatch):
     monkeypatch.setattr(module, "_host", False)
     want = module.process_logits(x, **kw)
     assert torch.equal(got, want) and torch.equal(native, want)
+
+
+def test_captures_have_their_own_workspace():
+    """Two graphs of several calls each, replayed in turn and beside eager calls."""
+    from pbs_attn_b200.decode import paged_attn_fwd, paged_kv_append
+    cache = make_cache(300, 16, 2, 64, torch.float16, 4, 32)
+    past = torch.randn(2, 2, 2000, 64, device="cuda").to(torch.float16)
+    table = make_table(cache, [2000, 1500])
+    lens = ints(2000, 1500)
+    paged_kv_append(cache, past, past, table, lens, new_lens=lens)
+    q = [torch.randn(2, 8, 1, 64, device="cuda").to(torch.float16) for _ in range(4)]
+    want = [paged_attn_fwd(x, cache, table, lens) for x in q]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for pair in (q[:2], q[2:]):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs += [paged_attn_fwd(x, cache, table, lens) for x in pair]
+        graphs.append(g)
+    for _ in range(5):
+        for o in outs:
+            o.zero_()
+        for g in graphs:
+            g.replay()
+        again = paged_attn_fwd(q[0], cache, table, lens)
+        assert torch.equal(again, want[0]) and all(torch.equal(o, w) for o, w in zip(outs, want))
+    cache.check_status()
+    torch.cuda.synchronize()
+    del graphs

@@ -282,3 +282,42 @@ def test_refusals():
             paged_attn_fwd(*args, **kw)
     assert paged_attn_fwd(q[:0], cache, table[:0], n[:0]).shape == (0, 8, 1, 128)
     cache.check_status()
+
+
+def test_calls_that_overlap_on_streams():
+    """Calls whose blocks wait for one another, under way on several streams at a time."""
+    from pbs_attn_b200.decode import paged_attn_fwd
+    cases = []
+    for i, lens in enumerate(([20000], [5000, 300], [60000], [100, 9000, 40])):
+        q, cache, table = _case(lens, 8, 2, 1, seed=i, ps=64)
+        t = ints(*lens)
+        cases.append((torch.cuda.Stream(), q, cache, table, t, paged_attn_fwd(q, cache, table, t)))
+    torch.cuda.synchronize()
+    got = [[] for _ in cases]
+    for _ in range(30):
+        for i, (s, q, cache, table, t, _) in enumerate(cases):
+            with torch.cuda.stream(s):
+                got[i].append(paged_attn_fwd(q, cache, table, t))
+    torch.cuda.synchronize()
+    for g, c in zip(got, cases):
+        c[2].check_status()
+        assert all(torch.equal(x, c[5]) for x in g)
+
+
+def test_a_wait_that_runs_out_is_reported():
+    from pbs_attn_b200 import _cabi
+    from pbs_attn_b200.decode import paged_attn_fwd
+    q, cache, table = _case([5000], 8, 2, 1)
+    want = paged_attn_fwd(q, cache, table, ints(5000))
+    torch.cuda.synchronize()
+    lib = _cabi.load()
+    try:
+        lib.pbs_debug_set_attn_wait(5_000_000, 1)              # 5 ms; the first block does not arrive
+        paged_attn_fwd(q, cache, table, ints(5000))
+        torch.cuda.synchronize()
+    finally:
+        lib.pbs_debug_set_attn_wait(0, 0)
+    with pytest.raises(_cabi.PbsError, match="bounded wait"):
+        paged_attn_fwd(q, cache, table, ints(5000))
+    assert torch.equal(paged_attn_fwd(q, cache, table, ints(5000)), want)
+    cache.check_status()
