@@ -60,8 +60,10 @@ struct Cfg {
   static constexpr int OROW = D + 4;                               // floats of a row of partial sums: four on, so that stores spread over the banks
   static constexpr int MERGE = WARPS * COLS * (OROW + 2) * 4;
   static constexpr int POOL = RING > MERGE ? RING : MERGE;
+  static constexpr bool LESS8 = BITS == 4 && DT == PBS_FP16;       // V's products are of code - 8 (see Warp)
+  static constexpr int SHIFT = BITS == 4 && !LESS8 ? WARPS * COLS * NG * 4 : 0;
   static constexpr int QFRAG = COLS * D * 2;
-  static constexpr int FIXED = POOL + QFRAG + COLS * NG * 4 + COLS * 8;      // then the batch's prefix sums
+  static constexpr int FIXED = POOL + QFRAG + SHIFT + COLS * NG * 4 + COLS * 8;      // then the batch's prefix sums
   static_assert(FIXED + kMaxBatch * 4 + 256 <= 227 * 1024, "shared memory");
 };
 
@@ -174,6 +176,15 @@ __device__ __forceinline__ void load_params(uint32_t (&w)[C::NG], const uint8_t*
 // Weights are p = 2^(score - ref) with a reference per query that is raised only when a product p * step could leave fp16's range (above
 // 2^15), to where the largest is 2^7: so the maximum over the warp is taken once in a while and not every tile, and the products, which
 // are what the result is made of, keep 2^21 below the largest before they lose bits.
+//
+// Sums of V's codes as they are grow with the number of tokens, while in flat attention what they leave beside the minima shrinks with its
+// root; what the tensor cores cut off such sums then shows (8 sequences of 131072: relative error 5.2e-3).  So
+//   fp16: each product is followed by one of -8 with the same weights, and the minimum moves up by 8 steps; a weight's rounding, too, acts on
+//         code - 8 then and not on the code (3.1e-4, of which the result's own rounding is 2.1e-4);
+//   bf16: every kShiftEvery tiles the sums are moved by what one of each group's has come to, and that is kept aside (1.7e-3, the result's
+//         own rounding).  The other way costs 10 % of the time where it goes into arithmetic, this one 1.
+constexpr int kShiftEvery = 8;
+
 template <class C>
 struct Warp {
   using T = typename C::T;
@@ -184,9 +195,14 @@ struct Warp {
   const float* qsum;
   const float* factor;
   const int* limit;
+  float* shift;                                                    // bf16: what sums were moved by, [group][query]
   int lane;
 
   __device__ __forceinline__ void start() {
+    if constexpr (C::SHIFT > 0) {
+      for (int i = lane; i < C::NG * C::COLS; i += 32) shift[i] = 0.f;
+      __syncwarp();
+    }
 #pragma unroll
     for (int i = 0; i < C::D / 16; ++i)
 #pragma unroll
@@ -313,7 +329,10 @@ struct Warp {
           o[i][n][c + 2] *= keep;
         }
 #pragma unroll
-        for (int g = 0; g < (C::BITS == 4 ? C::NG : 1); ++g) om[g][n][c] *= keep;
+        for (int g = 0; g < (C::BITS == 4 ? C::NG : 1); ++g) {
+          om[g][n][c] *= keep;
+          if (C::SHIFT > 0 && lane < 4) shift[g * C::COLS + 8 * n + 2 * lane + c] *= keep;
+        }
 #pragma unroll
         for (int m = 0; m < C::MT; ++m)
 #pragma unroll
@@ -337,6 +356,26 @@ struct Warp {
             for (int c = 0; c < 2; ++c)
               if (t0 + t < limit[8 * n + 2 * (lane % 4) + c]) o[i][n][2 * h + c] += x;
         }
+  }
+
+  __device__ __forceinline__ void move_sums() {
+    if constexpr (C::SHIFT > 0) {
+#pragma unroll
+      for (int g = 0; g < C::NG; ++g)
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            constexpr int TILES = C::G / 16;                       // of 16 channels, in a group
+            const float x = __shfl_sync(0xffffffffu, o[g * TILES][n][c], lane % 4);
+#pragma unroll
+            for (int i = g * TILES; i < (g + 1) * TILES; ++i) {
+              o[i][n][c] -= x;
+              o[i][n][c + 2] = fmaf(-17.f, x, o[i][n][c + 2]);     // (low + 16 high)
+            }
+            if (lane < 4) shift[g * C::COLS + 8 * n + 2 * lane + c] += x;
+          }
+    }
   }
 
   // Takes in the tile of tokens t0 .. in shared memory.  MASKED: some query does not see all of them, or 16 of them (a bit of hole) have no page.
@@ -483,7 +522,7 @@ struct Warp {
               const int g = j * 32 / C::G;
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                const float s = step_of<T>(vp[m][h][g]), low = low_of<T>(vp[m][h][g]);
+                const float s = step_of<T>(vp[m][h][g]), low = C::LESS8 ? fmaf(8.f, s, low_of<T>(vp[m][h][g])) : low_of<T>(vp[m][h][g]);
 #pragma unroll
                 for (int n = 0; n < C::NT; ++n) {
                   // a weight of 0 must not meet a step or minimum that is not finite, of a token that this query does not see
@@ -499,11 +538,14 @@ struct Warp {
             // rows of the product: the low code of a byte, and the byte (low + 16 high, eight bits that fp16 holds as well): four
             // operations for eight codes, where masking the high ones out takes five
             constexpr uint32_t M0 = 0x000f000fu, M = 0x00ff00ffu;
+            [[maybe_unused]] constexpr uint32_t kLess = 0x80088008u, kLess16 = 0x80888088u;          // -8 and -(8 + 16 * 8), times 2^-24
             const uint32_t y = r[2 * jj] & M, z = r[2 * jj + 1] & M, y8 = __byte_perm(r[2 * jj], 0, 0x4341), z8 = __byte_perm(r[2 * jj + 1], 0, 0x4341);
 #pragma unroll
             for (int n = 0; n < C::NT; ++n) {
               mma<PBS_FP16>(o[2 * j][n], y & M0, y, z & M0, z, b[n][0], b[n][1]);
+              if constexpr (C::LESS8) mma<PBS_FP16>(o[2 * j][n], kLess, kLess16, kLess, kLess16, b[n][0], b[n][1]);
               mma<PBS_FP16>(o[2 * j + 1][n], y8 & M0, y8, z8 & M0, z8, b[n][0], b[n][1]);
+              if constexpr (C::LESS8) mma<PBS_FP16>(o[2 * j + 1][n], kLess, kLess16, kLess, kLess16, b[n][0], b[n][1]);
             }
           }
         }
@@ -513,6 +555,7 @@ struct Warp {
 
   // Sums, reference and weights' sum of this warp's tokens to shared memory, query by query.
   __device__ __forceinline__ void put(float* sums, float* refs, float* weights) {
+    __syncwarp();
 #pragma unroll
     for (int n = 0; n < C::NT; ++n)
 #pragma unroll
@@ -534,10 +577,12 @@ struct Warp {
         if constexpr (C::BITS == 4) {
 #pragma unroll
           for (int j = 0; j < C::CH; ++j) {
-            const float low = om[j * 32 / C::G][n][c];
+            const int g = j * 32 / C::G;
+            const float (&e)[4] = o[2 * j][n], (&f)[4] = o[2 * j + 1][n];
+            float low = om[g][n][c];
+            if constexpr (C::SHIFT > 0) low = fmaf(shift[g * C::COLS + col], 0x1p24f, low);
             *reinterpret_cast<float4*>(row + 32 * j + 4 * (lane / 4)) =
-                make_float4(fmaf(o[2 * j][n][c], 0x1p24f, low), fmaf(o[2 * j][n][c + 2] - o[2 * j][n][c], 0x1p20f, low),
-                            fmaf(o[2 * j + 1][n][c], 0x1p24f, low), fmaf(o[2 * j + 1][n][c + 2] - o[2 * j + 1][n][c], 0x1p20f, low));
+                make_float4(fmaf(e[c], 0x1p24f, low), fmaf(e[c + 2] - e[c], 0x1p20f, low), fmaf(f[c], 0x1p24f, low), fmaf(f[c + 2] - f[c], 0x1p20f, low));
           }
         } else {
 #pragma unroll
@@ -614,7 +659,7 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
   using T = typename C::T;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* frag = smem + C::POOL;
-  float* qsum = reinterpret_cast<float*>(frag + C::QFRAG);
+  float* qsum = reinterpret_cast<float*>(frag + C::QFRAG + C::SHIFT);
   float* factor = qsum + C::COLS * C::NG;
   int* limit = reinterpret_cast<int*>(factor + C::COLS);
   int* prefix = limit + C::COLS;                                   // units before sequence b
@@ -663,6 +708,7 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
   w.qsum = qsum;
   w.factor = factor;
   w.limit = limit;
+  w.shift = reinterpret_cast<float*>(frag + C::QFRAG) + warp * C::NG * C::COLS;
   uint8_t* const ring = smem + warp * C::STAGES * C::STAGE;
   const uint32_t ring_at = smem_addr(ring);
 
@@ -809,6 +855,7 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
       const uint32_t hole = holes >> slot * C::MT & ((1u << C::MT) - 1);
       if (t0 > plain || hole) w.template tile<true>(stage, t0, hole);
       else w.template tile<false>(stage, t0, 0);
+      if (C::SHIFT > 0 && i % kShiftEvery == kShiftEvery - 1) w.move_sums();
       slot = slot == C::STAGES - 1 ? 0 : slot + 1;
     }
     copy_wait<0>();

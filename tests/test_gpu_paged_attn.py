@@ -321,3 +321,27 @@ def test_a_wait_that_runs_out_is_reported():
         paged_attn_fwd(q, cache, table, ints(5000))
     assert torch.equal(paged_attn_fwd(q, cache, table, ints(5000)), want)
     cache.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("group", [32, 64])
+def test_flat_attention_over_many_tokens_keeps_its_precision(dtype, group):
+    """All tokens weigh about the same, and what they leave is the root of their number: errors that grow with the number would show.
+
+    Rounding a result to its type is 0.42 unit of relative error in the mean square; in fp16 the weights' rounding, the same of 2^-11, acts
+    on code - 8, about 3.3 steps of a range of 15 that covers 4.6 deviations (64 channels) of a value.  A quarter on top."""
+    from pbs_attn_b200.decode import paged_attn_fwd, paged_kv_append
+    B, H, n, D, ps = 16, 8, 20000, 128, 64
+    cache = make_cache(B * -(-n // ps) + 2, ps, H, D, dtype, 4, group)
+    lens = [n] * B
+    table = make_table(cache, lens)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for b in range(B):
+        k, v = (torch.randn(1, H, n, D, generator=g, device="cuda").to(dtype) for _ in "kv")
+        paged_kv_append(cache, k, v, table[b:b + 1], ints(n))
+    q = (torch.randn(B, 8, 1, D, generator=g, device="cuda") * 0.2).to(dtype)
+    got = paged_attn_fwd(q, cache, table, ints(*lens)).double()
+    want = torch.cat([attention(q[b:b + 1], cache, table[b:b + 1], [n])[0] for b in range(B)])
+    rounding = 0.42 * (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11)
+    weights = 0.42 * 2.0 ** -11 * 3.3 * 4.6 / 15 if dtype == torch.float16 else 0.0
+    assert (got - want).norm() / want.norm() <= 1.25 * (rounding ** 2 + weights ** 2) ** 0.5
