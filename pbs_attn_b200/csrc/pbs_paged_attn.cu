@@ -999,9 +999,11 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
 // Shared memory of a SM, and what a CTA takes of it beyond its dynamic part.
 constexpr int kSmemPerSm = 228 * 1024, kOverhead = 1024 + 256;
 
-int query_tiles(const PagedArgs& a, int q_heads) {                 // NT: the narrowest that holds all queries of a KV head, or the widest
+// NT: the narrowest that holds all queries of a KV head, or the widest (of 256 channels two, for its registers).  Columns that hold no query
+// cost as much as others: 20 queries over pages of 16 bits (8 sequences of up to 8192) take 39.7 us in three, 41.7 in four.
+int query_tiles(const PagedArgs& a, int q_heads) {
   const int64_t rows = (int64_t)q_heads / a.c.kv_heads * a.b.new_tokens;
-  return rows <= 8 ? 1 : rows <= 16 || a.c.head_dim == 256 ? 2 : 4;
+  return rows <= 8 ? 1 : rows <= 16 || a.c.head_dim == 256 ? 2 : rows <= 24 ? 3 : 4;
 }
 
 template <class C>
@@ -1075,6 +1077,8 @@ template <int DT, int D, int BITS, int G>
 int by_queries(const AttnArgs& p, void* w, bool measure, int64_t* bytes, cudaStream_t st) {
   const int nt = query_tiles(p.a, p.q_heads);
   if (nt == 1) return launch<Cfg<DT, D, BITS, G, 1>>(p, w, measure, bytes, st);
+  if constexpr (D != 256)
+    if (nt == 3) return launch<Cfg<DT, D, BITS, G, 3>>(p, w, measure, bytes, st);
   if constexpr (D != 256)
     if (nt == 4) return launch<Cfg<DT, D, BITS, G, 4>>(p, w, measure, bytes, st);
   return launch<Cfg<DT, D, BITS, G, 2>>(p, w, measure, bytes, st);
