@@ -1,5 +1,6 @@
 // The calls of decode.py and logits.py without Python in between, for plain CUDA tensors that the kernels can read in place.  Whatever they do not cover they leave, untouched, to the Python code (they return None), which also raises all errors.
-// A step's kernels take a few us; through Python and ctypes a call of the attention took 24 us, one of the logits 30, here 6 and 6.
+// A step's kernels take a few us; through Python and ctypes a call of the attention over 187 tokens took 24 us and one of the logits 30,
+// here 6 and 6.
 #include "host_common.h"
 
 #include <ATen/ops/empty.h>

