@@ -14,18 +14,18 @@
 // padding.  mma.sync and not tcgen05: the operand that changes is unpacked in registers, tcgen05 would take it back through shared
 // memory (four times the bytes that came in), and the tensor cores are far from being the limit.
 //
-// Work is cut by tokens, not by sequences: all (sequence, row tile, KV head) items in a row, in units of kWarps tiles, are dealt
+// Work is cut by tokens, not by sequences: all (sequence, row tile, KV head) items in a row, in units of a tile a warp, are dealt
 // to the resident CTAs in equal contiguous shares, so lengths may differ at will and nothing about them has to be known on the host.
 // Items that several CTAs share are joined by all of them together, once each has written its partial result (they wait for one another, so
 // the grid is launched cooperatively): each joins its part of the rows, from the partial results in the order of the CTAs: same bits every time.
-// (With the last CTA of an item joining all of it, one SM read up to 256 KB while the others were done: 5 us instead of 2.)
+// (With the last CTA of an item joining all of it, one SM read up to 256 KB while the others were done: 5 us instead of 3.)
 //
-// Measured (B200, GPU time): 64 sequences of 12000 to 16384, 8 KV heads of 128, groups of 64, bf16: 205 us for 1.05 GB, 5.1 TB/s, 78 % of the
+// Measured (B200, GPU time): 64 sequences of 12000 to 16384, 8 KV heads of 128, groups of 64, bf16: 203 us for 1.05 GB, 5.1 TB/s, 79 % of the
 // copy rate (the copies alone take 164 us, the arithmetic alone 172: 560 instructions for 32 tokens, half of them on the ALU pipe); one
-// sequence of 131072: 41 us, 3.6 TB/s; of 32768 with 4 KV heads: 13 us.  Pages of 16 bits, 64 sequences of up to 4096: 121 us for 0.8 GB, the
+// sequence of 131072: 40 us, 3.7 TB/s; of 32768 with 4 KV heads: 13 us.  Pages of 16 bits, 64 sequences of up to 4096: 121 us for 0.8 GB, the
 // copy rate.
 //
-// Within a CTA every warp takes every kWarps-th tile of 16 or 32 tokens through its own ring of cp.async stages, with its own running
+// Within a CTA every warp takes every eighth (fourth) tile of 16 or 32 tokens through its own ring of cp.async stages, with its own running
 // reference and sums; warps meet once an item.
 #include <atomic>
 #include <climits>
@@ -58,7 +58,9 @@ struct Cfg {
   static constexpr int PROW = BITS == 4 ? 4 * NG : 0;
   static constexpr int STAGE = TILE * 2 * (ROW + PROW);
   static constexpr int OCC = BITS == 4 && NT == 1 && D <= 128 ? 2 : 1;       // CTAs a SM
-  static constexpr int BUDGET = (OCC == 2 ? 112 : 200) * 1024;
+  // (with two CTAs a SM a third stage of 128 channels gained nothing: 64 sequences of 16384 205 us with it, 203 without; and the batch's
+  // prefix sums have room)
+  static constexpr int BUDGET = (OCC == 2 ? 96 : 200) * 1024;
   static constexpr int STAGES_FIT = BUDGET / (WARPS * STAGE);
   static constexpr int STAGES = STAGES_FIT < 2 ? 2 : STAGES_FIT > 4 ? 4 : STAGES_FIT;
   static constexpr int RING = WARPS * STAGES * STAGE;

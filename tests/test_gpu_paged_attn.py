@@ -345,3 +345,14 @@ def test_flat_attention_over_many_tokens_keeps_its_precision(dtype, group):
     rounding = 0.42 * (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11)
     weights = 0.42 * 2.0 ** -11 * 3.3 * 4.6 / 15 if dtype == torch.float16 else 0.0
     assert (got - want).norm() / want.norm() <= 1.25 * (rounding ** 2 + weights ** 2) ** 0.5
+
+
+def test_the_largest_batch():
+    lens = [(7 * b) % 40 for b in range(4096)]
+    lens[4000] = 3000
+    q, cache, table = _case(lens, 2, 1, 1, 64)
+    from pbs_attn_b200.decode import paged_attn_fwd
+    got = paged_attn_fwd(q, cache, table, ints(*lens))
+    cache.check_status()
+    for b in (0, 1, 17, 2000, 4000, 4095):
+        assert_within(got[b:b + 1], *attention(q[b:b + 1], cache, table[b:b + 1], [lens[b]]))
