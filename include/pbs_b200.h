@@ -360,8 +360,9 @@ int pbs_paged_attn(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* batc
  *   c times in its written part:      x - frequency * c, then x - presence if c > 0
  *   listed in the row's biases:       x + value (values of a token that is listed twice add up, in their order)
  *   bit v % 32 of word v / 32 is 0:   -infinity
- * The history of row b is tokens[b][0 .. token_lens[b]), its first prompt_lens[b] the prompt, the rest written.  Ids outside
- * the vocabulary are skipped, in biases too.  NULL: without that part (NULL lengths: the whole row, no prompt).  A row of the
+ * The history of row b is tokens[b][0 .. token_lens[b]), its first prompt_lens[b] the prompt, the rest written; lengths outside
+ * 0 .. history, and prompts longer than the history, are taken as the nearer end.  Ids outside the vocabulary are skipped, in
+ * biases too.  NULL: without that part (NULL lengths: the whole row, no prompt).  A row of the
  * bias's values is in the order of its ids; repetition is above 0. */
 typedef struct {
   int32_t dtype;                  /* pbs_dtype_t of logits and out                              */

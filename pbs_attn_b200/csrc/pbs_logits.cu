@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(kThreads, kResident) logits_kernel(const __gri
     }
   } else if (counts || biased) {
     const int n = !counts ? 0 : a.token_lens ? min(max(a.token_lens[row], 0), a.history) : a.history;
-    const int prompt = a.prompt_lens ? a.prompt_lens[row] : 0;
+    const int prompt = a.prompt_lens ? min(max(a.prompt_lens[row], 0), n) : 0;           // (any number is taken: "all of it" may be 2^31 - 1)
     const int words = ((hi - first) * (int)sizeof(W) + 15) / 16;
     for (int i = tid; i < words; i += kHalf) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
     if (tid == 0) n_listed = n_biases = 0;
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kThreads, kResident) logits_kernel(const __gri
     };
     const bool wide_ids = a.token_bytes == 8;
     const int64_t base = row * a.tokens_stride;
-    for (int i = tid + (rep == 1.f ? max(prompt, 0) : 0); i < n; i += kIds * kHalf) {       // (the prompt is for the repetition penalty only)
+    for (int i = tid + (rep == 1.f ? prompt : 0); i < n; i += kIds * kHalf) {       // (the prompt is for the repetition penalty only)
       int64_t id[kIds];
       if (wide_ids) {
 #pragma unroll

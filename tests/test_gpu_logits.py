@@ -101,6 +101,18 @@ def test_numbers_for_penalties_and_whole_rows():
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("repetition", [None, 1.3])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_prompts_longer_than_any_history(repetition, dtype):
+    """A prompt length of 2^31 - 1 says that all of the row is the prompt, as that of its history does; one of -2^31, none of it."""
+    most, L = 2 ** 31 - 1, 700
+    logits, kw = _inputs(6, 3000, L, dtype, seed=4)
+    args = dict(tokens=kw["tokens"], token_lens=ints(L, 600, 0, L, 300, most), repetition_penalty=repetition, frequency_penalty=kw["frequency_penalty"],
+                presence_penalty=kw["presence_penalty"])
+    got = _check(logits, prompt_lens=ints(most, most - 255, most, -most - 1, 301, most - 100), **args)
+    assert torch.equal(got, _check(logits, prompt_lens=ints(L, 600, 0, 0, 300, L), **args))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("lead,out_lead", [(0, 0), (1, 1), (3, 3), (1, 2), (0, 5)])
 def test_rows_that_start_anywhere(dtype, lead, out_lead):
