@@ -93,50 +93,51 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, bits: int =
         raise ValueError("a prompt and at least one new token are needed")
     if step_logits is not None and cuda_graph:
         raise ValueError("step_logits are collected in eager steps (cuda_graph=False)")
-    cache = PagedModelCache(model, B, S + max_new_tokens, bits, page_size, group_size)
-    history = torch.zeros(B, S + max_new_tokens, dtype=torch.long, device=input_ids.device)
-    history[:, :S] = input_ids
-    prompt_lens = torch.full((B,), S, dtype=torch.int32, device=input_ids.device)
-    penalties = dict(repetition_penalty=repetition_penalty, frequency_penalty=frequency_penalty, presence_penalty=presence_penalty)
-    if any(p is not None for p in penalties.values()):
-        penalties.update(tokens=history, token_lens=cache.seq_lens, prompt_lens=prompt_lens)
+    with torch.cuda.device(input_ids.device):              # (graphs, streams and events belong to the current one)
+        cache = PagedModelCache(model, B, S + max_new_tokens, bits, page_size, group_size)
+        history = torch.zeros(B, S + max_new_tokens, dtype=torch.long, device=input_ids.device)
+        history[:, :S] = input_ids
+        prompt_lens = torch.full((B,), S, dtype=torch.int32, device=input_ids.device)
+        penalties = dict(repetition_penalty=repetition_penalty, frequency_penalty=frequency_penalty, presence_penalty=presence_penalty)
+        if any(p is not None for p in penalties.values()):
+            penalties.update(tokens=history, token_lens=cache.seq_lens, prompt_lens=prompt_lens)
 
-    def choose(logits):
-        if step_logits is not None:
-            step_logits.append(logits.clone())
-        logits = process_logits(logits, bias_ids=bias_ids, bias_values=bias_values, allowed=allowed, **penalties)
-        token = logits.argmax(-1, keepdim=True)
-        history.scatter_(1, cache.seq_lens.long()[:, None], token)      # behind the tokens that there are
-        return token
+        def choose(logits):
+            if step_logits is not None:
+                step_logits.append(logits.clone())
+            logits = process_logits(logits, bias_ids=bias_ids, bias_values=bias_values, allowed=allowed, **penalties)
+            token = logits.argmax(-1, keepdim=True)
+            history.scatter_(1, cache.seq_lens.long()[:, None], token)      # behind the tokens that there are
+            return token
 
-    cache.add(S)
-    token = choose(_run_layers(model, input_ids, cache))
+        cache.add(S)
+        token = choose(_run_layers(model, input_ids, cache))
 
-    def step():
-        token.copy_(choose(_run_layers(model, token, cache)))
+        def step():
+            token.copy_(choose(_run_layers(model, token, cache)))
 
-    if max_new_tokens > 1:
-        cache.add(1)
-        step()                                             # (also brings up what a capture must not)
-    if max_new_tokens > 2:
-        if cuda_graph:
-            torch.cuda.synchronize(input_ids.device)
-            graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph):
-                cache.seq_lens += 1
-                step()
-            more = graph.replay
-        else:
-            def more():
-                cache.add(1)
-                step()
-        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-        start.record()
-        for _ in range(max_new_tokens - 2):
-            more()
-        end.record()
-        if timings is not None:
-            end.synchronize()
-            timings["ms_per_token"] = start.elapsed_time(end) / (max_new_tokens - 2)
-    cache.check_status()
-    return history
+        if max_new_tokens > 1:
+            cache.add(1)
+            step()                                             # (also brings up what a capture must not)
+        if max_new_tokens > 2:
+            if cuda_graph:
+                torch.cuda.synchronize(input_ids.device)
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=torch.cuda.Stream(input_ids.device)):     # (by default one stream of whichever device captured first)
+                    cache.seq_lens += 1
+                    step()
+                more = graph.replay
+            else:
+                def more():
+                    cache.add(1)
+                    step()
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            for _ in range(max_new_tokens - 2):
+                more()
+            end.record()
+            if timings is not None:
+                end.synchronize()
+                timings["ms_per_token"] = start.elapsed_time(end) / (max_new_tokens - 2)
+        cache.check_status()
+        return history

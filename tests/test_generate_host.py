@@ -1,0 +1,73 @@
+"""CPU-only: the host side of generation, with the model's layers and CUDA replaced by fakes."""
+import contextlib
+import types
+
+import pytest
+import torch
+
+import pbs_attn_b200.generate as module
+
+
+@pytest.fixture
+def fakes(monkeypatch):
+    """Fakes that note (what, device that was current, device of the stream that was given)."""
+    seen, current = [], [None]
+
+    @contextlib.contextmanager
+    def device(d):
+        before, current[0] = current[0], d
+        yield
+        current[0] = before
+
+    @contextlib.contextmanager
+    def graph(g, stream=None, **kw):
+        seen.append(("graph", current[0], getattr(stream, "device", None)))
+        yield
+
+    class Event:
+        def __init__(self, **kw):
+            seen.append(("event", current[0], None))
+
+        def record(self):
+            pass
+
+        def synchronize(self):
+            pass
+
+        def elapsed_time(self, other):
+            return 1.0
+
+    class Cache:
+        def __init__(self, model, batch, *a):
+            self.seq_lens = torch.zeros(batch, dtype=torch.int32)
+
+        def add(self, n):
+            self.seq_lens += n
+
+        def check_status(self):
+            pass
+
+    for name, x in (("device", device), ("graph", graph), ("Event", Event), ("synchronize", lambda d=None: None),
+                    ("Stream", lambda d=None: types.SimpleNamespace(device=d)), ("CUDAGraph", lambda: types.SimpleNamespace(replay=lambda: None))):
+        monkeypatch.setattr(torch.cuda, name, x)
+    monkeypatch.setattr(module, "PagedModelCache", Cache)
+    monkeypatch.setattr(module, "is_model_supported", lambda m: True)
+    monkeypatch.setattr(module, "process_logits", lambda x, **kw: x)
+
+    def layers(model, ids, cache):
+        seen.append(("layers", current[0], None))
+        return torch.zeros(ids.shape[0], 5)
+
+    monkeypatch.setattr(module, "_run_layers", layers)
+    return seen
+
+
+def test_everything_runs_with_the_inputs_device_current(fakes):
+    """The current device is not the model's: streams, graphs and events are those of the model's all the same."""
+    model = types.SimpleNamespace(model=types.SimpleNamespace(layers=[]))
+    ids = torch.zeros(1, 4, dtype=torch.long)
+    timings = {}
+    assert module.generate(model, ids, 5, timings=timings).shape == (1, 9) and timings["ms_per_token"] > 0
+    assert [w for w, _, _ in fakes] == ["layers", "layers", "graph", "layers", "event", "event"]
+    assert all(d == ids.device for _, d, _ in fakes)
+    assert all(s == ids.device for w, _, s in fakes if w == "graph")

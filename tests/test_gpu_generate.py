@@ -55,6 +55,16 @@ def test_graph_and_eager_choose_the_same(bits):
     assert torch.equal(a, b)
 
 
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
+def test_on_a_device_that_is_not_current():
+    from pbs_attn_b200.generate import generate
+    model, first = _patched(_model()).to("cuda:1"), _patched(_model())
+    ids = torch.randint(0, 300, (2, 150), device="cuda")
+    want = generate(first, ids, 20, repetition_penalty=1.3)              # (a capture on the current device comes first)
+    for graph in (True, False):
+        assert torch.equal(generate(model, ids.to("cuda:1"), 20, repetition_penalty=1.3, cuda_graph=graph).to("cuda"), want)
+
+
 def test_masks_and_penalties_reach_the_choice():
     from pbs_attn_b200.generate import generate
     model = _patched(_model())
