@@ -7,9 +7,9 @@
 #include <ATen/ops/empty_strided.h>
 #include <ATen/ops/zeros.h>
 
+#include <algorithm>
 #include <cmath>
-#include <map>
-#include <tuple>
+#include <vector>
 
 namespace {
 
@@ -80,23 +80,35 @@ bool batch_of(const Cache* c, PyObject* table, PyObject* lens, PyObject* new_len
 }
 
 // Memory for partial results, one piece a stream, or a stream of a capture: calls there come after one another.  A capture's comes from
-// its graph's own pool and is cleared by the graph, once for all its calls.  (Never destroyed: the interpreter ends after the allocator
-// that it would go back to.)
-using Spaces = std::map<std::tuple<int, cudaStream_t, unsigned long long>, at::Tensor>;
-Spaces& spaces() {
-  static Spaces* s = new Spaces;
+// its graph's own pool and is cleared by the graph, once for all its calls.
+struct Space {
+  int device;
+  cudaStream_t st;
+  unsigned long long capture;                                      // 0: none
+  at::Tensor memory;
+};
+
+constexpr size_t kMaxSpaces = 8;
+
+// In the order of their last use.  (Never destroyed: the interpreter ends after the allocator that they would go back to.)
+std::vector<Space>& spaces() {
+  static auto* s = new std::vector<Space>;
   return *s;
 }
 
-at::Tensor& space_of(int device, cudaStream_t st, unsigned long long capture, int64_t need) {
-  Spaces& s = spaces();
-  const auto key = std::make_tuple(device, st, capture);
-  auto it = s.find(key);
-  if (it == s.end() && s.size() >= 8) s.erase(s.begin());
-  at::Tensor& t = s[key];
-  if (!t.defined() || t.numel() < need)
-    t = at::zeros({need}, at::TensorOptions().dtype(at::kByte).device(at::Device(at::kCUDA, (c10::DeviceIndex)device)));
-  return t;
+// The place of a stream's memory, which is what `memory` is undefined for where there is none yet.  What makes room are the captures before
+// this one, whose graphs no longer ask (what they hold would keep those graphs' pools), then what was used longest ago.
+at::Tensor& space_of(int device, cudaStream_t st, unsigned long long capture) {
+  std::vector<Space>& s = spaces();
+  for (size_t i = s.size(); i-- > 0;) {
+    if (s[i].device != device || s[i].st != st || s[i].capture != capture) continue;
+    std::rotate(s.begin() + i, s.begin() + i + 1, s.end());
+    return s.back().memory;
+  }
+  s.erase(std::remove_if(s.begin(), s.end(), [&](const Space& x) { return x.capture != 0 && x.capture != capture; }), s.end());
+  if (s.size() >= kMaxSpaces) s.erase(s.begin());
+  s.push_back(Space{device, st, capture, at::Tensor()});
+  return s.back().memory;
 }
 
 // paged_attn(cache, q, table, lens, new_lens, scale, out): the result, or None
@@ -124,17 +136,16 @@ PyObject* py_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (status == cudaStreamCaptureStatusNone) capture = 0;
   at::Tensor out = a[6] == Py_None ? at::empty_like(q) : THPVariable_Unpack(a[6]);
   if (!readable(out, false)) Py_RETURN_NONE;
+  at::Tensor& space = space_of(c->device, st, capture);
   int rc = PBS_ERR_SHAPE;
-  at::Tensor* space = &space_of(c->device, st, capture, PBS_PAGED_COUNTER_BYTES);
   for (int round = 0; rc == PBS_ERR_SHAPE && round < 2; ++round) {
-    if (round == 1) {                                              // too small, perhaps
+    if (round == 1 || !space.defined()) {                          // too small, perhaps
       int64_t need = 0;
-      if (c->workspace(c->c, &batch, (int32_t)q.size(1), &need) != PBS_OK || need <= space->numel()) Py_RETURN_NONE;
-      space = &space_of(c->device, st, capture, need);
+      if (c->workspace(c->c, &batch, (int32_t)q.size(1), &need) != PBS_OK || (space.defined() && need <= space.numel())) Py_RETURN_NONE;
+      space = at::zeros({need}, at::TensorOptions().dtype(at::kByte).device(at::Device(at::kCUDA, (c10::DeviceIndex)c->device)));
     }
-    const int64_t bytes = space->numel();
-    void* const at = space->data_ptr();
-    rc = c->attn(c->c, &batch, (int32_t)q.size(1), q.data_ptr(), q.strides().data(), out.data_ptr(), out.strides().data(), (float)scale, at, bytes, st);
+    rc = c->attn(c->c, &batch, (int32_t)q.size(1), q.data_ptr(), q.strides().data(), out.data_ptr(), out.strides().data(), (float)scale,
+                 space.data_ptr(), space.numel(), st);
   }
   if (rc != PBS_OK) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));

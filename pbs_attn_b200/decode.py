@@ -263,11 +263,12 @@ def _workspace(device: torch.device, need: int) -> torch.Tensor:
         space[:_cabi.PAGED_COUNTER_BYTES].zero_()
         return space
     key = (device.index, torch.cuda.current_stream(device).cuda_stream)
-    space = _WORKSPACES.get(key)
+    space = _WORKSPACES.pop(key, None)                     # (back in behind the others: what was used longest ago goes first)
     if space is None or space.numel() < need:
         while len(_WORKSPACES) >= _MAX_WORKSPACES:
             _WORKSPACES.pop(next(iter(_WORKSPACES), None), None)
-        space = _WORKSPACES[key] = torch.zeros(need, dtype=torch.uint8, device=device)
+        space = torch.zeros(need, dtype=torch.uint8, device=device)
+    _WORKSPACES[key] = space
     return space
 
 

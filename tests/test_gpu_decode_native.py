@@ -142,3 +142,57 @@ def test_captures_have_their_own_workspace():
     cache.check_status()
     torch.cuda.synchronize()
     del graphs
+
+
+def _captures(n, q, cache, table, lens):
+    for _ in range(n):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = paged_attn(q, cache, table, lens)
+        g.replay()
+        torch.cuda.synchronize()
+        del g, out
+
+
+def paged_attn(*a, **kw):
+    from pbs_attn_b200.decode import paged_attn_fwd
+    return paged_attn_fwd(*a, **kw)
+
+
+def _filled(n=2000):
+    from pbs_attn_b200.decode import paged_kv_append
+    cache = make_cache(300, 16, 2, 64, torch.float16, 4, 32)
+    past = torch.randn(1, 2, n, 64, device="cuda").to(torch.float16)
+    table, lens = make_table(cache, [n]), ints(n)
+    paged_kv_append(cache, past, past, table, lens, new_lens=lens)
+    return torch.randn(1, 8, 1, 64, device="cuda").to(torch.float16), cache, table, lens
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_captures_and_streams_leave_the_memory_of_the_stream_in_use(native):
+    """A stream that keeps calling keeps its memory: no call on it allocates, however many captures and other streams come between."""
+    q, cache, table, lens = _filled()
+    if not native:
+        cache._native = None
+    out = torch.empty_like(q)
+    want = paged_attn(q, cache, table, lens)
+    torch.cuda.synchronize()
+    count = lambda: torch.cuda.memory_stats()["allocation.all.allocated"]  # noqa: E731
+    for s in [torch.cuda.Stream() for _ in range(12)]:
+        _captures(1, q, cache, table, lens)
+        with torch.cuda.stream(s):
+            paged_attn(q, cache, table, lens)
+        s.synchronize()
+        before = count()
+        paged_attn(q, cache, table, lens, out=out)
+        assert count() == before and torch.equal(out, want)
+
+
+def test_memory_of_captures_that_are_gone_is_given_back():
+    q, cache, table, lens = _filled()
+    cache._host.paged_forget()
+    paged_attn(q, cache, table, lens)
+    _captures(2, q, cache, table, lens)
+    before = torch.cuda.memory_allocated()
+    _captures(12, q, cache, table, lens)
+    assert torch.cuda.memory_allocated() <= before
