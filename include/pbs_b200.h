@@ -343,7 +343,8 @@ int pbs_paged_gather(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* ba
                      void* v, const int64_t v_strides[4], void* stream);
 
 /* Causal attention of the new tokens' queries, q (B, q_heads, S, D), over the cache: token i sees the positions up to its own.
- * out has q's shape; rows that see nothing are 0.  Softmax and sums are held in 32 bits.  Range for 4 bits: |q| and |v| up to 2^100 in bf16
+ * out has q's shape; rows that see nothing are 0.  Softmax and sums are held in 32 bits.  Range for 16 bits: that of the type (bf16
+ * values below 2^-90 may count as 0); for 4 bits: |q| and |v| up to 2^100 in bf16
  * (what is 2^29 below the largest of a query's row counts as 0); fp16 values cannot leave it.  What a row does not see does not
  * reach it, infinities and NaNs included, and every bit of its result depends on what it sees alone.
  * The blocks of the kernel wait for one another (it is launched cooperatively) where a sequence may be worked on by several.

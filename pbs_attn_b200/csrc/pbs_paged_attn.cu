@@ -190,11 +190,15 @@ __device__ __forceinline__ void load_params(uint32_t (&w)[C::NG], const uint8_t*
 //         code - 8 then and not on the code (3.1e-4, of which the result's own rounding is 2.1e-4);
 //   bf16: every kShiftEvery tiles the sums are moved by what one of each group's has come to, and that is kept aside (1.7e-3, the result's
 //         own rounding).  The other way costs 10 % of the time where it goes into arithmetic, this one 1.
+//
+// 16 bits: what a weight meets is a value of the type.  In fp16 that is up to 2^16 and 32 bits have room for it; bf16's values go up to 2^128, so its
+// weights, which are bf16 themselves, are kept 2^40 smaller: 2^25 tokens of the largest value and weight add up to less than 2^128.
 constexpr int kShiftEvery = 8;
 
 template <class C>
 struct Warp {
   using T = typename C::T;
+  static constexpr int kRoom = C::BITS == 16 && C::DT == PBS_BF16 ? 40 : 0;        // powers of 2 that weights are kept smaller by
   float o[C::D / 16][C::NT][4];
   float om[C::BITS == 4 ? C::NG : 1][C::NT][2];                    // sums of p * lo, this lane's tokens
   float l[C::NT][2], ref[C::NT][2];
@@ -327,7 +331,7 @@ struct Warp {
         }
         if (!(need & 0x11111111u << lane % 4)) continue;           // (whole columns of lanes agree)
         const float old = ref[n][c];
-        if (most > -CUDART_INF_F) ref[n][c] = fmaxf(old, most + (C::BITS == 4 ? __log2f(step) : 0.f) - 7.f);
+        if (most > -CUDART_INF_F) ref[n][c] = fmaxf(old, most + (C::BITS == 4 ? __log2f(step) : (float)kRoom) - 7.f);
         const float keep = ref[n][c] == old ? 1.f : exp2_fast(old - ref[n][c]);
         l[n][c] *= keep;
 #pragma unroll
@@ -411,7 +415,7 @@ struct Warp {
     }
     uint32_t vp[C::MT][2][C::NG];
     float wide[C::NT][2];
-    float widest = 1.f;
+    float widest = (float)(1ull << kRoom);
     if constexpr (C::BITS == 4) {
       constexpr float kLeast = 0x1p-40f;                           // (weights stay below 2^55, their sum within 32 bits' range)
       widest = kLeast;

@@ -1,0 +1,41 @@
+"""Values far from 1 in the attention over a paged cache, against the formula in 64 bits on the values that the cache stands for."""
+import math
+
+import pytest
+import torch
+
+from paged_ref import assert_within, attention, ints, make_cache, make_table, pages_for
+
+pytestmark = pytest.mark.gpu
+
+
+def _run(q, k, v, bits, group, dtype, scale=None, ps=16):
+    """Attention of the queries (1, Hq, S, D) over keys and values (1, 1, n, D)."""
+    from pbs_attn_b200.decode import paged_attn_fwd, paged_kv_append
+    n, D = k.shape[2:]
+    cache = make_cache(pages_for([n], ps), ps, 1, D, dtype, bits, group)
+    table = make_table(cache, [n])
+    q, k, v = (t.to(dtype) for t in (q, k, v))
+    paged_kv_append(cache, k, v, table, ints(n))
+    got = paged_attn_fwd(q, cache, table, ints(n), scale=scale)
+    cache.check_status()
+    assert_within(got, *attention(q, cache, table, [n], None, scale))
+    return got
+
+
+def _random(n, D=128, S=1, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [torch.randn(1, h, s, D, generator=g, device="cuda") for h, s in ((4, S), (1, n), (1, n))]
+
+
+@pytest.mark.parametrize("S", [1, 5])
+@pytest.mark.parametrize("n", [1, 100, 20000])
+def test_values_up_to_the_largest_that_16_bits_hold(n, S):
+    """The weights' sum is not 1 while the sums grow: that must not cost the values their range."""
+    for dtype in (torch.bfloat16, torch.float16):
+        q, k, v = _random(n, S=S if n > 1 else 1)
+        _run(q * 0.1, k, v.clamp(-1, 1).sign() * torch.finfo(dtype).max * 0.9, 16, 0, dtype)
+        same = torch.linspace(-0.9, 0.9, 128, device="cuda").expand_as(v) * torch.finfo(dtype).max
+        _run(q * 0.1, k, same, 16, 0, dtype)
+        rise = torch.linspace(0, 2, n, device="cuda")[:, None] * q[0, 0, 0] / q[0, 0, 0].norm()
+        _run(q, k + 4 * rise, same, 16, 0, dtype)
