@@ -155,6 +155,18 @@ __device__ __forceinline__ float low_of(uint32_t w) {
   else return __uint_as_float(w & 0xffff0000u);
 }
 
+// The larger step and the minimum of larger magnitude of two words of params (NaN gives way).
+template <class T>
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&a), __habs2(*reinterpret_cast<const __half2*>(&b)));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), __habs2(*reinterpret_cast<const __nv_bfloat162*>(&b)));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
 // 16-byte piece `ch` of row `row` in shared memory: neighbouring rows' pieces lie in different banks, so eight rows are read at once.
 template <class C>
 __device__ __forceinline__ int piece(int row, int ch) {
@@ -191,6 +203,9 @@ __device__ __forceinline__ void load_params(uint32_t (&w)[C::NG], const uint8_t*
 //   bf16: every kShiftEvery tiles the sums are moved by what one of each group's has come to, and that is kept aside (1.7e-3, the result's
 //         own rounding).  The other way costs 10 % of the time where it goes into arithmetic, this one 1.
 //
+// In bf16 a minimum may be much larger than any step (a group of equal values has none), up to 2^128, and 32 bits hold its products with weights if
+// it counts as a step of 2^-64 of it: they stay below 2^79.
+//
 // 16 bits: what a weight meets is a value of the type.  In fp16 that is up to 2^16 and 32 bits have room for it; bf16's values go up to 2^128, so its
 // weights, which are bf16 themselves, are kept 2^40 smaller: 2^25 tokens of the largest value and weight add up to less than 2^128.
 constexpr int kShiftEvery = 8;
@@ -198,6 +213,7 @@ constexpr int kShiftEvery = 8;
 template <class C>
 struct Warp {
   using T = typename C::T;
+  [[maybe_unused]] static constexpr float kLeast = 0x1p-40f;                        // (weights stay below 2^55)
   static constexpr int kRoom = C::BITS == 16 && C::DT == PBS_BF16 ? 40 : 0;        // powers of 2 that weights are kept smaller by
   float o[C::D / 16][C::NT][4];
   float om[C::BITS == 4 ? C::NG : 1][C::NT][2];                    // sums of p * lo, this lane's tokens
@@ -306,12 +322,18 @@ struct Warp {
     }
   }
 
+  // What the weights of tokens meet, for the largest of their steps and minima.
+  static __device__ __forceinline__ float met(uint32_t w) {
+    if constexpr (C::DT == PBS_BF16) return fmaxf(fmaxf(step_of<T>(w), low_of<T>(w) * 0x1p-64f), kLeast);
+    else return fmaxf(step_of<T>(w), kLeast);
+  }
+
   static __device__ __forceinline__ bool too_large(float weight, float wide, float ref) {
     return !(weight * wide <= 32768.f) || ref == -CUDART_INF_F;
   }
 
-  // Raises the references of the queries that need it to this tile's scores (x, in powers of 2; wide: the largest step that a query
-  // sees), and weighs the tile anew.  A query's reference depends on what it sees alone, and so does every bit of its result.
+  // Raises the references of the queries that need it to this tile's scores (x, in powers of 2; wide: the most that weights of
+  // what a query sees meet), and weighs the tile anew.  A query's reference depends on what it sees alone, and so does every bit of its result.
   __device__ __forceinline__ void raise(const float (&x)[C::MT][C::NT][4], float (&p)[C::MT][C::NT][4], const float (&wide)[C::NT][2]) {
 #pragma unroll
     for (int n = 0; n < C::NT; ++n)
@@ -417,20 +439,19 @@ struct Warp {
     float wide[C::NT][2];
     float widest = (float)(1ull << kRoom);
     if constexpr (C::BITS == 4) {
-      constexpr float kLeast = 0x1p-40f;                           // (weights stay below 2^55, their sum within 32 bits' range)
-      widest = kLeast;
-      float steps[C::MT][2];
+      uint32_t token[C::MT][2], all = 0;
       const uint8_t* params = stage + 2 * C::TILE * C::ROW + C::TILE * C::PROW;
 #pragma unroll
       for (int m = 0; m < C::MT; ++m)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           load_params<C>(vp[m][h], params + (16 * m + lane / 4 + 8 * h) * C::PROW);
-          steps[m][h] = kLeast;
+          token[m][h] = 0;
 #pragma unroll
-          for (int g = 0; g < C::NG; ++g) steps[m][h] = fmaxf(steps[m][h], step_of<T>(vp[m][h][g]));
-          widest = fmaxf(widest, steps[m][h]);
+          for (int g = 0; g < C::NG; ++g) token[m][h] = larger<T>(token[m][h], vp[m][h][g]);
+          all = larger<T>(all, token[m][h]);
         }
+      widest = met(all);
       if constexpr (MASKED) {
 #pragma unroll
         for (int n = 0; n < C::NT; ++n)
@@ -441,7 +462,7 @@ struct Warp {
             for (int m = 0; m < C::MT; ++m)
 #pragma unroll
               for (int h = 0; h < 2; ++h)
-                if (seen[m][n][2 * h + c]) wide[n][c] = fmaxf(wide[n][c], steps[m][h]);
+                if (seen[m][n][2 * h + c]) wide[n][c] = fmaxf(wide[n][c], met(token[m][h]));
           }
       }
     }

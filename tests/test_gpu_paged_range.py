@@ -39,3 +39,21 @@ def test_values_up_to_the_largest_that_16_bits_hold(n, S):
         _run(q * 0.1, k, same, 16, 0, dtype)
         rise = torch.linspace(0, 2, n, device="cuda")[:, None] * q[0, 0, 0] / q[0, 0, 0].norm()
         _run(q, k + 4 * rise, same, 16, 0, dtype)
+
+
+@pytest.mark.parametrize("group", [32, 64])
+@pytest.mark.parametrize("S", [1, 3])
+@pytest.mark.parametrize("first", ["nothing", "zeros", "small"])
+def test_large_groups_without_a_range(group, S, first):
+    """All channels of a group alike: its step is 0 and its minimum large, and the weights, which steps hold back, must not outgrow it."""
+    n = 900
+    for size in (2.0 ** 60, 2.0 ** 80, 2.0 ** 99):
+        q, k, v = _random(n, S=S)
+        flat = v.unflatten(-1, (-1, group))[..., :1].sign().expand(-1, -1, -1, -1, group).flatten(-2) * size
+        if first == "zeros":
+            flat[:, :, :400] = 0
+        if first == "small":
+            flat[:, :, :400] = v[:, :, :400] * 2.0 ** -70
+        _run(q, k, flat, 4, group, torch.bfloat16)
+        rise = torch.linspace(-2, 2, n, device="cuda")[:, None] * q[0, 0, 0] / q[0, 0, 0].norm()
+        _run(q, k + 4 * rise, flat, 4, group, torch.bfloat16)
