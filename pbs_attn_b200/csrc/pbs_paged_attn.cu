@@ -213,7 +213,6 @@ constexpr int kShiftEvery = 8;
 template <class C>
 struct Warp {
   using T = typename C::T;
-  [[maybe_unused]] static constexpr float kLeast = 0x1p-40f;                        // (weights stay below 2^55)
   static constexpr int kRoom = C::BITS == 16 && C::DT == PBS_BF16 ? 40 : 0;        // powers of 2 that weights are kept smaller by
   float o[C::D / 16][C::NT][4];
   float om[C::BITS == 4 ? C::NG : 1][C::NT][2];                    // sums of p * lo, this lane's tokens
@@ -322,38 +321,51 @@ struct Warp {
     }
   }
 
-  // What the weights of tokens meet, for the largest of their steps and minima.
+  // What the weights of tokens meet, for the largest of their steps and minima; at least `least`, for weights to stay below 2^85.
+  static __device__ __forceinline__ constexpr float least() { return C::DT == PBS_BF16 ? 0x1p-70f : 0x1p-40f; }
   static __device__ __forceinline__ float met(uint32_t w) {
-    if constexpr (C::DT == PBS_BF16) return fmaxf(fmaxf(step_of<T>(w), low_of<T>(w) * 0x1p-64f), kLeast);
-    else return fmaxf(step_of<T>(w), kLeast);
+    if constexpr (C::DT == PBS_BF16) return fmaxf(fmaxf(step_of<T>(w), low_of<T>(w) * 0x1p-64f), least());
+    else return fmaxf(step_of<T>(w), least());
   }
 
   static __device__ __forceinline__ bool too_large(float weight, float wide, float ref) {
     return !(weight * wide <= 32768.f) || ref == -CUDART_INF_F;
   }
 
-  // Raises the references of the queries that need it to this tile's scores (x, in powers of 2; wide: the most that weights of
-  // what a query sees meet), and weighs the tile anew.  A query's reference depends on what it sees alone, and so does every bit of its result.
-  __device__ __forceinline__ void raise(const float (&x)[C::MT][C::NT][4], float (&p)[C::MT][C::NT][4], const float (&wide)[C::NT][2]) {
+  // Raises the references of the queries that need it to the largest product of this tile (x: scores, in powers of 2; wide: the most that weights
+  // of what a query sees meet), and weighs the tile anew.  The largest product and not the largest score and step: a token that hardly weighs
+  // must not push the weights of the others, whose steps may be much smaller, out of fp16.
+  __device__ __forceinline__ void raise(const float (&x)[C::MT][C::NT][4], float (&p)[C::MT][C::NT][4], const float (&wide)[C::NT][2],
+                                        const uint32_t (&vp)[C::MT][2][C::NG]) {
+    float meets[C::MT][2];                                         // by token, in powers of 2
+#pragma unroll
+    for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        meets[m][h] = (float)kRoom;
+        if constexpr (C::BITS == 4) {
+          uint32_t w = 0;
+#pragma unroll
+          for (int g = 0; g < C::NG; ++g) w = larger<T>(w, vp[m][h][g]);
+          meets[m][h] = __log2f(fminf(met(w), 0x1p127f));
+        }
+      }
 #pragma unroll
     for (int n = 0; n < C::NT; ++n)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float most = -CUDART_INF_F, weight = 0.f, step = wide[n][c];
+        float most = -CUDART_INF_F, weight = 0.f;
 #pragma unroll
         for (int m = 0; m < C::MT; ++m) {
-          most = fmaxf(most, fmaxf(x[m][n][c], x[m][n][c + 2]));
+          most = fmaxf(most, fmaxf(x[m][n][c] + meets[m][0], x[m][n][c + 2] + meets[m][1]));
           weight = fmaxf(weight, fmaxf(p[m][n][c], p[m][n][c + 2]));
         }
-        const uint32_t need = __ballot_sync(0xffffffffu, too_large(weight, step, ref[n][c]));
+        const uint32_t need = __ballot_sync(0xffffffffu, too_large(weight, wide[n][c], ref[n][c]));
 #pragma unroll
-        for (int s = 4; s < 32; s <<= 1) {
-          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
-          step = fmaxf(step, __shfl_xor_sync(0xffffffffu, step, s));
-        }
+        for (int s = 4; s < 32; s <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
         if (!(need & 0x11111111u << lane % 4)) continue;           // (whole columns of lanes agree)
         const float old = ref[n][c];
-        if (most > -CUDART_INF_F) ref[n][c] = fmaxf(old, most + (C::BITS == 4 ? __log2f(step) : (float)kRoom) - 7.f);
+        if (most > -CUDART_INF_F) ref[n][c] = fmaxf(old, most - 7.f);
         const float keep = ref[n][c] == old ? 1.f : exp2_fast(old - ref[n][c]);
         l[n][c] *= keep;
 #pragma unroll
@@ -457,7 +469,7 @@ struct Warp {
         for (int n = 0; n < C::NT; ++n)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            wide[n][c] = kLeast;
+            wide[n][c] = least();
 #pragma unroll
             for (int m = 0; m < C::MT; ++m)
 #pragma unroll
@@ -488,7 +500,7 @@ struct Warp {
             for (int c = 0; c < 4; ++c) x[m][n][c] *= c % 2 ? f.y : f.x;
         }
       }
-      raise(x, p, wide);
+      raise(x, p, wide, vp);
     }
 #pragma unroll
     for (int n = 0; n < C::NT; ++n)

@@ -57,3 +57,27 @@ def test_large_groups_without_a_range(group, S, first):
         _run(q, k, flat, 4, group, torch.bfloat16)
         rise = torch.linspace(-2, 2, n, device="cuda")[:, None] * q[0, 0, 0] / q[0, 0, 0].norm()
         _run(q, k + 4 * rise, flat, 4, group, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype,large,small", [(torch.float16, 60000.0, 2.0 ** -13), (torch.bfloat16, 2.0 ** 40, 2.0 ** -20)])
+@pytest.mark.parametrize("group", [32, 64])
+@pytest.mark.parametrize("S", [1, 3])
+def test_small_values_beside_large_ones_that_hardly_weigh(dtype, large, small, group, S):
+    """Every other token is large, but its score is so far below that it leaves nothing: the small ones keep their codes."""
+    n = 700
+    q, k, v = _random(n, S=S)
+    shared = torch.randn(128, generator=torch.Generator(device="cuda").manual_seed(9), device="cuda")
+    shared /= shared.norm()
+    odd = (torch.arange(n, device="cuda") % 2 == 1)[:, None]
+    # scores of the two differ by 2 * 20 * 40 / sqrt(128) = 141 and more than 2^200 in weight
+    q, k = q * 0.1 + 40 * shared, k + torch.where(odd, -20.0, 20.0) * shared
+    _run(q, k, torch.where(odd, v.sign() * large, v * small), 4, group, dtype)
+
+
+@pytest.mark.parametrize("bits,group", [(16, 0), (4, 32), (4, 64)])
+def test_values_that_are_all_small(bits, group):
+    """Weights make up for it, as far as the header's range goes."""
+    for size in (2.0 ** -30, 2.0 ** -60, 2.0 ** -78):
+        q, k, v = _random(900, S=3)
+        _run(q, k, v * size, bits, group, torch.bfloat16)
+    _run(q, k, v * 2.0 ** -13, bits, group, torch.float16)
