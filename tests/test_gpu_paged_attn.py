@@ -356,3 +356,21 @@ def test_the_largest_batch():
     cache.check_status()
     for b in (0, 1, 17, 2000, 4000, 4095):
         assert_within(got[b:b + 1], *attention(q[b:b + 1], cache, table[b:b + 1], [lens[b]]))
+
+
+@pytest.mark.parametrize("bits,group", FORMATS)
+def test_values_of_others_leave_a_row_its_bits(bits, group):
+    """Other sequences' values, far larger ones among them, and other queries do not reach a row, lengths and sizes being the same."""
+    from pbs_attn_b200.decode import paged_attn_fwd, paged_kv_append
+    lens, D = [3000, 500, 70], 128
+    q, cache, table = _case(lens, S=2, bits=bits, group=group)
+    want = paged_attn_fwd(q, cache, table, ints(*lens))
+    other = torch.randn(1, 2, 500, D, device="cuda").to(q.dtype) * 2.0 ** 20
+    paged_kv_append(cache, other, other, table[1:2], ints(500))
+    bad = q.clone(memory_format=torch.preserve_format)
+    bad[1] *= 100
+    bad[0, 3] *= 50
+    got = paged_attn_fwd(bad, cache, table, ints(*lens))
+    cache.check_status()
+    rows = torch.arange(8, device="cuda") != 3
+    assert torch.equal(got[0, rows], want[0, rows]) and torch.equal(got[2], want[2]) and not torch.equal(got[1], want[1])
