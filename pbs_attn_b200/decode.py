@@ -201,6 +201,8 @@ def paged_kv_append(cache: PagedKVCache, key_states: torch.Tensor, value_states:
             query_out = torch.empty_like(query_states)
         else:
             _written("query_out", query_out, query_states)
+    elif query_out is not None:
+        raise ValueError("query_out is for query_states, which are not given")
     rows, cs = 0, None
     if cos is not None:
         D = cache.head_dim

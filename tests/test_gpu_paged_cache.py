@@ -137,6 +137,18 @@ def test_queries_rotated_in_place_and_into_a_given_tensor():
     assert _append(cache, k, k, table, ints(20), cos=cos, sin=sin, query_states=q, query_out=q) is q and torch.equal(q, want)
 
 
+@pytest.mark.parametrize("rope", [True, False])
+def test_a_place_for_queries_that_are_not_given_is_refused(rope):
+    """It would come back as it was."""
+    from pbs_attn_b200.decode import paged_kv_append
+    cache = make_cache(3, 16, 2, 128, torch.bfloat16, 4, 64)
+    table = make_table(cache, [20])
+    k = _inputs(1, 2, 3, 128, torch.bfloat16, 2)
+    cos, sin = rope_tables(32, 128, torch.bfloat16) if rope else (None, None)
+    with pytest.raises(ValueError, match="query_out"):
+        paged_kv_append(cache, k, k, table, ints(20), cos=cos, sin=sin, query_out=torch.zeros(1, 4, 3, 128, dtype=torch.bfloat16, device="cuda"))
+
+
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_a_group_that_is_not_finite_reads_back_as_nan(value, dtype):
