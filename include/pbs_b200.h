@@ -310,7 +310,8 @@ typedef struct {
 #define PBS_PAGED_BAD_PAGE 1    /* a page number outside the pool: such a token is neither written nor attended  */
 #define PBS_PAGED_BAD_LENGTH 2  /* a sequence longer than its row of the block table: it ends with that row      */
 #define PBS_PAGED_BAD_ROTARY 3  /* a position behind the rotary tables: the token is neither rotated nor written */
-#define PBS_PAGED_TIMEOUT 4     /* pbs_paged_attn: a bounded wait ran out; the output is invalid, and the workspace has to be cleared */
+#define PBS_PAGED_TIMEOUT 4     /* pbs_paged_attn: a bounded wait ran out; the output is invalid, and those of later calls with the same
+                                   workspace are until its first PBS_PAGED_COUNTER_BYTES have been cleared */
 
 /* The sequences of a call.  seq_lens counts the new tokens in: token i of the new_lens[b] new ones of sequence b is at
  * position seq_lens[b] - new_lens[b] + i.  Tokens at negative positions are left out (an unused row of a batch has length

@@ -53,7 +53,8 @@ def _raise_fault(word: C.c_int32):
         host = _cabi.load_host()
         if host is not None:
             host.paged_forget()
-        raise _cabi.PbsError("paged attention: a bounded wait ran out in an earlier call on this device; its output is invalid")
+        raise _cabi.PbsError("paged attention: a bounded wait ran out in an earlier call on this device; its output is invalid, and "
+                             "so are those of the attention calls enqueued behind it up to now")
     raise _cabi.PbsError(f"paged cache: {_FAULTS.get(code, code)} (in an earlier call on this device, which left the tokens concerned out)")
 
 
