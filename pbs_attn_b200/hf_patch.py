@@ -102,14 +102,15 @@ def _takes_grouped_kv(prefill_fn) -> bool:
     return kern in (permuted_block_sparse_attn_fwd, MeanPooling_prefill) or bool(getattr(kern, "takes_grouped_kv", False))
 
 
-def _grouped(prefill_fn):
-    """``prefill_fn`` as a function of queries and un-repeated keys and values."""
-    if _takes_grouped_kv(prefill_fn):
-        return prefill_fn
-
+def _grouped(prefill_fn, attn):
+    """``prefill_fn`` as the attention layer ``attn`` calls it: a function of queries and un-repeated keys and values."""
     def call(q, k, v):
-        n_rep = max(1, q.shape[1] // k.shape[1])
-        return prefill_fn(q, repeat_kv(k, n_rep), repeat_kv(v, n_rep))
+        if not _takes_grouped_kv(prefill_fn):
+            n_rep = max(1, q.shape[1] // max(1, k.shape[1]))
+            k, v = repeat_kv(k, n_rep), repeat_kv(v, n_rep)
+        if "layer_idx" in _kernel_of(prefill_fn).__code__.co_varnames:
+            return prefill_fn(q, k, v, layer_idx=attn.layer_idx)
+        return prefill_fn(q, k, v)
     return call
 
 
@@ -127,14 +128,15 @@ def patched_attention_forward(
 
     Prompts (q_len > 1) go through ``prefill_fn(query, key, value)`` on (B, H, S, D) tensors after
     projection, RoPE and the KV-cache update; single-token decode goes to the layer's original
-    forward, or with a ``PagedModelCache`` for ``past_key_values`` (``generate``) through that.  Head counts are derived from the projection widths, so a tensor-parallel shard works
+    forward, or with a ``PagedModelCache`` for ``past_key_values`` (``generate``) through that.
+    Head counts are derived from the projection widths, so a tensor-parallel shard works
     unchanged.  Returns ``(attn_output, None)``.
     """
     bsz, q_len, _ = hidden_states.size()
     if hasattr(past_key_values, "attend"):                 # a paged cache (generate.PagedModelCache) takes prompts and single tokens
         if prefill_fn is None:
             raise RuntimeError("prefill_fn required.")
-        return past_key_values.attend(self, hidden_states, _grouped(prefill_fn)), None
+        return past_key_values.attend(self, hidden_states, _grouped(prefill_fn, self)), None
     if q_len <= 1:
         return self.original_forward(hidden_states=hidden_states, position_embeddings=position_embeddings,
                                      attention_mask=attention_mask, past_key_values=past_key_values,
@@ -157,13 +159,7 @@ def patched_attention_forward(
         q, k = apply_rotary_pos_emb(q, k, cos, sin)
     if past_key_values is not None:
         past_key_values.update(k, v, self.layer_idx, {"sin": sin, "cos": cos, "cache_position": cache_position})
-    if not _takes_grouped_kv(prefill_fn):
-        n_rep = max(1, n_q // max(1, n_kv))
-        k, v = repeat_kv(k, n_rep), repeat_kv(v, n_rep)
-    if "layer_idx" in _kernel_of(prefill_fn).__code__.co_varnames:
-        o = prefill_fn(q, k, v, layer_idx=self.layer_idx)
-    else:
-        o = prefill_fn(q, k, v)
+    o = _grouped(prefill_fn, self)(q, k, v)
     o = o.transpose(1, 2).reshape(bsz, q_len, n_q * d)
     return self.o_proj(o), None
 

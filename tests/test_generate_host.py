@@ -71,3 +71,23 @@ def test_everything_runs_with_the_inputs_device_current(fakes):
     assert [w for w, _, _ in fakes] == ["layers", "layers", "graph", "layers", "event", "event"]
     assert all(d == ids.device for _, d, _ in fakes)
     assert all(s == ids.device for w, _, s in fakes if w == "graph")
+
+
+@pytest.mark.parametrize("grouped", [False, True])
+def test_a_prefill_function_is_told_its_layer_in_front_of_a_paged_cache_too(grouped):
+    from pbs_attn_b200.hf_patch import patched_attention_forward
+    told = []
+
+    def fn(q, k, v, layer_idx):
+        told.append((layer_idx, k.shape[1], v.shape[1]))
+        return q
+
+    fn.takes_grouped_kv = grouped
+
+    class Cache:
+        def attend(self, attn, hidden, prefill_fn):
+            return prefill_fn(torch.zeros(1, 8, 5, 4), torch.zeros(1, 2, 5, 4), torch.zeros(1, 2, 5, 4))
+
+    layer = types.SimpleNamespace(layer_idx=3)
+    out, _ = patched_attention_forward(layer, torch.zeros(1, 5, 32), None, None, past_key_values=Cache(), prefill_fn=fn)
+    assert out.shape == (1, 8, 5, 4) and told == [(3, 2, 2) if grouped else (3, 8, 8)]
