@@ -9,6 +9,7 @@ reference patches prompts only and leaves single tokens to the model's own forwa
 """
 from __future__ import annotations
 
+import copy
 from typing import Optional
 
 import torch
@@ -29,6 +30,14 @@ class PagedModelCache:
         first = model.model.layers[0].self_attn
         weight = first.k_proj.weight
         self.head_dim = first.head_dim
+
+        def tables(n):                                     # (of a copy: the module keeps what depends on the length, and the model's is its own)
+            return copy.deepcopy(model.model.rotary_emb)(weight[:1, :1], torch.arange(n, device=weight.device)[None])
+
+        cos, sin = tables(max_tokens)
+        if not torch.equal(cos[:, :2], tables(2)[0][:, :max_tokens]):
+            raise ValueError(f"the model's rotary tables change up to {max_tokens} tokens: keys that are cached rotated would not be the model's")
+        self.cos, self.sin = (t[0].to(weight.dtype).contiguous() for t in (cos, sin))
         heads = weight.shape[0] // self.head_dim           # (of this rank's share, if the model is sharded by heads)
         per = -(-max_tokens // page_size)
         self.layers = [PagedKVCache(batch * per, page_size, heads, self.head_dim, weight.dtype, weight.device, bits, group_size)
@@ -36,8 +45,6 @@ class PagedModelCache:
         self.block_table = torch.arange(batch * per, dtype=torch.int32, device=weight.device).view(batch, per)
         self.seq_lens = torch.zeros(batch, dtype=torch.int32, device=weight.device)
         self.max_tokens, self.tokens = max_tokens, 0
-        cos, sin = model.model.rotary_emb(weight[:1, :1], torch.arange(max_tokens, device=weight.device)[None])
-        self.cos, self.sin = (t[0].to(weight.dtype).contiguous() for t in (cos, sin))
 
     def add(self, tokens: int):
         """Counts the next call's tokens in."""

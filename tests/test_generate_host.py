@@ -91,3 +91,21 @@ def test_a_prefill_function_is_told_its_layer_in_front_of_a_paged_cache_too(grou
     layer = types.SimpleNamespace(layer_idx=3)
     out, _ = patched_attention_forward(layer, torch.zeros(1, 5, 32), None, None, past_key_values=Cache(), prefill_fn=fn)
     assert out.shape == (1, 8, 5, 4) and told == [(3, 2, 2) if grouped else (3, 8, 8)]
+
+
+def _llama(**kw):
+    from transformers import LlamaConfig, LlamaForCausalLM
+    return LlamaForCausalLM(LlamaConfig(vocab_size=300, hidden_size=256, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4,
+                                        num_key_value_heads=2, head_dim=64, max_position_embeddings=64, **kw)).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("rope,changes", [("default", False), ("dynamic", True)])
+def test_rotary_tables_that_change_with_the_length_are_refused(rope, changes):
+    """A cached key was rotated by the tables of its time; where they change as the sequence grows, one set of tables is not the model's."""
+    model = _llama(rope_parameters={"rope_type": rope, "rope_theta": 10000.0, "factor": 2.0})
+    before = model.model.rotary_emb.inv_freq.clone()
+    with pytest.raises(RuntimeError, match="CUDA"):        # (within the length that it was made for: as far as the cache itself)
+        module.PagedModelCache(model, 1, 60)
+    with pytest.raises(ValueError if changes else RuntimeError, match="rotary" if changes else "CUDA"):
+        module.PagedModelCache(model, 1, 200)
+    assert torch.equal(model.model.rotary_emb.inv_freq, before)
