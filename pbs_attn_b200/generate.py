@@ -30,6 +30,9 @@ class PagedModelCache:
         first = model.model.layers[0].self_attn
         weight = first.k_proj.weight
         self.head_dim = first.head_dim
+        window = min((w for layer in model.model.layers if (w := getattr(layer.self_attn, "sliding_window", None))), default=max_tokens)
+        if window < max_tokens:
+            raise ValueError(f"a layer of the model sees a window of {window} tokens, and {max_tokens} are asked for: its steps would see them all")
 
         def tables(n):                                     # (of a copy: the module keeps what depends on the length, and the model's is its own)
             return copy.deepcopy(model.model.rotary_emb)(weight[:1, :1], torch.arange(n, device=weight.device)[None])

@@ -109,3 +109,14 @@ def test_rotary_tables_that_change_with_the_length_are_refused(rope, changes):
     with pytest.raises(ValueError if changes else RuntimeError, match="rotary" if changes else "CUDA"):
         module.PagedModelCache(model, 1, 200)
     assert torch.equal(model.model.rotary_emb.inv_freq, before)
+
+
+def test_layers_that_see_a_window_alone_are_refused_beyond_it():
+    """The steps attend to everything that is cached."""
+    from transformers import Qwen2Config, Qwen2ForCausalLM
+    model = Qwen2ForCausalLM(Qwen2Config(vocab_size=300, hidden_size=256, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4,
+                                         num_key_value_heads=2, use_sliding_window=True, sliding_window=16, max_window_layers=1)).to(torch.bfloat16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        module.PagedModelCache(model, 1, 16)
+    with pytest.raises(ValueError, match="window"):
+        module.PagedModelCache(model, 1, 17)
