@@ -212,7 +212,7 @@ def paged_kv_append(cache: PagedKVCache, key_states: torch.Tensor, value_states:
         if cos.dtype != cache.dtype or sin.dtype != cache.dtype or cos.device != cache.device or sin.device != cache.device:
             raise TypeError(f"cos / sin must be {cache.dtype} on {cache.device}, like the cache")
         if not all(t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s * 2 % 16 for s in t.stride()[:-1]) for t in (cos, sin)) or sin.stride() != cos.stride():
-            cos, sin = cos.contiguous(), sin.contiguous()
+            cos, sin = (t.clone(memory_format=torch.contiguous_format) for t in (cos, sin))
         if cos.dim() == 2:
             rows, cs = cos.shape[0], (C.c_int64 * 3)(0, cos.stride(0), 1)
         else:

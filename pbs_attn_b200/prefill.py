@@ -31,14 +31,14 @@ def _strides(t: torch.Tensor):
 
 def _readable(t: torch.Tensor, need_distinct_heads: bool = False) -> torch.Tensor:
     """Returns ``t`` if the kernels can read it in place (unit head-dim stride, 16-byte aligned
-    rows), else a contiguous copy."""
+    rows), else a contiguous copy (a copy also of a tensor that is dense but begins between the boundaries)."""
     sb, sh, ss, sd = t.stride()
     # the row pieces are 16 bytes, a power of two of elements: one test of the strides' common low bits covers all three
     ok = sd == 1 and ss > 0 and sb >= 0 and sh >= 0 and ((sb | sh | ss) * t.element_size()) % 16 == 0 and t.data_ptr() % 16 == 0
     if ok and need_distinct_heads:
         # the TMA descriptor of the query tensor cannot describe broadcast (stride-0) batch / head dims
         ok = (sb > 0 or t.shape[0] == 1) and (sh > 0 or t.shape[1] == 1)
-    return t if ok else t.contiguous()
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 class _Turn:

@@ -196,3 +196,22 @@ def test_memory_of_captures_that_are_gone_is_given_back():
     before = torch.cuda.memory_allocated()
     _captures(12, q, cache, table, lens)
     assert torch.cuda.memory_allocated() <= before
+
+
+def test_dense_tensors_between_the_16_byte_boundaries():
+    """Queries, results, keys, values and rotary tables that are dense and begin anywhere."""
+    from pbs_attn_b200.decode import paged_kv_append
+    cache, table, lens, q, k, v = _case()
+    cos, sin = rope_tables(128, 128, torch.bfloat16)
+
+    def shifted(t):
+        room = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape)
+        return room.copy_(t)
+
+    want = paged_kv_append(cache, k, v, table, lens, cos=cos, sin=sin, query_states=q)
+    got = paged_kv_append(cache, shifted(k), shifted(v), table, lens, cos=shifted(cos), sin=shifted(sin), query_states=shifted(q), query_out=shifted(q))
+    assert torch.equal(got, want)
+    past = torch.randn(2, 2, 100, 128, device="cuda").to(torch.bfloat16)
+    paged_kv_append(cache, past, past, table, lens, new_lens=lens)
+    out = shifted(q)
+    assert paged_attn(shifted(q), cache, table, lens, out=out) is out and torch.equal(out, paged_attn(q, cache, table, lens))
