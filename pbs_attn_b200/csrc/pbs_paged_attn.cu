@@ -174,6 +174,16 @@ __device__ __forceinline__ int piece(int row, int ch) {
   return row * C::ROW + ((ch ^ ((row / PER) & MASK)) << 4);
 }
 
+// Brings sums from one reference to another, whose difference is d.  References of bf16 caches of 4 bits differ with the steps, too, up to 2^170, while
+// the sums of weights that they are for are of one size: the factor is applied as its root, twice (in `raise`, whose time shows, in two parts
+// where it is that small).
+template <class C>
+__device__ __forceinline__ float factor_of(float d) { return exp2_fast(C::SHIFT > 0 ? 0.5f * d : d); }
+template <class C>
+__device__ __forceinline__ float scaled(float x, float f) { return C::SHIFT > 0 ? x * f * f : x * f; }
+template <class C>
+__device__ __forceinline__ float add_scaled(float f, float x, float sum) { return fmaf(f, C::SHIFT > 0 ? x * f : x, sum); }
+
 // Params of one token, NG words.
 template <class C>
 __device__ __forceinline__ void load_params(uint32_t (&w)[C::NG], const uint8_t* p) {
@@ -366,7 +376,22 @@ struct Warp {
         if (!(need & 0x11111111u << lane % 4)) continue;           // (whole columns of lanes agree)
         const float old = ref[n][c];
         if (most > -CUDART_INF_F) ref[n][c] = fmaxf(old, most - 7.f);
-        const float keep = ref[n][c] == old ? 1.f : exp2_fast(old - ref[n][c]);
+        float d = ref[n][c] == old ? 0.f : old - ref[n][c];
+        if (C::SHIFT > 0 && d < -100.f && old > -CUDART_INF_F) {
+          d += 100.f;
+          l[n][c] *= 0x1p-100f;
+#pragma unroll
+          for (int i = 0; i < C::D / 16; ++i) {
+            o[i][n][c] *= 0x1p-100f;
+            o[i][n][c + 2] *= 0x1p-100f;
+          }
+#pragma unroll
+          for (int g = 0; g < (C::BITS == 4 ? C::NG : 1); ++g) {
+            om[g][n][c] *= 0x1p-100f;
+            if (lane < 4) shift[g * C::COLS + 8 * n + 2 * lane + c] *= 0x1p-100f;
+          }
+        }
+        const float keep = exp2_fast(d);
         l[n][c] *= keep;
 #pragma unroll
         for (int i = 0; i < C::D / 16; ++i) {
@@ -922,13 +947,13 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int v = 0; v < C::WARPS; ++v) {
-        const float rv = refs[v * C::COLS + col], wt = rv == top ? 1.f : exp2_fast(rv - top);
+        const float rv = refs[v * C::COLS + col], wt = rv == top ? 1.f : factor_of<C>(rv - top);
         const float4 y = *reinterpret_cast<const float4*>(sums + (v * C::COLS + col) * C::OROW + d);
-        sum = fmaf(wt, weights[v * C::COLS + col], sum);
-        x.x = fmaf(wt, y.x, x.x);
-        x.y = fmaf(wt, y.y, x.y);
-        x.z = fmaf(wt, y.z, x.z);
-        x.w = fmaf(wt, y.w, x.w);
+        sum = add_scaled<C>(wt, weights[v * C::COLS + col], sum);
+        x.x = add_scaled<C>(wt, y.x, x.x);
+        x.y = add_scaled<C>(wt, y.y, x.y);
+        x.z = add_scaled<C>(wt, y.z, x.z);
+        x.w = add_scaled<C>(wt, y.w, x.w);
       }
       if (i0 == i1) {
         write(col, d, x, sum);
@@ -991,12 +1016,12 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
       for (int k = 0; k < 8; ++k) top = fmaxf(top, rv[k]);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float wt = rv[k] == top ? 1.f : exp2_fast(rv[k] - top);
-        sum = fmaf(wt, lv[k], sum);
-        x.x = fmaf(wt, y[k].x, x.x);
-        x.y = fmaf(wt, y[k].y, x.y);
-        x.z = fmaf(wt, y[k].z, x.z);
-        x.w = fmaf(wt, y[k].w, x.w);
+        const float wt = rv[k] == top ? 1.f : factor_of<C>(rv[k] - top);
+        sum = add_scaled<C>(wt, lv[k], sum);
+        x.x = add_scaled<C>(wt, y[k].x, x.x);
+        x.y = add_scaled<C>(wt, y[k].y, x.y);
+        x.z = add_scaled<C>(wt, y[k].z, x.z);
+        x.w = add_scaled<C>(wt, y[k].w, x.w);
       }
       write(col, d, x, sum);
     }
@@ -1020,18 +1045,18 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
         lv[a] = __ldcg(from(k) + C::COLS * (C::D + 1) + col);
         y[a] = __ldcg(reinterpret_cast<const float4*>(from(k) + col * C::D + d));
       }
-      const float most = fmaxf(top, warp_max(fmaxf(fmaxf(rv[0], rv[1]), fmaxf(rv[2], rv[3])))), keep = top == most ? 1.f : exp2_fast(top - most);
+      const float most = fmaxf(top, warp_max(fmaxf(fmaxf(rv[0], rv[1]), fmaxf(rv[2], rv[3])))), keep = top == most ? 1.f : factor_of<C>(top - most);
       top = most;
-      sum *= keep;
-      x = make_float4(x.x * keep, x.y * keep, x.z * keep, x.w * keep);
+      sum = scaled<C>(sum, keep);
+      x = make_float4(scaled<C>(x.x, keep), scaled<C>(x.y, keep), scaled<C>(x.z, keep), scaled<C>(x.w, keep));
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
-        const float wt = rv[a] == top ? 1.f : exp2_fast(rv[a] - top);
-        sum = fmaf(wt, lv[a], sum);
-        x.x = fmaf(wt, y[a].x, x.x);
-        x.y = fmaf(wt, y[a].y, x.y);
-        x.z = fmaf(wt, y[a].z, x.z);
-        x.w = fmaf(wt, y[a].w, x.w);
+        const float wt = rv[a] == top ? 1.f : factor_of<C>(rv[a] - top);
+        sum = add_scaled<C>(wt, lv[a], sum);
+        x.x = add_scaled<C>(wt, y[a].x, x.x);
+        x.y = add_scaled<C>(wt, y[a].y, x.y);
+        x.z = add_scaled<C>(wt, y[a].z, x.z);
+        x.w = add_scaled<C>(wt, y[a].w, x.w);
       }
     }
     x = make_float4(warp_sum(x.x), warp_sum(x.y), warp_sum(x.z), warp_sum(x.w));

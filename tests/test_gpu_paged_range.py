@@ -81,3 +81,16 @@ def test_values_that_are_all_small(bits, group):
         q, k, v = _random(900, S=3)
         _run(q, k, v * size, bits, group, torch.bfloat16)
     _run(q, k, v * 2.0 ** -13, bits, group, torch.float16)
+
+
+@pytest.mark.parametrize("n", [100, 900, 9000])
+@pytest.mark.parametrize("group", [32, 64])
+@pytest.mark.parametrize("small", [0.0, 2.0 ** -76])
+def test_runs_of_very_different_sizes_keep_their_weights(small, group, n):
+    """Stretches of large values and of none at all: the latter leave nothing but their weights, whose sums are as far apart as the values."""
+    for large in (2.0 ** 50, 2.0 ** 90):
+        for run in (32, 128, 3000):
+            q, k, v = _random(n, S=3)
+            few = (torch.arange(n, device="cuda") // run % 2 == 0)[:, None]
+            for one in (few, ~few):
+                _run(q * 0.3, k, torch.where(one, v * small, v * large), 4, group, torch.bfloat16)
