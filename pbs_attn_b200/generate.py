@@ -20,6 +20,16 @@ from .logits import process_logits
 from .prefill import apply_rope_
 
 
+_STREAMS: dict = {}
+
+
+def _capture_stream(device: torch.device):
+    """One a device, as torch's own default is one of whichever device captured first: libraries keep workspaces by stream."""
+    if device not in _STREAMS:
+        _STREAMS[device] = torch.cuda.Stream(device)
+    return _STREAMS[device]
+
+
 class PagedModelCache:
     """A ``PagedKVCache`` for every layer of a model, with the block table and lengths that they share.
 
@@ -133,7 +143,7 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, bits: int =
             if cuda_graph:
                 torch.cuda.synchronize(input_ids.device)
                 graph = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(graph, stream=torch.cuda.Stream(input_ids.device)):     # (by default one stream of whichever device captured first)
+                with torch.cuda.graph(graph, stream=_capture_stream(input_ids.device)):
                     cache.seq_lens += 1
                     step()
                 more = graph.replay

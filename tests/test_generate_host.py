@@ -50,6 +50,7 @@ def fakes(monkeypatch):
     for name, x in (("device", device), ("graph", graph), ("Event", Event), ("synchronize", lambda d=None: None),
                     ("Stream", lambda d=None: types.SimpleNamespace(device=d)), ("CUDAGraph", lambda: types.SimpleNamespace(replay=lambda: None))):
         monkeypatch.setattr(torch.cuda, name, x)
+    monkeypatch.setattr(module, "_STREAMS", {})
     monkeypatch.setattr(module, "PagedModelCache", Cache)
     monkeypatch.setattr(module, "is_model_supported", lambda m: True)
     monkeypatch.setattr(module, "process_logits", lambda x, **kw: x)

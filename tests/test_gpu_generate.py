@@ -65,6 +65,18 @@ def test_on_a_device_that_is_not_current():
         assert torch.equal(generate(model, ids.to("cuda:1"), 20, repetition_penalty=1.3, cuda_graph=graph).to("cuda"), want)
 
 
+def test_call_after_call_keeps_no_memory():
+    """What libraries keep for the stream of a capture they keep once."""
+    from pbs_attn_b200.generate import generate
+    model = _patched(_model())
+    ids = torch.randint(0, 300, (2, 150), device="cuda")
+    held = []
+    for _ in range(4):
+        generate(model, ids, 6, repetition_penalty=1.3)
+        held.append(torch.cuda.memory_allocated())
+    assert held[3] <= held[0]
+
+
 def test_masks_and_penalties_reach_the_choice():
     from pbs_attn_b200.generate import generate
     model = _patched(_model())
