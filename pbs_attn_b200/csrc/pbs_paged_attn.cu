@@ -175,8 +175,7 @@ __device__ __forceinline__ int piece(int row, int ch) {
 }
 
 // Brings sums from one reference to another, whose difference is d.  References of bf16 caches of 4 bits differ with the steps, too, up to 2^170, while
-// the sums of weights that they are for are of one size: the factor is applied as its root, twice (in `raise`, whose time shows, in two parts
-// where it is that small).
+// the sums of weights that they are for are of one size: the factor is applied as its root, twice.
 template <class C>
 __device__ __forceinline__ float factor_of(float d) { return exp2_fast(C::SHIFT > 0 ? 0.5f * d : d); }
 template <class C>
@@ -376,32 +375,19 @@ struct Warp {
         if (!(need & 0x11111111u << lane % 4)) continue;           // (whole columns of lanes agree)
         const float old = ref[n][c];
         if (most > -CUDART_INF_F) ref[n][c] = fmaxf(old, most - 7.f);
-        float d = ref[n][c] == old ? 0.f : old - ref[n][c];
-        if (C::SHIFT > 0 && d < -100.f && old > -CUDART_INF_F) {
-          d += 100.f;
-          l[n][c] *= 0x1p-100f;
+        if (ref[n][c] != old && old > -CUDART_INF_F) {             // (before the first reference nothing has been summed up)
+          const float keep = factor_of<C>(old - ref[n][c]);
+          l[n][c] = scaled<C>(l[n][c], keep);
 #pragma unroll
           for (int i = 0; i < C::D / 16; ++i) {
-            o[i][n][c] *= 0x1p-100f;
-            o[i][n][c + 2] *= 0x1p-100f;
+            o[i][n][c] = scaled<C>(o[i][n][c], keep);
+            o[i][n][c + 2] = scaled<C>(o[i][n][c + 2], keep);
           }
 #pragma unroll
           for (int g = 0; g < (C::BITS == 4 ? C::NG : 1); ++g) {
-            om[g][n][c] *= 0x1p-100f;
-            if (lane < 4) shift[g * C::COLS + 8 * n + 2 * lane + c] *= 0x1p-100f;
+            om[g][n][c] = scaled<C>(om[g][n][c], keep);
+            if (C::SHIFT > 0 && lane < 4) shift[g * C::COLS + 8 * n + 2 * lane + c] = scaled<C>(shift[g * C::COLS + 8 * n + 2 * lane + c], keep);
           }
-        }
-        const float keep = exp2_fast(d);
-        l[n][c] *= keep;
-#pragma unroll
-        for (int i = 0; i < C::D / 16; ++i) {
-          o[i][n][c] *= keep;
-          o[i][n][c + 2] *= keep;
-        }
-#pragma unroll
-        for (int g = 0; g < (C::BITS == 4 ? C::NG : 1); ++g) {
-          om[g][n][c] *= keep;
-          if (C::SHIFT > 0 && lane < 4) shift[g * C::COLS + 8 * n + 2 * lane + c] *= keep;
         }
 #pragma unroll
         for (int m = 0; m < C::MT; ++m)
