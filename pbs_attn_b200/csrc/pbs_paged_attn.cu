@@ -20,10 +20,12 @@
 // the grid is launched cooperatively): each joins its part of the rows, from the partial results in the order of the CTAs: same bits every time.
 // (With the last CTA of an item joining all of it, one SM read up to 256 KB while the others were done: 5 us instead of 3.)
 //
-// Measured (B200, GPU time): 64 sequences of 12000 to 16384, 8 KV heads of 128, groups of 64, bf16: 203 us for 1.05 GB, 5.1 TB/s, 79 % of the
-// copy rate (the copies alone take 164 us, the arithmetic alone 172: 560 instructions for 32 tokens, half of them on the ALU pipe); one
-// sequence of 131072: 40 us, 3.7 TB/s; of 32768 with 4 KV heads: 13 us.  Pages of 16 bits, 64 sequences of up to 4096: 121 us for 0.8 GB, the
-// copy rate.
+// Measured (B200, GPU time): 64 sequences of 12000 to 16384, 8 KV heads of 128, groups of 64, bf16: 207 us for 1.05 GB, 5.1 TB/s, 77 % of the copy
+// rate; 231 us and 69 % under load for seconds, when the power cap lowers the clock.  (The copies alone take 164 us, the arithmetic alone 172: 575
+// instructions for 32 tokens, half of them on the ALU pipe.)  One sequence of 131072: 41 us, 3.7 TB/s; of 32768 with 4 KV heads: 13 us.  Several
+// queries a head make it arithmetic: 20 (64 sequences of up to 4096) run at 25 % of the copy rate, 32 (8 of up to 8192) at 15; 8 heads of 64
+// channels at 38, two of 256 at 30.  Pages of 16 bits, 64 sequences of up to 4096: 121 us for 0.8 GB, the copy rate, under load too; one of
+// 131072: 89 us, 92 %; 20 queries a head, 8 of up to 8192: 40 us, 64 %.
 //
 // Within a CTA every warp takes every eighth (fourth) tile of 16 or 32 tokens through its own ring of cp.async stages, with its own running
 // reference and sums; warps meet once an item.
@@ -540,7 +542,11 @@ struct Warp {
 #pragma unroll
         for (int n = 0; n < C::NT; ++n)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) b[n][h] = transpose8(pack<T>(p[m][n][2 * h], p[m][n][2 * h + 1]));
+          for (int h = 0; h < 2; ++h) {
+            // rounded to the pages' type, which is what the tensor cores multiply pages of 16 bits by: relative error 2.3e-3 in bf16 and 2.9e-4 in
+            // fp16 (8 sequences of 2000 to 8192), where the result's own rounding leaves 1.7e-3 and 2.1e-4
+            b[n][h] = transpose8(pack<T>(p[m][n][2 * h], p[m][n][2 * h + 1]));
+          }
 #pragma unroll
         for (int i = 0; i < C::D / 16; ++i) {
           uint32_t r[4];

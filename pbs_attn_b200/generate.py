@@ -34,7 +34,9 @@ class PagedModelCache:
     """A ``PagedKVCache`` for every layer of a model, with the block table and lengths that they share.
 
     Handed to the layers of a patched model as ``past_key_values``.  ``seq_lens`` counts the tokens of the current call in before
-    the layers run; a call whose tokens are all that there are is the prompt and goes through the prefill function."""
+    the layers run; a call whose tokens are all that there are is the prompt and goes through the prefill function.  Any later call goes
+    through ``paged_attn_fwd``, which is made for a few tokens: it reads the cache
+    anew for every 32 rows of a KV head (tokens times queries; 16 rows of 256 channels)."""
 
     def __init__(self, model, batch: int, max_tokens: int, bits: int = 16, page_size: int = 64, group_size: int = 64):
         first = model.model.layers[0].self_attn

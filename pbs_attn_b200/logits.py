@@ -28,8 +28,8 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     The history of row b is ``tokens[b, :token_lens[b]]``, the first ``prompt_lens[b]`` of it the prompt (without the lengths: the
     whole row, no prompt; lengths that the row does not have are taken as the nearest that it has).  ``tokens`` and ``bias_ids`` are
     int32 or int64; ids outside 0 .. V - 1 are skipped.  Penalties are numbers or (B,) float32 tensors.  All in 32 bits, rounded
-    once.  Runs on the current stream without synchronising; tokens are counted anew in every call, so nothing has to be kept in
-    step when rows move, leave or take back tokens."""
+    once.  Made for some hundreds of biases a row; thousands work, slowly.  Runs on the current stream without synchronising;
+    tokens are counted anew in every call, so nothing has to be kept in step when rows move, leave or take back tokens."""
     global _host, _address
     if _host is None:
         _host, _address = _cabi.load_host() or False, C.cast(_cabi.load().pbs_process_logits, C.c_void_p).value
