@@ -372,8 +372,8 @@ int pbs_paged_attn(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* batc
 typedef struct {
   int32_t dtype;                  /* pbs_dtype_t of logits and out                              */
   int32_t rows, vocab;
-  int32_t history;                /* entries a row of tokens                                    */
-  int32_t biases;                 /* entries a row of bias_ids and bias_values                  */
+  int32_t history;                /* entries a row of tokens, below 2^30                        */
+  int32_t biases;                 /* entries a row of bias_ids and bias_values, below 2^30      */
   int32_t token_bytes;            /* 4 or 8: integers in tokens                                 */
   int32_t bias_id_bytes;          /* 4 or 8: integers in bias_ids                               */
   int32_t reserved;

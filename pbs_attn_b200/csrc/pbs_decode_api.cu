@@ -152,7 +152,7 @@ int pbs_process_logits(const pbs_logits_t* args, void* stream) {
     set_error("logits: rows of out must not share memory, strides must not be negative");
     return PBS_ERR_LAYOUT;
   }
-  if (a.history < 0 || a.history >= (1 << 30) || a.biases < 0) { set_error("logits: history %d, biases %d", a.history, a.biases); return PBS_ERR_SHAPE; }
+  if (a.history < 0 || a.history >= (1 << 30) || a.biases < 0 || a.biases >= (1 << 30)) { set_error("logits: history %d, biases %d", a.history, a.biases); return PBS_ERR_SHAPE; }
   if (a.tokens && a.token_bytes != 4 && a.token_bytes != 8) { set_error("tokens: integers of %d bytes", a.token_bytes); return PBS_ERR_ARG; }
   if (a.history == 0) a.tokens = nullptr;
   if (a.biases == 0) a.bias_ids = nullptr;

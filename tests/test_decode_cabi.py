@@ -100,3 +100,13 @@ def test_structs_lie_as_in_the_header():
     assert C.sizeof(_cabi.PagedCache) == 4 * 8 + 4 * 24 + 8 * 4 + 8 and _cabi.PagedCache.num_pages.offset == 128
     assert C.sizeof(_cabi.PagedBatch) == 4 * 8 + 4 * 4
     assert _cabi.Logits.logits.offset == 32 and _cabi.Logits.repetition_all.offset == 120 and C.sizeof(_cabi.Logits) == 184
+
+
+def test_numbers_of_biases_that_an_index_cannot_count_are_refused(lib):
+    """A thread's index goes on by 256 behind the last of them."""
+    for n in (1 << 30, 2 ** 31 - 1):
+        d = _cabi.Logits(dtype=_cabi.BF16, rows=1, vocab=100, biases=n, bias_ids=1 << 27, bias_values=1 << 28, bias_id_bytes=8, bias_ids_stride=n,
+                         bias_values_stride=n, logits=1 << 24, out=1 << 25, logits_stride=100, out_stride=100, repetition_all=1.0)
+        before = lib.pbs_launch_count()
+        assert lib.pbs_process_logits(C.byref(d), None) == -1 and b"biases" in lib.pbs_last_error_string()
+        assert lib.pbs_launch_count() == before
