@@ -1072,7 +1072,7 @@ int launch(AttnArgs p, void* workspace, bool measure, int64_t* bytes, cudaStream
   const int64_t rows = (int64_t)p.group * p.a.b.new_tokens;
   p.row_tiles = (int)((rows + C::COLS - 1) / C::COLS);
   const int64_t most = ((int64_t)p.a.b.max_pages * p.a.c.page_size / C::UNIT + 1) * p.row_tiles * p.a.c.kv_heads * p.a.b.batch;
-  if (most > INT_MAX) { set_error("paged attention: sequences x heads x tokens beyond what a call can count"); return PBS_ERR_SHAPE; }
+  if (most > INT_MAX - (1 << 20)) { set_error("paged attention: sequences x heads x tokens beyond what a call can count"); return PBS_ERR_SHAPE; }
   // One CTA a SM where that leaves at most kShort units each (by the table, whose sequences may be shorter): what a second one saves on a
   // few tiles goes on joining twice the parts.  One sequence of 32768 with 4 KV heads 13.6 us so, 14.7 with two; of 131072 with 8, 28
   // units each, 47.4 against 44.5.

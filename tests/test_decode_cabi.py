@@ -110,3 +110,11 @@ def test_numbers_of_biases_that_an_index_cannot_count_are_refused(lib):
         before = lib.pbs_launch_count()
         assert lib.pbs_process_logits(C.byref(d), None) == -1 and b"biases" in lib.pbs_last_error_string()
         assert lib.pbs_launch_count() == before
+
+
+def test_units_that_the_dealing_cannot_count_are_refused(lib):
+    """The last block's share may end behind the last unit: that has to fit 32 bits as well."""
+    n = C.c_int64()
+    call = lambda pages: lib.pbs_paged_attn_workspace(C.byref(_cache(kv_heads=1)), C.byref(_batch(max_pages=pages, batch=510)), 1, C.byref(n))  # noqa: E731
+    assert call((4210752 - 1) * 16) == -1 and b"count" in lib.pbs_last_error_string()       # 510 * 4210752 = 2^31 - 128 units
+    assert call((4200000 - 1) * 16) == 0
