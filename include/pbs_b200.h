@@ -286,24 +286,28 @@ int pbs_prefill_fwd(const pbs_shape_t* shape,
  *              high half of byte i; params are (pages, Hkv, page_size, D / group_size, 2) of `dtype`: step and
  *              minimum of each group of group_size neighbouring channels of one token and head.  A code c
  *              stands for minimum + c * step.
+ *   bits = 8:  k and v are (pages, Hkv, page_size, D) signed bytes, -127 .. 127; params are (pages, Hkv,
+ *              page_size / block_size) floats: a scale for each block of block_size neighbouring tokens of a
+ *              page and head.  A code c stands for c * scale.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct {
   void* k;
   void* v;
-  void* k_params;          /* bits = 4 only (NULL otherwise)                                            */
+  void* k_params;          /* bits = 4 and 8 only (NULL otherwise)                                      */
   void* v_params;
-  int64_t k_strides[3];    /* page, head, slot, in elements: of dtype for 16 bits, bytes for 4.  Rows   */
-  int64_t v_strides[3];    /* start on 16-byte boundaries                                               */
-  int64_t k_params_strides[3];   /* page, head, slot, in elements of dtype; a token's row of steps and  */
-  int64_t v_params_strides[3];   /* minima is dense and starts on a multiple of min(16, its size) bytes */
+  int64_t k_strides[3];    /* page, head, slot, in elements: of dtype for 16 bits, bytes for 8 and 4.   */
+  int64_t v_strides[3];    /* Rows start on 16-byte boundaries                                          */
+  int64_t k_params_strides[3];   /* 4 bits: page, head, slot, in elements of dtype; a token's row of    */
+  int64_t v_params_strides[3];   /* steps and minima is dense and starts on a multiple of min(16, its
+                                    size) bytes.  8 bits: page, head, block, in floats                  */
   int32_t num_pages;
   int32_t page_size;       /* a power of two, 16 .. 1024                                                */
   int32_t kv_heads;
   int32_t head_dim;        /* 64, 128 or 256                                                            */
   int32_t dtype;           /* PBS_BF16 or PBS_FP16                                                      */
-  int32_t bits;            /* 16 or 4                                                                   */
+  int32_t bits;            /* 16, 8 or 4                                                                */
   int32_t group_size;      /* bits = 4: 32 or 64                                                        */
-  int32_t reserved;
+  int32_t block_size;      /* bits = 8: 16, 32 or 64, at most page_size                                 */
   int32_t* status;         /* one word that the device can write (pinned host memory will do); a call   */
 } pbs_paged_cache_t;       /* that finds one of the faults below stores it there and works around it    */
 
@@ -332,14 +336,20 @@ typedef struct {
  * that are left out become 0.  cos and sin: (table_rows, D), indexed by position, with cs_strides = {0, row, 1}; or, with
  * table_rows = 0, (B or 1, S, D) with cs_strides = {batch (0 to share), token, 1}.  NULL: no rotation, and no queries.
  * 4 bits, per group, in 32 bits: step = (max / 2 - min / 2) * (2 / 15) and minimum, both rounded to dtype, and code =
- * round((x - minimum) * (1 / step)) within 0 .. 15.  A group that holds an infinity or a NaN reads back as NaN. */
+ * round((x - minimum) * (1 / step)) within 0 .. 15.  A group that holds an infinity or a NaN reads back as NaN.
+ * 8 bits, per block and head, in 32 bits: scale = max(most * (1 / 127), 2^-120), most the largest magnitude of the call's tokens in
+ * the block, and code = round(x * (1 / scale)), the product rounded once.  Where the block's first token is among them, the block
+ * begins anew; else the tokens before stay, the scale is at least what it was, and where it has grown their codes become
+ * round(code * (old scale / scale)).  So what the block's tokens stand for may change with each that is added (a token's code is rounded
+ * anew each time, by half of a step that is larger then), and a block that holds an infinity or a NaN reads back as NaN for
+ * this head.  What lies in a block behind the call's tokens is not kept: tokens that are taken back are written anew. */
 int pbs_paged_append(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* batch,
                      const void* k, const int64_t k_strides[4], const void* v, const int64_t v_strides[4],
                      int32_t q_heads, const void* q, const int64_t q_strides[4], void* q_out, const int64_t q_out_strides[4],
                      const void* cos_table, const void* sin_table, const int64_t cs_strides[3], int32_t table_rows, void* stream);
 
 /* The new tokens' keys and values as they are in the cache, back as (B, Hkv, S, D) of dtype; 0 for what was left out.
- * A value of 4 bits beyond the finite numbers of dtype (its step was rounded up) becomes the nearest of them. */
+ * A value of 8 or 4 bits beyond the finite numbers of dtype (its step was rounded up) becomes the nearest of them. */
 int pbs_paged_gather(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* batch, void* k, const int64_t k_strides[4],
                      void* v, const int64_t v_strides[4], void* stream);
 

@@ -59,7 +59,7 @@ Strides4 = C.c_int64 * 4
 class PagedCache(C.Structure):
     _fields_ = ([(n, C.c_void_p) for n in ("k", "v", "k_params", "v_params")]
                 + [(n, C.c_int64 * 3) for n in ("k_strides", "v_strides", "k_params_strides", "v_params_strides")]
-                + [(n, C.c_int32) for n in ("num_pages", "page_size", "kv_heads", "head_dim", "dtype", "bits", "group_size", "reserved")]
+                + [(n, C.c_int32) for n in ("num_pages", "page_size", "kv_heads", "head_dim", "dtype", "bits", "group_size", "block_size")]
                 + [("status", C.c_void_p)])
 
 

@@ -18,10 +18,14 @@ int check_paged(const pbs_paged_cache_t* c, const pbs_paged_batch_t* b, PagedArg
   PBS_NONNULL(c);
   PBS_NONNULL(b);
   if (c->dtype != PBS_BF16 && c->dtype != PBS_FP16) { set_error("paged cache: dtype %d is not bf16/fp16", c->dtype); return PBS_ERR_ARG; }
-  if (c->bits != 16 && c->bits != 4) { set_error("paged cache: %d bits, need 16 or 4", c->bits); return PBS_ERR_ARG; }
+  if (c->bits != 16 && c->bits != 8 && c->bits != 4) { set_error("paged cache: %d bits, need 16, 8 or 4", c->bits); return PBS_ERR_ARG; }
   if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) { set_error("paged cache: head_dim %d, need 64, 128 or 256", c->head_dim); return PBS_ERR_SHAPE; }
   if (c->bits == 4 && c->group_size != 32 && c->group_size != 64) { set_error("paged cache: group_size %d, need 32 or 64", c->group_size); return PBS_ERR_SHAPE; }
   if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1))) { set_error("paged cache: page_size %d, need a power of two in [16, 1024]", c->page_size); return PBS_ERR_SHAPE; }
+  if (c->bits == 8 && ((c->block_size != 16 && c->block_size != 32 && c->block_size != 64) || c->block_size > c->page_size)) {
+    set_error("paged cache: block_size %d, need 16, 32 or 64 and at most page_size (%d)", c->block_size, c->page_size);
+    return PBS_ERR_ARG;
+  }
   if (c->num_pages < 1 || c->kv_heads < 1) { set_error("paged cache: %d pages, %d heads", c->num_pages, c->kv_heads); return PBS_ERR_SHAPE; }
   if (b->batch < 1 || b->new_tokens < 1 || b->max_pages < 1) {
     set_error("batch, new_tokens and max_pages must be positive (got %d, %d, %d)", b->batch, b->new_tokens, b->max_pages);
@@ -40,10 +44,15 @@ int check_paged(const pbs_paged_cache_t* c, const pbs_paged_batch_t* b, PagedArg
     PBS_TRY(check_pages("k_params", c->k_params, c->k_params_strides, 2, align));
     PBS_TRY(check_pages("v_params", c->v_params, c->v_params_strides, 2, align));
   }
+  if (c->bits == 8) {
+    PBS_TRY(check_pages("k_params", c->k_params, c->k_params_strides, 4, 4));
+    PBS_TRY(check_pages("v_params", c->v_params, c->v_params_strides, 4, 4));
+  }
   out->c = *c;
   out->b = *b;
   out->shift = 0;
   while ((1 << out->shift) < c->page_size) ++out->shift;
+  out->block_shift = c->bits != 8 ? 0 : c->block_size == 16 ? 4 : c->block_size == 32 ? 5 : 6;
   return PBS_OK;
 }
 

@@ -10,6 +10,7 @@ struct PagedArgs {
   pbs_paged_cache_t c;
   pbs_paged_batch_t b;
   int shift;              // log2(page_size)
+  int block_shift;        // 8 bits: log2(block_size)
 };
 
 // Strides of a (B, heads, S, D) operand, in elements.

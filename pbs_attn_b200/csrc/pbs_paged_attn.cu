@@ -54,21 +54,23 @@ struct Cfg {
   static constexpr int WARPS = BITS == 16 && D == 256 ? 4 : 8;
   static constexpr int THREADS = 32 * WARPS;
   static constexpr int UNIT = WARPS * TILE;                        // tokens that work is dealt in
-  static constexpr int ROW = BITS == 4 ? D / 2 : 2 * D;            // bytes of a token's row
+  static constexpr int ROW = D * BITS / 8;                         // bytes of a token's row
   static constexpr int CH = ROW / 16;
   static constexpr int NG = BITS == 4 ? D / G : 1;
   static constexpr int PROW = BITS == 4 ? 4 * NG : 0;
-  static constexpr int STAGE = TILE * 2 * (ROW + PROW);
-  static constexpr int OCC = BITS == 4 && NT == 1 && D <= 128 ? 2 : 1;       // CTAs a SM
+  static constexpr int SCALES = BITS == 8 ? 16 : 0;                // bytes of a tile's scales: of keys and of values, for each 16 tokens
+  static constexpr int STAGE = TILE * 2 * (ROW + PROW) + SCALES;
+  static constexpr int OCC = BITS != 16 && NT == 1 && D <= 128 ? 2 : 1;      // CTAs a SM
   // (with two CTAs a SM a third stage of 128 channels gained nothing: 64 sequences of 16384 205 us with it, 203 without; and the batch's
   // prefix sums have room)
-  static constexpr int BUDGET = (OCC == 2 ? 96 : 200) * 1024;
+  static constexpr int BUDGET = (OCC == 2 ? BITS == 8 ? 97 : 96 : 200) * 1024;
   static constexpr int STAGES_FIT = BUDGET / (WARPS * STAGE);
   static constexpr int STAGES = STAGES_FIT < 2 ? 2 : STAGES_FIT > 4 ? 4 : STAGES_FIT;
   static constexpr int RING = WARPS * STAGES * STAGE;
   static constexpr int OROW = D + 4;                               // floats of a row of partial sums: four on, so that stores spread over the banks
   static constexpr int MERGE = WARPS * COLS * (OROW + 2) * 4;
   static constexpr int POOL = RING > MERGE ? RING : MERGE;
+  static constexpr bool FAR = BITS != 16 && DT == PBS_BF16;        // references may lie 2^170 apart (see factor_of)
   static constexpr bool LESS8 = BITS == 4 && DT == PBS_FP16;       // V's products are of code - 8 (see Warp)
   static constexpr int SHIFT = BITS == 4 && !LESS8 ? WARPS * COLS * NG * 4 : 0;
   static constexpr int QFRAG = COLS * D * 2;
@@ -145,6 +147,13 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
+// Signed bytes 0 and 2, or 1 and 3, of a word as two halves: 1024 + (byte + 128) by its bits, less 1152, which is exact.
+__device__ __forceinline__ uint32_t bytes02(uint32_t w) {
+  const uint32_t h = (w & 0x00ff00ffu) ^ 0x64806480u, b = 0x64806480u;
+  const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
+__device__ __forceinline__ uint32_t bytes13(uint32_t w) { return bytes02(w >> 8); }
 // Step (low half) and minimum (high half) of a word of params.
 template <class T>
 __device__ __forceinline__ float step_of(uint32_t w) {
@@ -176,14 +185,14 @@ __device__ __forceinline__ int piece(int row, int ch) {
   return row * C::ROW + ((ch ^ ((row / PER) & MASK)) << 4);
 }
 
-// Brings sums from one reference to another, whose difference is d.  References of bf16 caches of 4 bits differ with the steps, too, up to 2^170, while
+// Brings sums from one reference to another, whose difference is d.  References of bf16 caches of 8 and 4 bits differ with the steps, too, up to 2^170, while
 // the sums of weights that they are for are of one size: the factor is applied as its root, twice.
 template <class C>
-__device__ __forceinline__ float factor_of(float d) { return exp2_fast(C::SHIFT > 0 ? 0.5f * d : d); }
+__device__ __forceinline__ float factor_of(float d) { return exp2_fast(C::FAR ? 0.5f * d : d); }
 template <class C>
-__device__ __forceinline__ float scaled(float x, float f) { return C::SHIFT > 0 ? x * f * f : x * f; }
+__device__ __forceinline__ float scaled(float x, float f) { return C::FAR ? x * f * f : x * f; }
 template <class C>
-__device__ __forceinline__ float add_scaled(float f, float x, float sum) { return fmaf(f, C::SHIFT > 0 ? x * f : x, sum); }
+__device__ __forceinline__ float add_scaled(float f, float x, float sum) { return fmaf(f, C::FAR ? x * f : x, sum); }
 
 // Params of one token, NG words.
 template <class C>
@@ -280,6 +289,25 @@ struct Warp {
           for (int m = 0; m < C::MT; ++m) mma<C::DT>(tot[m][n], r[m][0], r[m][1], r[m][2], r[m][3], ks % 2 ? q.z : q.x, ks % 2 ? q.w : q.y);
         }
       }
+    } else if constexpr (C::BITS == 8) {
+#pragma unroll
+      for (int j = 0; j < C::CH / 2; ++j) {
+        uint32_t r[C::MT][4];
+#pragma unroll
+        for (int m = 0; m < C::MT; ++m) load_matrices(r[m], k_at + piece<C>(16 * m + row, 2 * j + half));
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+          for (int m = 0; m < C::MT; ++m) {
+            const uint32_t x = r[m][2 * jj], y = r[m][2 * jj + 1];
+            const uint32_t a0 = bytes02(x), a1 = bytes02(y), a2 = bytes13(x), a3 = bytes13(y);
+#pragma unroll
+            for (int n = 0; n < C::NT; ++n) {
+              const uint4 q = qf[(j * C::NT + n) * 32];
+              mma<PBS_FP16>(tot[m][n], a0, a1, a2, a3, jj ? q.z : q.x, jj ? q.w : q.y);
+            }
+          }
+      }
     } else {
       uint32_t kp[C::MT][2][C::NG];
       const uint8_t* params = stage + 2 * C::TILE * C::ROW;
@@ -335,6 +363,7 @@ struct Warp {
   // What the weights of tokens meet, for the largest of their steps and minima; at least `least`, for weights to stay below 2^85.
   static __device__ __forceinline__ constexpr float least() { return C::DT == PBS_BF16 ? 0x1p-70f : 0x1p-40f; }
   static __device__ __forceinline__ float met(uint32_t w) {
+    if constexpr (C::BITS == 8) return fmaxf(__uint_as_float(w), least());
     if constexpr (C::DT == PBS_BF16) return fmaxf(fmaxf(step_of<T>(w), low_of<T>(w) * 0x1p-64f), least());
     else return fmaxf(step_of<T>(w), least());
   }
@@ -354,6 +383,7 @@ struct Warp {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         meets[m][h] = (float)kRoom;
+        if constexpr (C::BITS == 8) meets[m][h] = __log2f(fminf(met(vp[m][0][0]), 0x1p127f));
         if constexpr (C::BITS == 4) {
           uint32_t w = 0;
 #pragma unroll
@@ -441,13 +471,19 @@ struct Warp {
   __device__ __forceinline__ void tile(const uint8_t* stage, int t0, uint32_t hole) {
     float x[C::MT][C::NT][4], p[C::MT][C::NT][4];
     scores(x, stage);
+    [[maybe_unused]] float ks[C::MT];                              // 8 bits: scales of the keys
+    if constexpr (C::BITS == 8) {
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m) ks[m] = *reinterpret_cast<const float*>(stage + 2 * C::TILE * C::ROW + 8 * m);
+    }
     bool seen[C::MT][C::NT][4];
 #pragma unroll
     for (int n = 0; n < C::NT; ++n) {
-      const float2 f = *reinterpret_cast<const float2*>(factor + 8 * n + 2 * (lane % 4));
+      const float2 f_all = *reinterpret_cast<const float2*>(factor + 8 * n + 2 * (lane % 4));
       const int2 lim = MASKED ? *reinterpret_cast<const int2*>(limit + 8 * n + 2 * (lane % 4)) : make_int2(0, 0);
 #pragma unroll
-      for (int m = 0; m < C::MT; ++m)
+      for (int m = 0; m < C::MT; ++m) {
+        const float2 f = C::BITS == 8 ? make_float2(f_all.x * ks[m], f_all.y * ks[m]) : f_all;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           if (MASKED) {
@@ -459,6 +495,7 @@ struct Warp {
             p[m][n][c] = exp2_fast(fmaf(x[m][n][c], c % 2 ? f.y : f.x, -ref[n][c % 2]));
           }
         }
+      }
     }
     uint32_t vp[C::MT][2][C::NG];
     float wide[C::NT][2];
@@ -491,6 +528,25 @@ struct Warp {
           }
       }
     }
+    if constexpr (C::BITS == 8) {
+      widest = least();
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m) {
+        vp[m][0][0] = *reinterpret_cast<const uint32_t*>(stage + 2 * C::TILE * C::ROW + 8 * m + 4);
+        widest = fmaxf(widest, met(vp[m][0][0]));
+      }
+      if constexpr (MASKED) {
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            wide[n][c] = least();
+#pragma unroll
+            for (int m = 0; m < C::MT; ++m)
+              if (seen[m][n][c] || seen[m][n][2 + c]) wide[n][c] = fmaxf(wide[n][c], met(vp[m][0][0]));
+          }
+      }
+    }
     bool need = false;
 #pragma unroll
     for (int n = 0; n < C::NT; ++n)
@@ -510,7 +566,7 @@ struct Warp {
 #pragma unroll
           for (int m = 0; m < C::MT; ++m)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) x[m][n][c] *= c % 2 ? f.y : f.x;
+            for (int c = 0; c < 4; ++c) x[m][n][c] *= C::BITS == 8 ? (c % 2 ? f.y : f.x) * ks[m] : c % 2 ? f.y : f.x;
         }
       }
       raise(x, p, wide, vp);
@@ -567,6 +623,34 @@ struct Warp {
       }
       if constexpr (MASKED) {
         if (!clean) add_not_finite(v, t0);
+      }
+    } else if constexpr (C::BITS == 8) {
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m) {
+        uint32_t b[C::NT][2];
+        const float s = __uint_as_float(vp[m][0][0]);
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            // a weight of 0 must not meet a scale that is not finite, of tokens that this query does not see; rounded to fp16, 11 bits: the
+            // codes have 8, the result 8 or 11
+            const bool s0 = !MASKED || seen[m][n][2 * h], s1 = !MASKED || seen[m][n][2 * h + 1];
+            b[n][h] = transpose8(pack_half(s0 ? p[m][n][2 * h] * s : 0.f, s1 ? p[m][n][2 * h + 1] * s : 0.f));
+          }
+#pragma unroll
+        for (int j2 = 0; j2 < C::CH / 2; ++j2) {
+          uint32_t r[4];
+          load_matrices_t(r, v_at + piece<C>(16 * m + (lane & 15), 2 * j2 + (lane >> 4)));
+#pragma unroll
+          for (int jj = 0; jj < 2; ++jj) {
+            // rows of the product: channels 2 i and 2 i + 1 of 16
+            const uint32_t y = r[2 * jj], z = r[2 * jj + 1];
+            const uint32_t a0 = bytes02(y), a1 = bytes13(y), a2 = bytes02(z), a3 = bytes13(z);
+#pragma unroll
+            for (int n = 0; n < C::NT; ++n) mma<PBS_FP16>(o[2 * j2 + jj][n], a0, a1, a2, a3, b[n][0], b[n][1]);
+          }
+        }
       }
     } else {
 #pragma unroll
@@ -645,6 +729,9 @@ struct Warp {
             *reinterpret_cast<float4*>(row + 32 * j + 4 * (lane / 4)) =
                 make_float4(fmaf(e[c], 0x1p24f, low), fmaf(e[c + 2] - e[c], 0x1p20f, low), fmaf(f[c], 0x1p24f, low), fmaf(f[c + 2] - f[c], 0x1p20f, low));
           }
+        } else if constexpr (C::BITS == 8) {
+#pragma unroll
+          for (int i = 0; i < C::D / 16; ++i) *reinterpret_cast<float2*>(row + 16 * i + 2 * (lane / 4)) = make_float2(o[i][n][c], o[i][n][c + 2]);
         } else {
 #pragma unroll
           for (int i = 0; i < C::D / 16; ++i) {
@@ -664,7 +751,7 @@ struct Item {
   int unit1;                                                       // the unit behind the item
 };
 
-// Brings the queries of an item into the order of the product's second operand (in 4 bits scaled by a power of two to a maximum in
+// Brings the queries of an item into the order of the product's second operand (in 8 and 4 bits scaled by a power of two to a maximum in
 // [2^14, 2^15), which fp16 holds to 2^-38 of it), and what belongs to each.
 template <class C>
 __device__ __forceinline__ void load_queries(const AttnArgs& p, const Item& it, uint8_t* frag, float* qsum, float* factor, int* limit) {
@@ -695,18 +782,25 @@ __device__ __forceinline__ void load_queries(const AttnArgs& p, const Item& it, 
       int k = most > 0.f ? 14 - ((int)(__float_as_uint(most) >> 23) - 127) : 0;
       k = min(max(k, -90), 120);
       const float up = __uint_as_float((uint32_t)(k + 127) << 23);
-      f *= __uint_as_float((uint32_t)(24 - k + 127) << 23);
+      f *= __uint_as_float((uint32_t)((C::BITS == 4 ? 24 : 0) - k + 127) << 23);
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
         x[t] = __half2float(__float2half_rn(x[t] * up));
         sum += x[t];
       }
+      if constexpr (C::BITS == 8) {
+        // codes 0 and 2, and 1 and 3, of a word meet in a register
+        uint8_t* const at = frag + (((pc / 4) * C::NT + col / 8) * 32 + (col % 8) * 4 + pc % 2 * 2) * 16 + pc / 2 % 2 * 8;
+        *reinterpret_cast<uint2*>(at) = make_uint2(pack_half(x[0], x[2]), pack_half(x[1], x[3]));
+        *reinterpret_cast<uint2*>(at + 16) = make_uint2(pack_half(x[4], x[6]), pack_half(x[5], x[7]));
+      } else {
 #pragma unroll
-      for (int s = C::G / 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-      if (pc % (C::G / 8) == 0) qsum[pc / (C::G / 8) * C::COLS + col] = sum * 0x1p-24f;
-      // codes i and i + 4 of a word meet in one register; those of bits 4-7 are 16 times too large
-      *reinterpret_cast<uint4*>(frag + (((pc / 4) * C::NT + col / 8) * 32 + (col % 8) * 4 + pc % 4) * 16) =
-          make_uint4(pack_half(x[0], x[4]), pack_half(x[1] * 0.0625f, x[5] * 0.0625f), pack_half(x[2], x[6]), pack_half(x[3] * 0.0625f, x[7] * 0.0625f));
+        for (int s = C::G / 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+        if (pc % (C::G / 8) == 0) qsum[pc / (C::G / 8) * C::COLS + col] = sum * 0x1p-24f;
+        // codes i and i + 4 of a word meet in one register; those of bits 4-7 are 16 times too large
+        *reinterpret_cast<uint4*>(frag + (((pc / 4) * C::NT + col / 8) * 32 + (col % 8) * 4 + pc % 4) * 16) =
+            make_uint4(pack_half(x[0], x[4]), pack_half(x[1] * 0.0625f, x[5] * 0.0625f), pack_half(x[2], x[6]), pack_half(x[3] * 0.0625f, x[7] * 0.0625f));
+      }
     }
     if (pc == 0) {
       factor[col] = f;
@@ -816,8 +910,9 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
     constexpr int ES = C::BITS == 16 ? 2 : 1;
     const uint8_t* const kb = (const uint8_t*)c.k + it.head * c.k_strides[1] * ES + lane % C::CH * 16;
     const uint8_t* const vb = (const uint8_t*)c.v + it.head * c.v_strides[1] * ES + lane % C::CH * 16;
-    const uint8_t* const kpb = (const uint8_t*)c.k_params + 2 * it.head * c.k_params_strides[1];
-    const uint8_t* const vpb = (const uint8_t*)c.v_params + 2 * it.head * c.v_params_strides[1];
+    constexpr int PS = C::BITS == 8 ? 4 : 2;
+    const uint8_t* const kpb = (const uint8_t*)c.k_params + PS * it.head * c.k_params_strides[1];
+    const uint8_t* const vpb = (const uint8_t*)c.v_params + PS * it.head * c.v_params_strides[1];
     const int* const table = bt.block_table + it.seq * bt.table_stride;
     int page[C::MT];
     uint32_t holes = 0;                                            // 16 tokens without a page: bit (place in the ring) * MT + m
@@ -837,6 +932,14 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
     auto issue = [&](int slot) {                                   // its copies, to this place in the ring, once its pages are here
       const int t0 = next - C::UNIT;
       const uint32_t at = ring_at + slot * C::STAGE;
+      if constexpr (C::BITS == 8) {                                // scales: a lane one
+        const int m = lane >> 1, pg = C::MT == 2 && m == 1 ? page[C::MT - 1] : page[0], first = t0 + 16 * m;
+        if (m < C::MT && pg >= 0 && first < tok1) {
+          const uint32_t block = (first & (c.page_size - 1)) >> p.a.block_shift;
+          copy_async<4>(at + 2 * C::TILE * C::ROW + 4 * lane,
+                        lane & 1 ? vpb + 4 * (uint64_t)(pg * p.vp_page + block * p.vp_slot) : kpb + 4 * (uint64_t)(pg * p.kp_page + block * p.kp_slot));
+        }
+      }
       if (p.dense && t0 + C::TILE <= tok1 && page[0] >= 0 && page[C::MT - 1] >= 0) {
         // the common case, whose copies are a few constants away from one another: half the instructions of the one below
         holes &= ~(((1u << C::MT) - 1) << slot * C::MT);
@@ -1089,19 +1192,20 @@ int launch(AttnArgs p, void* workspace, bool measure, int64_t* bytes, cudaStream
   }
   const pbs_paged_cache_t& c = p.a.c;
   bool fits = true;
-  auto steps = [&](const int64_t (&st)[3], int bytes, int unit, uint32_t& page, uint32_t& slot) {
+  auto steps = [&](const int64_t (&st)[3], int bytes, int unit, uint32_t& page, uint32_t& slot, int rows) {
     const int64_t a = st[0] * bytes / unit, b = st[2] * bytes / unit;
-    fits = fits && a <= UINT32_MAX && b <= UINT32_MAX && (__int128)(c.num_pages - 1) * a + (__int128)(c.page_size - 1) * b <= UINT32_MAX;
+    fits = fits && a <= UINT32_MAX && b <= UINT32_MAX && (__int128)(c.num_pages - 1) * a + (__int128)(rows - 1) * b <= UINT32_MAX;
     page = (uint32_t)a;
     slot = (uint32_t)b;
   };
   p.dense = c.k_strides[2] * (C::BITS == 16 ? 2 : 1) == C::ROW && c.v_strides[2] * (C::BITS == 16 ? 2 : 1) == C::ROW &&
-            (C::BITS == 16 || (c.k_params_strides[2] == 2 * C::NG && c.v_params_strides[2] == 2 * C::NG));
-  steps(c.k_strides, C::BITS == 16 ? 2 : 1, 16, p.k_page, p.k_slot);
-  steps(c.v_strides, C::BITS == 16 ? 2 : 1, 16, p.v_page, p.v_slot);
-  if (C::BITS == 4) {
-    steps(c.k_params_strides, 2, 4, p.kp_page, p.kp_slot);
-    steps(c.v_params_strides, 2, 4, p.vp_page, p.vp_slot);
+            (C::BITS != 4 || (c.k_params_strides[2] == 2 * C::NG && c.v_params_strides[2] == 2 * C::NG));
+  steps(c.k_strides, C::BITS == 16 ? 2 : 1, 16, p.k_page, p.k_slot, c.page_size);
+  steps(c.v_strides, C::BITS == 16 ? 2 : 1, 16, p.v_page, p.v_slot, c.page_size);
+  if (C::BITS != 16) {
+    const int rows = C::BITS == 4 ? c.page_size : c.page_size >> p.a.block_shift;
+    steps(c.k_params_strides, C::BITS == 4 ? 2 : 4, 4, p.kp_page, p.kp_slot, rows);
+    steps(c.v_params_strides, C::BITS == 4 ? 2 : 4, 4, p.vp_page, p.vp_slot, rows);
   }
   if (!fits) { set_error("paged attention: a pool of more than 64 GiB (params: 16 GiB)"); return PBS_ERR_SHAPE; }
   p.counters = (unsigned*)workspace;
@@ -1148,6 +1252,7 @@ int by_queries(const AttnArgs& p, void* w, bool measure, int64_t* bytes, cudaStr
 template <int DT, int D>
 int by_bits(const AttnArgs& p, void* w, bool measure, int64_t* bytes, cudaStream_t st) {
   if (p.a.c.bits == 16) return by_queries<DT, D, 16, D>(p, w, measure, bytes, st);
+  if (p.a.c.bits == 8) return by_queries<DT, D, 8, D>(p, w, measure, bytes, st);
   return p.a.c.group_size == 32 ? by_queries<DT, D, 4, 32>(p, w, measure, bytes, st) : by_queries<DT, D, 4, 64>(p, w, measure, bytes, st);
 }
 

@@ -8,6 +8,8 @@
 // HBM bounds prompts, latency and the launch single tokens.  8191 tokens of 8 KV heads into 4 bits: 15 us (33.5 MB read, 9.4 MB written, 2.9
 // TB/s; 75 % of the issue slots are taken: some 170 instructions for eight channels), back out 11 us; 64 sequences' next tokens, 32 query
 // heads rotated, 2.5 us.
+#include <climits>
+
 #include "pbs_paged.cuh"
 
 namespace pbs {
@@ -100,6 +102,20 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t& par
   return word - excess;
 }
 
+// A lane's eight channels of a row that LPR lanes hold, rotated: x cos + rotate_half(x) sin, each product and the sum rounded.
+template <class T, int LPR>
+__device__ __forceinline__ void turned8(const uint4& now, const uint4& cs, const uint4& sn, int lane, float (&x)[8]) {
+  const uint4 other = make_uint4(__shfl_xor_sync(0xffffffffu, now.x, LPR / 2), __shfl_xor_sync(0xffffffffu, now.y, LPR / 2),
+                                 __shfl_xor_sync(0xffffffffu, now.z, LPR / 2), __shfl_xor_sync(0xffffffffu, now.w, LPR / 2));
+  float y[8], cf[8], sf[8];
+  unpack8<T>(now, x);
+  unpack8<T>(other, y);
+  unpack8<T>(cs, cf);
+  unpack8<T>(sn, sf);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = __fadd_rn(__fmul_rn(x[j], cf[j]), __fmul_rn(lane < LPR / 2 ? -y[j] : y[j], sf[j]));
+}
+
 struct AppendArgs {
   PagedArgs a;
   RowTensor k, v, q, qo;
@@ -170,17 +186,8 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(const __grid_
     if (r + kAhead < n) raw[kAhead - 1] = *reinterpret_cast<const uint4*>(in + kAhead * step);
     in += step;
     float x[8];
-    unpack8<T>(now, x);
-    if (turn) {
-      const uint4 other = make_uint4(__shfl_xor_sync(0xffffffffu, now.x, LPR / 2), __shfl_xor_sync(0xffffffffu, now.y, LPR / 2),
-                                     __shfl_xor_sync(0xffffffffu, now.z, LPR / 2), __shfl_xor_sync(0xffffffffu, now.w, LPR / 2));
-      float y[8], cf[8], sf[8];
-      unpack8<T>(other, y);
-      unpack8<T>(cs, cf);
-      unpack8<T>(sn, sf);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = __fadd_rn(__fmul_rn(x[j], cf[j]), __fmul_rn(lane < LPR / 2 ? -y[j] : y[j], sf[j]));
-    }
+    if (turn) turned8<T, LPR>(now, cs, sn, lane, x);
+    else unpack8<T>(now, x);
     if (BITS == 16 || is_q) {
       uint4 w = pack8<T>(x);
       if (pos < 0) w = make_uint4(0, 0, 0, 0);             // (a query's row that is left out)
@@ -198,6 +205,194 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(const __grid_
   }
 }
 
+// --------------------------------------------------------------------------------------------------------------------------------
+// 8 bits.  A block's scale is known when all of the call's tokens in it have been looked at, so a warp takes 16 of its tokens (a head's keys or
+// values) and keeps them in registers, all loads under way at once; the warps of a block of 32 or 64 tokens meet in shared memory for the
+// largest magnitude.  Where the scale of a block with older tokens has grown, their codes are brought to it by the same warps.
+//
+// Rounding: a product and 1.5 * 2^23 in one fma leave the code, as a signed byte, in the lowest bits of the sum.
+
+// Largest magnitude of four words of two values; a NaN stays.
+__device__ __forceinline__ float most8(const uint4& w, __nv_bfloat16*) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+  __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u[0]));
+#pragma unroll
+  for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u[i])));
+  return max_nan(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float most8(const uint4& w, __half*) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+  __half2 m = __habs2(*reinterpret_cast<const __half2*>(&u[0]));
+#pragma unroll
+  for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&u[i])));
+  return max_nan(__low2float(m), __high2float(m));
+}
+
+// Codes of eight values at `inv` a step.
+__device__ __forceinline__ uint2 codes8(const float (&x)[8], float inv) {
+  uint32_t r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(fmaf(x[i], inv, 12582912.f));
+  return make_uint2(__byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(r[4], r[5], 0x0040), __byte_perm(r[6], r[7], 0x0040), 0x5410));
+}
+
+// The numbers that four signed bytes are.
+__device__ __forceinline__ void signed4(uint32_t w, float (&x)[4]) {
+  w ^= 0x80808080u;                                        // 0 .. 255, the lowest byte of 2^23 + that
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7650 + i)) - 8388736.f;
+}
+
+constexpr float kLeastScale = 7.52316385e-37f;             // 2^-120: its reciprocal is an ordinary number
+
+// blocks: of tokens that a sequence's new ones may lie in; kv_ctas: CTAs that write keys and values, the others turn queries
+template <int DT, int D, int W, bool ROPE>
+__global__ void __launch_bounds__(kThreads, ROPE && D == 256 ? 1 : 2) paged_append8_kernel(const __grid_constant__ AppendArgs p, int blocks, int units, int kv_ctas) {
+  using T = typename Elem<DT>::T;
+  constexpr int LPR = D / 8, RPI = 32 / LPR, NI = 16 / RPI;  // lanes a row; rows at a time, and times, of a warp's 16
+  const pbs_paged_cache_t& c = p.a.c;
+  const pbs_paged_batch_t& bt = p.a.b;
+  if (ROPE && (int)blockIdx.x >= kv_ctas) {                // queries: a token, and p.chunk of its heads, a group of lanes
+    const int lane = threadIdx.x % LPR, g = ((int)blockIdx.x - kv_ctas) * (kThreads / LPR) + threadIdx.x / LPR;
+    const int token = g / p.q_chunks, head0 = g % p.q_chunks * p.chunk;
+    const bool active = token < bt.batch * bt.new_tokens;    // (the other lanes go along: a warp's shuffles take all of them)
+    const int n = min(p.chunk, p.q_heads - head0), seq = active ? token / bt.new_tokens : 0, i = active ? token % bt.new_tokens : 0;
+    int pos = active ? new_position(bt, seq, i) : -1;
+    uint4 cs = make_uint4(0, 0, 0, 0), sn = cs;
+    if (pos >= 0) {
+      if (p.table_rows > 0 && pos >= p.table_rows) {
+        paged_fault(p.a, PBS_PAGED_BAD_ROTARY);
+        pos = -1;
+      } else {
+        const int64_t at = (p.table_rows > 0 ? pos * p.cs_s : seq * p.cs_b + i * p.cs_s) + 8 * lane;
+        cs = *reinterpret_cast<const uint4*>((const T*)p.cosp + at);
+        sn = *reinterpret_cast<const uint4*>((const T*)p.sinp + at);
+      }
+    }
+    const T* in = (const T*)p.q.p + seq * p.q.st.b + head0 * p.q.st.h + i * p.q.st.s + 8 * lane;
+    T* out = (T*)p.qo.p + seq * p.qo.st.b + head0 * p.qo.st.h + i * p.qo.st.s + 8 * lane;
+    for (int r = 0; r < p.chunk; ++r) {
+      uint4 w = r < n ? *reinterpret_cast<const uint4*>(in + r * p.q.st.h) : make_uint4(0, 0, 0, 0);
+      float x[8];
+      turned8<T, LPR>(w, cs, sn, lane, x);
+      w = pack8<T>(x);
+      if (pos < 0) w = make_uint4(0, 0, 0, 0);             // (a row that is left out)
+      if (active && r < n) *reinterpret_cast<uint4*>(out + r * p.qo.st.h) = w;
+    }
+    return;
+  }
+  // the warp's 16 tokens: positions t0 .. of a head's keys or values, of them first .. end - 1 new
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, col = lane % LPR;
+  const int unit = (int)blockIdx.x * (kThreads / 32 / W) + warp / W;
+  int head = 0, seq = 0, first = 0, end = 0, shift_i = 0, begin = 0, page = -1;
+  bool is_v = false;
+  if (unit < units) {
+    head = unit % c.kv_heads;
+    int rest = unit / c.kv_heads;
+    is_v = rest % 2;
+    rest /= 2;
+    seq = rest / blocks;
+    const int n = bt.new_lens ? min(max(bt.new_lens[seq], 0), bt.new_tokens) : bt.new_tokens, len = bt.seq_lens[seq];
+    shift_i = len - n;                                     // position of the first row
+    first = max(0, shift_i);
+    end = len;
+    if (p.cosp && p.table_rows > 0 && end > p.table_rows && n > 0) {
+      paged_fault(p.a, PBS_PAGED_BAD_ROTARY);
+      end = p.table_rows;
+    }
+    const int block = (first >> p.a.block_shift) + rest % blocks;
+    if (n > 0 && end > first && block <= (end - 1) >> p.a.block_shift) {
+      begin = block << p.a.block_shift;
+      page = page_of(p.a, seq, begin);
+    }
+  }
+  const bool active = page >= 0;
+  first = max(first, begin);
+  const int t0 = begin + warp % W * 16 + lane / LPR;       // this lane's first token, RPI apart
+  const RowTensor& src = is_v ? p.v : p.k;
+  const T* in = (const T*)src.p + seq * src.st.b + head * src.st.h + 8 * col;
+  uint4 raw[NI];
+#pragma unroll
+  for (int k = 0; k < NI; ++k) {
+    const int t = t0 + k * RPI;
+    raw[k] = make_uint4(0, 0, 0, 0);
+    if (active && t >= first && t < end) raw[k] = *reinterpret_cast<const uint4*>(in + (int64_t)(t - shift_i) * src.st.s);
+  }
+  const bool older = active && first > begin;              // the block holds tokens already
+  const int slot = begin & (c.page_size - 1);
+  float* const scale_at = (float*)(is_v ? c.v_params : c.k_params) +
+                          (active ? slot_offset(is_v ? c.v_params_strides : c.k_params_strides, page, head, slot >> p.a.block_shift) : 0);
+  const float old = older ? *scale_at : 0.f;
+  float most = 0.f;
+  float x[ROPE ? NI : 1][8];
+  const bool turn = ROPE && !is_v;
+  if (turn) {
+#pragma unroll
+    for (int k = 0; k < (ROPE ? NI : 0); ++k) {
+      const int t = t0 + k * RPI;
+      uint4 cs = make_uint4(0, 0, 0, 0), sn = cs;
+      if (active && t >= first && t < end) {
+        const int64_t at = (p.table_rows > 0 ? t * p.cs_s : seq * p.cs_b + (t - shift_i) * p.cs_s) + 8 * col;
+        cs = *reinterpret_cast<const uint4*>((const T*)p.cosp + at);
+        sn = *reinterpret_cast<const uint4*>((const T*)p.sinp + at);
+      }
+      turned8<T, LPR>(raw[k], cs, sn, col, x[k]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = max_nan(most, fabsf(x[k][j]));
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < NI; ++k) most = max_nan(most, most8(raw[k], (T*)nullptr));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+  if constexpr (W > 1) {
+    __shared__ float meet[kThreads / 32];
+    if (lane == 0) meet[warp] = most;
+    __syncthreads();                                       // (old scales have been read, too)
+    most = meet[warp / W * W];
+#pragma unroll
+    for (int k = 1; k < W; ++k) most = max_nan(most, meet[warp / W * W + k]);
+  }
+  if (!active) return;
+  float scale = fmaxf(__fmul_rn(most, 1.f / 127.f), kLeastScale);
+  if (!(most <= 3.402823466e38f)) scale = CUDART_NAN_F;
+  if (older) scale = max_nan(scale, old);
+  const bool grown = older && scale != old;                // (of one that is NaN the codes are nothing)
+  const float inv = __fdiv_rn(1.f, scale), ratio = grown ? __fdiv_rn(old, scale) : 1.f;
+  int8_t* const out = (int8_t*)(is_v ? c.v : c.k) + slot_offset(is_v ? c.v_strides : c.k_strides, page, head, 0) + 8 * col;
+  const int64_t step = (is_v ? c.v_strides : c.k_strides)[2];
+#pragma unroll
+  for (int k = 0; k < NI; ++k) {
+    const int t = t0 + k * RPI;
+    if (t < first ? !grown : t >= end) continue;
+    uint2* const at = reinterpret_cast<uint2*>(out + (t & (c.page_size - 1)) * step);
+    float y[8];
+    if (t < first) {
+      const uint2 w = *at;
+      float a[4], b[4];
+      signed4(w.x, a);
+      signed4(w.y, b);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        y[j] = a[j];
+        y[j + 4] = b[j];
+      }
+      *at = codes8(y, ratio);
+    } else {
+      if (turn) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = x[ROPE ? k : 0][j];
+      } else {
+        unpack8<T>(raw[k], y);
+      }
+      *at = codes8(y, inv);
+    }
+  }
+  if (lane == 0 && warp % W == 0) *scale_at = scale;
+}
+
 template <int DT, int D, int BITS, int G>
 __global__ void __launch_bounds__(kThreads, 4) paged_gather_kernel(const __grid_constant__ AppendArgs p, int tokens) {
   using T = typename Elem<DT>::T;
@@ -209,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 4) paged_gather_kernel(const __grid_
   if (token >= tokens) return;
   const int seq = token / p.a.b.new_tokens, i = token % p.a.b.new_tokens;
   const int pos = new_position(p.a.b, seq, i);
-  const int page = pos >= 0 ? page_of(p.a, seq, pos) : -1, slot = pos & (c.page_size - 1);
+  const int page = pos >= 0 ? page_of(p.a, seq, pos) : -1, slot = pos & (c.page_size - 1);   // (0 .. page_size - 1, of -1 too)
   constexpr int ES = BITS == 16 ? 2 : 1;
   const uint8_t* in = (const uint8_t*)(is_v ? c.v : c.k) + slot_offset(is_v ? c.v_strides : c.k_strides, max(page, 0), head0, slot) * ES + lane * BITS;
   const int64_t step = (is_v ? c.v_strides : c.k_strides)[1] * ES;
@@ -220,18 +415,26 @@ __global__ void __launch_bounds__(kThreads, 4) paged_gather_kernel(const __grid_
           lane / (BITS == 4 ? G / 8 : 1) * 4;
     pstep = (is_v ? c.v_params_strides : c.k_params_strides)[1] * (int)sizeof(T);
   }
+  if (BITS == 8) {
+    pin = (const uint8_t*)((const float*)(is_v ? c.v_params : c.k_params) +
+                           slot_offset(is_v ? c.v_params_strides : c.k_params_strides, max(page, 0), head0, slot >> p.a.block_shift));
+    pstep = (is_v ? c.v_params_strides : c.k_params_strides)[1] * 4;
+  }
   const RowTensor& dst = is_v ? p.v : p.k;
   T* out = (T*)dst.p + seq * dst.st.b + head0 * dst.st.h + i * dst.st.s + 8 * lane;
   const float most = finite_max((T*)nullptr);
   constexpr int U = 4;                                     // rows that a lane has under way
   for (int r = 0; r < n; r += U) {
-    uint4 w[U];                                            // 4 bits: word and params in x and y
+    uint4 w[U];                                            // 4 bits: word and params in x and y; 8: codes in x and y, scale in z
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       w[u] = make_uint4(0, 0, 0, 0);
       if (r + u >= n || page < 0) continue;
       if constexpr (BITS == 16) {
         w[u] = *reinterpret_cast<const uint4*>(in + u * step);
+      } else if constexpr (BITS == 8) {
+        const uint2 codes = *reinterpret_cast<const uint2*>(in + u * step);
+        w[u] = make_uint4(codes.x, codes.y, *reinterpret_cast<const uint32_t*>(pin + u * pstep), 0);
       } else {
         w[u].x = *reinterpret_cast<const uint32_t*>(in + u * step);
         w[u].y = *reinterpret_cast<const uint32_t*>(pin + u * pstep);
@@ -254,6 +457,23 @@ __global__ void __launch_bounds__(kThreads, 4) paged_gather_kernel(const __grid_
         }
         w[u] = pack8<T>(x);
       }
+      if constexpr (BITS == 8) {
+        const float scale = __uint_as_float(w[u].z);
+        float a[4], b[4], x[8];
+        signed4(w[u].x, a);
+        signed4(w[u].y, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[j] = a[j] * scale;
+          x[j + 4] = b[j] * scale;
+        }
+        if (127.f * scale > most) {                        // (a key that the rotation made larger than fp16 holds)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = fminf(fmaxf(x[j], -most), most);
+        }
+        w[u] = pack8<T>(x);
+        if (page < 0) w[u] = make_uint4(0, 0, 0, 0);
+      }
       *reinterpret_cast<uint4*>(out + u * dst.st.h) = w[u];
     }
     in += U * step;
@@ -262,26 +482,62 @@ __global__ void __launch_bounds__(kThreads, 4) paged_gather_kernel(const __grid_
   }
 }
 
-template <int DT, int D, int BITS, int G>
-int launch(AppendArgs p, bool gather, cudaStream_t st) {
-  // A group of lanes takes so many of a token's rows that all groups are resident at a time: what the rows of a token share (position, page,
-  // rotary factors, the index arithmetic) is then read and done once for them.  One token: a row each.
+// A group of lanes takes so many of a token's rows that all groups are resident at a time: what the rows of a token share (position, page,
+// rotary factors, the index arithmetic) is then read and done once for them.  One token: a row each.
+template <int D>
+dim3 deal(AppendArgs& p) {
   constexpr int RPB = kThreads / (D / 8);
   const int64_t tokens = (int64_t)p.a.b.batch * p.a.b.new_tokens, resident = (int64_t)device_sms() * 4 * RPB;
   const int64_t chunk = (tokens * (p.q_heads + 2 * p.a.c.kv_heads) + resident - 1) / resident;
   p.chunk = (int)(chunk < 8 ? chunk : 8);
   p.q_chunks = (p.q_heads + p.chunk - 1) / p.chunk;
   p.kv_chunks = (p.a.c.kv_heads + p.chunk - 1) / p.chunk;
-  const dim3 grid((unsigned)((tokens + RPB - 1) / RPB), (unsigned)(p.q_chunks + 2 * p.kv_chunks));
-  if (gather) paged_gather_kernel<DT, D, BITS, G><<<grid, kThreads, 0, st>>>(p, (int)tokens);
-  else paged_append_kernel<DT, D, BITS, G><<<grid, kThreads, 0, st>>>(p, (int)tokens);
-  PBS_CUDA_CHECK_LAUNCH(gather ? "paged_gather_kernel" : "paged_append_kernel");
+  return dim3((unsigned)((tokens + RPB - 1) / RPB), (unsigned)(p.q_chunks + 2 * p.kv_chunks));
+}
+
+template <int DT, int D, int BITS, int G>
+int launch_gather(AppendArgs p, cudaStream_t st) {
+  const dim3 grid = deal<D>(p);
+  paged_gather_kernel<DT, D, BITS, G><<<grid, kThreads, 0, st>>>(p, p.a.b.batch * p.a.b.new_tokens);
+  PBS_CUDA_CHECK_LAUNCH("paged_gather_kernel");
+  return PBS_OK;
+}
+
+template <int DT, int D, int BITS, int G>
+int launch(AppendArgs p, bool gather, cudaStream_t st) {
+  if (gather) return launch_gather<DT, D, BITS, G>(p, st);
+  const dim3 grid = deal<D>(p);
+  paged_append_kernel<DT, D, BITS, G><<<grid, kThreads, 0, st>>>(p, p.a.b.batch * p.a.b.new_tokens);
+  PBS_CUDA_CHECK_LAUNCH("paged_append_kernel");
+  return PBS_OK;
+}
+
+template <int DT, int D, int W>
+int launch_append8(AppendArgs p, cudaStream_t st) {
+  constexpr int UPC = kThreads / 32 / W, RPB = kThreads / (D / 8);
+  const int S = p.a.b.new_tokens, bs = 16 * W;
+  const int64_t blocks = ((int64_t)S + 2 * bs - 2) / bs;   // that S tokens reach into, wherever they begin
+  const int64_t units = blocks * p.a.b.batch * 2 * p.a.c.kv_heads, kv_ctas = (units + UPC - 1) / UPC;
+  // heads of a token's queries share its rotary factors: as many as leave every group of lanes something to do
+  const int64_t tokens = (int64_t)p.a.b.batch * S, groups = (int64_t)device_sms() * 4 * RPB;
+  const int64_t chunk = (tokens * p.q_heads + groups - 1) / groups;
+  p.chunk = (int)(chunk < 1 ? 1 : chunk < 8 ? chunk : 8);
+  p.q_chunks = (p.q_heads + p.chunk - 1) / p.chunk;
+  const int64_t ctas = kv_ctas + (tokens * p.q_chunks + RPB - 1) / RPB;
+  if (units > INT_MAX - 1024 || ctas > INT_MAX) { set_error("paged append: too many blocks of tokens in a call"); return PBS_ERR_SHAPE; }
+  if (p.cosp) paged_append8_kernel<DT, D, W, true><<<(unsigned)ctas, kThreads, 0, st>>>(p, (int)blocks, (int)units, (int)kv_ctas);
+  else paged_append8_kernel<DT, D, W, false><<<(unsigned)kv_ctas, kThreads, 0, st>>>(p, (int)blocks, (int)units, (int)kv_ctas);
+  PBS_CUDA_CHECK_LAUNCH("paged_append8_kernel");
   return PBS_OK;
 }
 
 template <int DT, int D>
 int by_bits(const AppendArgs& p, bool gather, cudaStream_t st) {
   if (p.a.c.bits == 16) return launch<DT, D, 16, 0>(p, gather, st);
+  if (p.a.c.bits == 8) {
+    if (gather) return launch_gather<DT, D, 8, 0>(p, st);
+    return p.a.block_shift == 4 ? launch_append8<DT, D, 1>(p, st) : p.a.block_shift == 5 ? launch_append8<DT, D, 2>(p, st) : launch_append8<DT, D, 4>(p, st);
+  }
   return p.a.c.group_size == 32 ? launch<DT, D, 4, 32>(p, gather, st) : launch<DT, D, 4, 64>(p, gather, st);
 }
 

@@ -1,4 +1,4 @@
-"""What follows a prompt: a paged cache of keys and values in 16 or 4 bits, and the attention of new tokens over it.
+"""What follows a prompt: a paged cache of keys and values in 16, 8 or 4 bits, and the attention of new tokens over it.
 
     cache = PagedKVCache(num_pages, page_size, kv_heads, head_dim, torch.bfloat16, "cuda", bits=4)     # one per layer
     q = paged_kv_append(cache, k, v, block_table, seq_lens, cos=cos, sin=sin, query_states=q)
@@ -61,53 +61,76 @@ def _raise_fault(word: C.c_int32):
 class PagedKVCache:
     """Pages of keys and values of one layer.
 
-    ``k`` and ``v`` are (num_pages, kv_heads, page_size, head_dim) of ``dtype`` for 16 bits and (..., head_dim / 2) uint8 for 4
-    (channel 2i in the low half of byte i); with 4 bits ``k_params`` and ``v_params``, (num_pages, kv_heads, page_size,
+    ``k`` and ``v`` are (num_pages, kv_heads, page_size, head_dim) of ``dtype`` for 16 bits, int8 for 8 and (..., head_dim / 2) uint8 for
+    4 (channel 2i in the low half of byte i).  With 4 bits ``k_params`` and ``v_params``, (num_pages, kv_heads, page_size,
     head_dim / group_size, 2) of ``dtype``, hold step and minimum of each group of channels of a token: a code c stands for
-    minimum + c * step.  ``page_size`` is a power of two from 16 to 1024, ``head_dim`` 64, 128 or 256, ``group_size`` 32 or 64.
+    minimum + c * step.  With 8 bits they are (num_pages, kv_heads, page_size / block_size) float32, the scales of the blocks of
+    ``block_size`` tokens of a page and head: a code c stands for c * scale.  A scale grows with the tokens that come into its block, so
+    what the block's older tokens stand for may change in the last bits until it is full; tokens that are taken back (rejected drafts) leave
+    their scale behind until the block begins anew.
+    ``page_size`` is a power of two from 16 to 1024, ``head_dim`` 64, 128 or 256, ``group_size`` 32 or 64, ``block_size`` (needed for 8
+    bits) 16, 32 or 64 and at most ``page_size``.
     New pages hold whatever the memory held: no token is read that was not appended.
     """
 
     def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
-                 device="cuda", bits: int = 16, group_size: int = 64):
-        if bits not in (4, 16):
-            raise ValueError(f"bits={bits}: a cache holds 16 or 4 bits a value")
+                 device="cuda", bits: int = 16, group_size: int = 64, block_size: Optional[int] = None):
+        if bits not in (4, 8, 16):
+            raise ValueError(f"bits={bits}: a cache holds 16, 8 or 4 bits a value")
+        if bits == 8 and block_size is None:
+            raise ValueError("bits=8: block_size, the number of tokens that share a scale, is needed")
         make = lambda *s, dt=dtype: torch.empty(num_pages, kv_heads, page_size, *s, dtype=dt, device=device)  # noqa: E731
         if bits == 16:
-            self._set(make(head_dim), make(head_dim), None, None)
+            self._set(make(head_dim), make(head_dim), None, None, dtype)
+        elif bits == 8:
+            if block_size < 1 or page_size % block_size:
+                raise ValueError(f"block_size={block_size} does not divide page_size={page_size}")
+            scales = (torch.empty(num_pages, kv_heads, page_size // block_size, dtype=torch.float32, device=device) for _ in "kv")
+            self._set(*(make(head_dim, dt=torch.int8) for _ in "kv"), *scales, dtype)
         else:
             if head_dim % group_size:
                 raise ValueError(f"group_size={group_size} does not divide head_dim={head_dim}")
-            self._set(*(make(head_dim // 2, dt=torch.uint8) for _ in "kv"), *(make(head_dim // group_size, 2) for _ in "kv"))
+            self._set(*(make(head_dim // 2, dt=torch.uint8) for _ in "kv"), *(make(head_dim // group_size, 2) for _ in "kv"), dtype)
 
     @classmethod
-    def from_tensors(cls, k, v, k_params=None, v_params=None) -> "PagedKVCache":
-        """A cache over tensors that exist, of any strides that the kernels can read (a token's row dense, rows on 16-byte boundaries)."""
+    def from_tensors(cls, k, v, k_params=None, v_params=None, dtype: Optional[torch.dtype] = None) -> "PagedKVCache":
+        """A cache over tensors that exist, of any strides that the kernels can read (a token's row dense, rows on 16-byte boundaries).
+        ``dtype``, that of the queries, keys and values, is needed where the tensors do not tell: for 8 bits."""
         self = object.__new__(cls)
-        self._set(k, v, k_params, v_params)
+        self._set(k, v, k_params, v_params, dtype)
         return self
 
-    def _set(self, k, v, k_params, v_params):
+    def _set(self, k, v, k_params, v_params, dtype=None):
         self.lib = _cabi.load()
-        self.bits = 4 if k.dtype == torch.uint8 else 16
+        self.bits = {torch.uint8: 4, torch.int8: 8}.get(k.dtype, 16)
         pages, heads, page_size, row = k.shape
-        if self.bits == 4 and (k_params is None or v_params is None):
-            raise ValueError("pages of 4 bits need k_params and v_params")
-        self.dtype = k.dtype if self.bits == 16 else k_params.dtype
+        if self.bits != 16 and (k_params is None or v_params is None):
+            raise ValueError(f"pages of {self.bits} bits need k_params and v_params")
+        if self.bits == 8 and dtype is None:
+            raise ValueError("pages of 8 bits need the dtype of the keys and values")
+        self.dtype = k.dtype if self.bits == 16 else k_params.dtype if self.bits == 4 else dtype
         if self.dtype not in _DTYPES:
             raise TypeError(f"unsupported dtype {self.dtype}: need bfloat16 or float16")
+        if dtype not in (None, self.dtype):
+            raise TypeError(f"dtype {dtype} is not that of the tensors, {self.dtype}")
         if not k.is_cuda:
             raise RuntimeError("pbs_attn_b200 runs on CUDA devices only; there is no CPU path")
         if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
             raise ValueError("k and v pages must have one shape, dtype and device")
-        self.head_dim = row * 16 // self.bits if self.bits == 16 else 2 * row
-        self.group_size = 0
+        self.head_dim = 2 * row if self.bits == 4 else row
+        self.group_size = self.block_size = 0
+        if self.bits != 16 and (v_params.shape != k_params.shape or v_params.dtype != k_params.dtype or k_params.device != k.device or v_params.device != k.device):
+            raise ValueError("k_params and v_params must have one shape and dtype, and the pages' device")
         if self.bits == 4:
-            if (k_params.dim() != 5 or k_params.shape[:3] != k.shape[:3] or k_params.shape[4] != 2 or v_params.shape != k_params.shape
-                    or v_params.dtype != k_params.dtype or self.head_dim % k_params.shape[3] or k_params.device != k.device
-                    or v_params.device != k.device):
+            if k_params.dim() != 5 or k_params.shape[:3] != k.shape[:3] or k_params.shape[4] != 2 or self.head_dim % k_params.shape[3]:
                 raise ValueError("k_params and v_params must be (pages, heads, page_size, head_dim / group_size, 2)")
             self.group_size = self.head_dim // k_params.shape[3]
+        elif self.bits == 8:
+            if k_params.dim() != 3 or k_params.shape[:2] != k.shape[:2] or k_params.shape[2] < 1 or page_size % k_params.shape[2]:
+                raise ValueError("k_params and v_params must be (pages, heads, page_size / block_size)")
+            if k_params.dtype != torch.float32:
+                raise TypeError("scales must be float32")
+            self.block_size = page_size // k_params.shape[2]
         elif k_params is not None or v_params is not None:
             raise ValueError("pages of 16 bits have no params")
         for t in (k, v):
@@ -119,10 +142,10 @@ class PagedKVCache:
         self.k, self.v, self.k_params, self.v_params = k, v, k_params, v_params
         self.num_pages, self.kv_heads, self.page_size, self.device = pages, heads, page_size, k.device
         three = lambda t: (C.c_int64 * 3)(*(t.stride()[:3] if t is not None else (0, 0, 0)))  # noqa: E731
+        params = [None if t is None else t.data_ptr() for t in (k_params, v_params)]
         self._word = _status_word(self.device)
-        self._c = _cabi.PagedCache(k.data_ptr(), v.data_ptr(), k_params.data_ptr() if self.bits == 4 else None,
-                                   v_params.data_ptr() if self.bits == 4 else None, three(k), three(v), three(k_params), three(v_params),
-                                   pages, page_size, heads, self.head_dim, _DTYPES[self.dtype], self.bits, self.group_size, 0,
+        self._c = _cabi.PagedCache(k.data_ptr(), v.data_ptr(), *params, three(k), three(v), three(k_params), three(v_params),
+                                   pages, page_size, heads, self.head_dim, _DTYPES[self.dtype], self.bits, self.group_size, self.block_size,
                                    C.addressof(self._word))
         # what the sizes alone decide is refused here, not at the first call
         bytes_ = C.c_int64()

@@ -1,0 +1,230 @@
+"""Attention of new tokens over a paged cache of 8 bits, against the formula in 64 bits on the values that the cache stands for."""
+import math
+
+import pytest
+import torch
+
+from paged_ref import assert_within, ints, make_table, pages_for
+from paged_ref8 import attention8, make_cache8
+
+pytestmark = pytest.mark.gpu
+
+
+def _case(lens, Hq=8, Hkv=2, S=1, D=128, dtype=torch.bfloat16, block=16, ps=64, seed=0, token_major=False, spread=1.0, spare=0):
+    """A cache with `lens` tokens, and queries: some keys are what the queries look for, some tokens are large."""
+    from pbs_attn_b200.decode import paged_kv_append
+    cache = make_cache8(pages_for(lens, ps), ps, Hkv, D, dtype, block, token_major)
+    table = make_table(cache, lens, seed, spare)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    n = max(max(lens), 1)
+    x = lambda h, s: torch.randn(len(lens), s, h, D, generator=g, device="cuda").transpose(1, 2)  # noqa: E731
+    shared = torch.randn(D, generator=g, device="cuda")
+    shared /= shared.norm()
+    k, v, q = x(Hkv, n), x(Hkv, n), x(Hq, S)
+    k += 4 * spread * shared * (torch.rand(len(lens), 1, n, 1, generator=g, device="cuda") < 0.05)
+    v *= torch.where(torch.rand(len(lens), Hkv, n, 1, generator=g, device="cuda") < 0.05, 8.0, 1.0)
+    q = (q + 2 * spread * shared).to(dtype)
+    if max(lens):
+        paged_kv_append(cache, k.to(dtype), v.to(dtype), table, ints(*lens), new_lens=ints(*lens))
+    return q, cache, table
+
+
+def _run(q, cache, table, lens, new=None, **kw):
+    from pbs_attn_b200.decode import paged_attn_fwd
+    got = paged_attn_fwd(q, cache, table, ints(*lens), new_lens=None if new is None else ints(*new), **kw)
+    cache.check_status()
+    assert got.shape == q.shape and got.dtype == q.dtype
+    assert_within(got, *attention8(q, cache, table, lens, new, kw.get("scale")))
+    return got
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("Hq,Hkv,S", [(4, 4, 1), (7, 1, 1), (8, 1, 1), (16, 2, 2), (28, 4, 5), (12, 1, 3), (20, 1, 1), (14, 2, 4)])
+def test_types_and_heads(dtype, D, Hq, Hkv, S):
+    lens = [300, 5, 77]
+    _run(*_case(lens, Hq, Hkv, S, D, dtype, block=(16, 32, 64)[Hq % 3]), lens)
+
+
+@pytest.mark.parametrize("block", [16, 64])
+@pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 511, 513, 1000, 2049, 5000])
+def test_lengths(block, n):
+    _run(*_case([n], block=block, seed=n), [n])
+
+
+@pytest.mark.parametrize("ps,block", [(16, 16), (32, 16), (32, 32), (64, 32), (128, 64), (1024, 16), (1024, 64)])
+@pytest.mark.parametrize("token_major", [False, True])
+def test_pages(ps, block, token_major):
+    lens = [1, ps - 1, ps, ps + 1, 3 * ps + 5]
+    _run(*_case(lens, block=block, ps=ps, token_major=token_major, spare=2), lens)
+
+
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("S,new", [(4, [4, 1, 0, 3, 2]), (9, None), (33, [33, 1, 20, 0, 7]), (40, None)])
+def test_new_tokens_that_differ_in_number_and_rows_that_see_nothing(block, S, new):
+    lens = [200, 0, 33, 3, 1]
+    _run(*_case(lens, 14, 2, S, block=block), lens, new)
+
+
+def test_many_sequences_of_all_lengths():
+    lens = [int(x) for x in torch.randint(0, 700, (150,), generator=torch.Generator().manual_seed(1))]
+    lens[7], lens[80] = 6000, 0
+    for dtype in (torch.bfloat16, torch.float16):
+        _run(*_case(lens, 8, 2, 1, dtype=dtype, ps=16), lens)
+
+
+def test_one_long_sequence():
+    _run(*_case([70001], 8, 1, 1, spread=1.5), [70001])
+    _run(*_case([70001], 8, 1, 1, dtype=torch.float16, block=64), [70001])
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-6, 1.0, 30.0, -0.1])
+def test_scales(scale):
+    lens = [400]
+    _run(*_case(lens), lens, scale=scale)
+
+
+def test_layouts_of_queries_and_result():
+    from pbs_attn_b200.decode import paged_attn_fwd
+    lens = [70, 200]
+    q, cache, table = _case(lens, S=3)
+    want = _run(q, cache, table, lens)
+    assert want.stride() == q.stride()
+    assert torch.equal(_run(q.contiguous(), cache, table, lens), want)
+    odd = torch.zeros(*q.shape[:3], 129, dtype=q.dtype, device="cuda")[..., 1:]
+    odd.copy_(q)
+    assert torch.equal(_run(odd, cache, table, lens), want)
+    out = torch.zeros(2, 11, 3, 128, dtype=q.dtype, device="cuda")
+    part = out[:, 2:10]
+    assert paged_attn_fwd(q, cache, table, ints(*lens), out=part) is part and torch.equal(part, want)
+    assert (out[:, :2] == 0).all() and (out[:, 10:] == 0).all()
+    same = q.clone(memory_format=torch.preserve_format)
+    assert paged_attn_fwd(same, cache, table, ints(*lens), out=same) is same and torch.equal(same, want)
+    _run(q[:, :1].expand(2, 8, 3, 128), cache, table, lens)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_scores_and_values_of_very_different_sizes(dtype):
+    """Maxima that rise from tile to tile, queries and values far from 1, steps that differ from block to block by up to 2^18."""
+    from pbs_attn_b200.decode import paged_kv_append
+    n, D, ps = 900, 128, 16
+    big = 2.0 ** 9 if dtype == torch.float16 else 2.0 ** 30
+    for q_size, k_size, v_size in ((1, 1, 1), (1 / big, big, 1 / big), (big, 1 / big, big), (1, 1, 2.0 ** -12)):
+        g = torch.Generator(device="cuda").manual_seed(3)
+        cache = make_cache8(60, ps, 1, D, dtype, 16)
+        x = lambda s: torch.randn(1, 1, s, D, generator=g, device="cuda")  # noqa: E731
+        k = x(n) * torch.linspace(0.1, 6, n, device="cuda")[:, None] * k_size
+        v = x(n) * 2.0 ** (torch.arange(n, device="cuda") // 16 % 10 * 2 - 12)[:, None] * v_size
+        q = (torch.randn(1, 8, 1, D, generator=g, device="cuda") * q_size).to(dtype)
+        table = torch.arange(60, dtype=torch.int32, device="cuda")[None]
+        paged_kv_append(cache, k.to(dtype), v.to(dtype), table, ints(n))
+        _run(q, cache, table, [n])
+
+
+def test_blocks_of_zeros_and_values_near_the_ends_of_bf16():
+    from pbs_attn_b200.decode import paged_kv_append
+    D, ps, n = 64, 16, 200
+    table = torch.arange(13, dtype=torch.int32, device="cuda")[None]
+    for size in (0.0, 2.0 ** -80, 2.0 ** 100):
+        g = torch.Generator(device="cuda").manual_seed(8)
+        cache = make_cache8(13, ps, 1, D, torch.bfloat16, 16)
+        x = torch.randn(2, 1, 1, n, D, generator=g, device="cuda")
+        v = x[1] * size
+        v[:, :, 32:64] = 0
+        q = torch.randn(1, 4, 1, D, generator=g, device="cuda").bfloat16()
+        paged_kv_append(cache, x[0].bfloat16(), v.bfloat16(), table, ints(n))
+        _run(q, cache, table, [n])
+        # keys that are all 0: every token weighs the same
+        cache = make_cache8(13, ps, 1, D, torch.bfloat16, 16)
+        paged_kv_append(cache, x[0].bfloat16() * 0, v.bfloat16(), table, ints(n))
+        _run(q, cache, table, [n])
+
+
+def test_what_a_row_does_not_see_does_not_reach_it():
+    """Blocks behind a row's last token that are not finite, stale pages among them; a block that a row sees makes it NaN."""
+    from pbs_attn_b200.decode import paged_attn_fwd, paged_kv_append
+    lens = [100]
+    q, cache, table = _case(lens, S=30, block=16, ps=16)
+    want = _run(q, cache, table, lens)
+    k = torch.full((1, 2, 4, 128), math.nan, dtype=torch.bfloat16, device="cuda")
+    cache.k_params[table[0, 6].long()] = math.nan             # tokens 96 .. 99, seen by the last four rows
+    cache.v_params[table[0, 6].long()] = math.inf
+    got = paged_attn_fwd(q, cache, table, ints(*lens))
+    assert got[:, :, 26:].isnan().all()
+    assert torch.equal(got[:, :, :26], want[:, :, :26])
+    # and before the row's own end in its block
+    lens2 = [96]
+    again = paged_attn_fwd(q[:, :, :26], cache, table, ints(*lens2))
+    assert not again.isnan().any()
+    assert_within(again, *attention8(q[:, :, :26], cache, table, lens2))
+    paged_kv_append(cache, k, k, table, ints(100))
+    assert paged_attn_fwd(q, cache, table, ints(100))[:, :, 26:].isnan().all()
+
+
+def test_pages_that_are_not_there():
+    from pbs_attn_b200 import _cabi
+    from pbs_attn_b200.decode import paged_attn_fwd
+    lens = [100]
+    q, cache, table = _case(lens, ps=16)
+    bad = table.clone()
+    bad[0, 2] = 99
+    got = paged_attn_fwd(q, cache, bad, ints(*lens))
+    with pytest.raises(_cabi.PbsError, match="outside the pool"):
+        cache.check_status()
+    want = torch.cat([table[:, :2], table[:, 3:]], 1)         # (attention does not ask where a token is)
+    assert_within(got, *attention8(q, cache, want, [84]))
+
+
+def test_same_bits_through_python_and_again(monkeypatch):
+    from pbs_attn_b200.decode import paged_attn_fwd, paged_kv_append, paged_kv_gather
+    lens = [3000, 17]
+    q, cache, table = _case(lens, S=2)
+    n = ints(*lens)
+    k, v = q[:, :2].clone(), q[:, 2:4].clone()
+    native = cache._native
+    assert native is not None
+    results = []
+    for handle in (native, None, native):
+        monkeypatch.setattr(cache, "_native", handle)
+        paged_kv_append(cache, k, v, table, n)
+        results.append([paged_attn_fwd(q, cache, table, n), *paged_kv_gather(cache, table, n, 50), cache.k.clone(), cache.v_params.clone()])
+    for other in results[1:]:
+        assert all(torch.equal(a.nan_to_num(7), b.nan_to_num(7)) for a, b in zip(results[0], other))
+
+
+def test_captured_and_replayed_beside_other_streams():
+    from pbs_attn_b200.decode import paged_attn_fwd
+    lens = [5000, 700]
+    q, cache, table = _case(lens)
+    q2, cache2, table2 = _case(lens, seed=5)
+    n = ints(*lens)
+    want, want2 = paged_attn_fwd(q, cache, table, n), paged_attn_fwd(q2, cache2, table2, n)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = paged_attn_fwd(q, cache, table, n)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        with torch.cuda.stream(side):
+            got2 = paged_attn_fwd(q2, cache2, table2, n)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(got2, want2)
+        out.zero_()
+    cache.check_status()
+
+
+def test_written_rows_attended_rows_and_rows_behind_them():
+    """Append and attention together, token by token, each step against the formula on what the cache stands for."""
+    from pbs_attn_b200.decode import paged_kv_append
+    lens = [29, 64]
+    q, cache, table = _case(lens, ps=32, block=16, spare=2)
+    g = torch.Generator(device="cuda").manual_seed(11)
+    free = [p for p in range(cache.num_pages) if p not in table[0, :1].tolist() + table[1, :2].tolist()]
+    table[0, 1], table[1, 2] = free[0], free[1]
+    for step in range(12):
+        lens = [n + 1 for n in lens]
+        x = torch.randn(3, 2, 2, 1, 128, generator=g, device="cuda").mul(1 + step / 3).bfloat16()
+        paged_kv_append(cache, x[0], x[1], table, ints(*lens))
+        _run(q, cache, table, lens)
