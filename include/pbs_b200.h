@@ -314,6 +314,7 @@ typedef struct {
 #define PBS_PAGED_BAD_PAGE 1    /* a page number outside the pool: such a token is neither written nor attended  */
 #define PBS_PAGED_BAD_LENGTH 2  /* a sequence longer than its row of the block table: it ends with that row      */
 #define PBS_PAGED_BAD_ROTARY 3  /* a position behind the rotary tables: the token is neither rotated nor written */
+#define PBS_PAGED_BAD_BEAM 5    /* pbs_paged_reorder: a parent outside the group, or of another length: the row stays as it is */
 #define PBS_PAGED_TIMEOUT 4     /* pbs_paged_attn: a bounded wait ran out; the output is invalid, and those of later calls with the same
                                    workspace are until its first PBS_PAGED_COUNTER_BYTES have been cleared */
 
@@ -406,6 +407,40 @@ typedef struct {
   int64_t allowed_stride;         /* words from row to row (0 to share)                         */
 } pbs_logits_t;
 int pbs_process_logits(const pbs_logits_t* args, void* stream);
+
+/* The best continuations of beams.  For each batch entry, over its beams i and all tokens v,
+ *   score(i, v) = scores[i] + logits[i][v] - log(sum over u of exp(logits[i][u])),
+ * the `keep` largest, larger ones first: scores, beams and tokens.  Of equal scores the lower beam comes first, within a beam the larger logit,
+ * of equal ones the lower token.  A NaN counts as -infinity, a logit of +infinity as the largest number of 32 bits.  Beams whose score is
+ * -infinity are not alive (their tokens come in their order, with -infinity, where there is nothing else).  Scores are formed in 64 bits from sums
+ * in 32 and rounded once.
+ * workspace: pbs_beam_select_workspace bytes; its first PBS_PAGED_COUNTER_BYTES are 0 before the first call and each call leaves them so.
+ * Calls that share one come after one another. */
+typedef struct {
+  int32_t dtype;                  /* pbs_dtype_t of logits                                       */
+  int32_t batch;                  /* entries, at most 1024                                       */
+  int32_t beams;                  /* 1 .. 32                                                     */
+  int32_t vocab;
+  int32_t keep;                   /* 1 .. 64, at most beams * vocab                              */
+  int32_t reserved;
+  const void* logits;             /* (batch * beams, vocab)                                      */
+  int64_t logits_stride;          /* elements from row to row                                    */
+  const float* scores;            /* (batch, beams)                                              */
+  int64_t scores_stride;          /* elements from entry to entry                                */
+  float* out_scores;              /* (batch, keep), dense                                        */
+  int32_t* out_beams;             /* (batch, keep), dense                                        */
+  int64_t* out_tokens;            /* (batch, keep), dense                                        */
+} pbs_beam_select_t;
+int pbs_beam_select_workspace(const pbs_beam_select_t* args, int64_t* bytes);
+int pbs_beam_select(const pbs_beam_select_t* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Row b * beams + i of the batch goes on from row b * beams + parents[b][i], for all i at once: `batch` counts the rows, a multiple of
+ * beams (1 .. 32), and seq_lens the tokens that their caches hold; new_tokens and new_lens are not looked at.  In the table, which is
+ * written, entries of full pages become those of the parent; tokens of the page under way are copied, in the caches of all layers, from the
+ * parent's page into the row's own (which no other row uses), with what stands for them.  A row and its parent have one length.
+ * The caches have one layout: their pages, params and status may differ, the other members not. */
+int pbs_paged_reorder(const pbs_paged_cache_t* const* caches, int32_t layers, const pbs_paged_batch_t* batch, int32_t* block_table,
+                      int32_t beams, const int32_t* parents, int64_t parents_stride, void* stream);
 
 #ifdef __cplusplus
 }

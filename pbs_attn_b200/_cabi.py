@@ -81,6 +81,12 @@ class Logits(C.Structure):
                    ("bias_values_stride", C.c_int64), ("allowed", C.c_void_p), ("allowed_stride", C.c_int64)])
 
 
+class BeamSelect(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "batch", "beams", "vocab", "keep", "reserved")]
+                + [("logits", C.c_void_p), ("logits_stride", C.c_int64), ("scores", C.c_void_p), ("scores_stride", C.c_int64)]
+                + [(n, C.c_void_p) for n in ("out_scores", "out_beams", "out_tokens")])
+
+
 _P = C.c_void_p
 _SH = C.POINTER(Shape)
 _ST = C.POINTER(C.c_int64)
@@ -110,6 +116,9 @@ SIGNATURES = {
     "pbs_paged_gather": [_PC, _PB, _P, _ST, _P, _ST, _P],
     "pbs_paged_attn_workspace": [_PC, _PB, C.c_int32, C.POINTER(C.c_int64)],
     "pbs_paged_attn": [_PC, _PB, C.c_int32, _P, _ST, _P, _ST, C.c_float, _P, C.c_int64, _P],
+    "pbs_paged_reorder": [C.POINTER(_PC), C.c_int32, _PB, _P, C.c_int32, _P, C.c_int64, _P],
+    "pbs_beam_select_workspace": [C.POINTER(BeamSelect), C.POINTER(C.c_int64)],
+    "pbs_beam_select": [C.POINTER(BeamSelect), _P, C.c_int64, _P],
     "pbs_process_logits": [C.POINTER(Logits), _P],
 }
 EXPORTS = ["pbs_last_error_string", "pbs_version", "pbs_launch_count"] + list(SIGNATURES)

@@ -1,4 +1,4 @@
-// The calls of decode.py and logits.py without Python in between, for plain CUDA tensors that the kernels can read in place.  Whatever they do not cover they leave, untouched, to the Python code (they return None), which also raises all errors.
+// The calls of decode.py, logits.py and beam.py without Python in between, for plain CUDA tensors that the kernels can read in place.  Whatever they do not cover they leave, untouched, to the Python code (they return None), which also raises all errors.
 // A step's kernels take a few us; through Python and ctypes a call of the attention over 187 tokens took 24 us and one of the logits 30,
 // here 6 and 6.
 #include "host_common.h"
@@ -81,7 +81,10 @@ bool batch_of(const Cache* c, PyObject* table, PyObject* lens, PyObject* new_len
 
 // Memory for partial results, one piece a stream, or a stream of a capture: calls there come after one another.  A capture's comes from
 // its graph's own pool and is cleared by the graph, once for all its calls.
+// What one kind of call leaves behind in an error is nothing to the others: each has its own.
+enum Kind { kAttention, kBeams };
 struct Space {
+  Kind kind;
   int device;
   cudaStream_t st;
   unsigned long long capture;                                      // 0: none
@@ -98,16 +101,16 @@ std::vector<Space>& spaces() {
 
 // The place of a stream's memory, which is what `memory` is undefined for where there is none yet.  What makes room are the captures before
 // this one, whose graphs no longer ask (what they hold would keep those graphs' pools), then what was used longest ago.
-at::Tensor& space_of(int device, cudaStream_t st, unsigned long long capture) {
+at::Tensor& space_of(Kind kind, int device, cudaStream_t st, unsigned long long capture) {
   std::vector<Space>& s = spaces();
   for (size_t i = s.size(); i-- > 0;) {
-    if (s[i].device != device || s[i].st != st || s[i].capture != capture) continue;
+    if (s[i].kind != kind || s[i].device != device || s[i].st != st || s[i].capture != capture) continue;
     std::rotate(s.begin() + i, s.begin() + i + 1, s.end());
     return s.back().memory;
   }
   s.erase(std::remove_if(s.begin(), s.end(), [&](const Space& x) { return x.capture != 0 && x.capture != capture; }), s.end());
   if (s.size() >= kMaxSpaces) s.erase(s.begin());
-  s.push_back(Space{device, st, capture, at::Tensor()});
+  s.push_back(Space{kind, device, st, capture, at::Tensor()});
   return s.back().memory;
 }
 
@@ -136,7 +139,7 @@ PyObject* py_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (status == cudaStreamCaptureStatusNone) capture = 0;
   at::Tensor out = a[6] == Py_None ? at::empty_like(q) : THPVariable_Unpack(a[6]);
   if (!readable(out, false)) Py_RETURN_NONE;
-  at::Tensor& space = space_of(c->device, st, capture);
+  at::Tensor& space = space_of(kAttention, c->device, st, capture);
   int rc = PBS_ERR_SHAPE;
   for (int round = 0; rc == PBS_ERR_SHAPE && round < 2; ++round) {
     if (round == 1 || !space.defined()) {                          // too small, perhaps
@@ -314,6 +317,100 @@ PyObject* py_logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// paged_reorder(function, caches, table, lens, beams): True, or False where Python has to do it
+PyObject* py_reorder(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5 || !PyList_CheckExact(a[1])) { PyErr_SetString(PyExc_TypeError, "paged_reorder takes 5 arguments, the second a list"); return nullptr; }
+  const auto fn = reinterpret_cast<decltype(&pbs_paged_reorder)>(PyLong_AsUnsignedLongLong(a[0]));
+  if (!fn) { if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "no function"); return nullptr; }
+  const Py_ssize_t layers = PyList_GET_SIZE(a[1]);
+  std::vector<const pbs_paged_cache_t*> caches((size_t)layers);
+  Cache* first = nullptr;
+  for (Py_ssize_t i = 0; i < layers; ++i) {
+    PyObject* o = PyList_GET_ITEM(a[1], i);
+    if (!PyCapsule_IsValid(o, kName)) Py_RETURN_FALSE;
+    Cache* c = get(o);
+    if (!first) first = c;
+    if (c->device != first->device) Py_RETURN_FALSE;
+    caches[(size_t)i] = c->c;
+  }
+  if (!first || layers > INT32_MAX || !dense_on(a[3], first->device, at::kInt, 1) || !dense_on(a[4], first->device, at::kInt, 2) ||
+      at::impl::torch_function_mode_enabled())
+    Py_RETURN_FALSE;
+  const at::Tensor& beams = THPVariable_Unpack(a[4]);
+  const int64_t rows = THPVariable_Unpack(a[3]).size(0);
+  pbs_paged_batch_t batch;
+  if (!batch_of(first, a[2], a[3], Py_None, rows, 1, &batch) || beams.size(0) * beams.size(1) != rows) Py_RETURN_FALSE;
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)first->device);
+  const cudaStream_t st = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)first->device).stream();
+  if (fn(caches.data(), (int32_t)layers, &batch, const_cast<int32_t*>(batch.block_table), (int32_t)beams.size(1), static_cast<const int32_t*>(beams.data_ptr()),
+         beams.stride(0), st) != PBS_OK)
+    Py_RETURN_FALSE;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// beam_select(function, workspace_function, logits, scores, keep): (scores, beams, tokens), or None
+PyObject* py_beams(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5) { PyErr_SetString(PyExc_TypeError, "beam_select takes 5 arguments"); return nullptr; }
+  const auto fn = reinterpret_cast<decltype(&pbs_beam_select)>(PyLong_AsUnsignedLongLong(a[0]));
+  const auto ws = reinterpret_cast<decltype(&pbs_beam_select_workspace)>(PyLong_AsUnsignedLongLong(a[1]));
+  if (!fn || !ws) { if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "no function"); return nullptr; }
+  if (!plain(a[2]) || at::impl::torch_function_mode_enabled()) Py_RETURN_NONE;
+  const at::Tensor& x = THPVariable_Unpack(a[2]);
+  const auto type = x.scalar_type();
+  if (!x.is_cuda() || (type != at::kBFloat16 && type != at::kHalf && type != at::kFloat)) Py_RETURN_NONE;
+  const int device = x.device().index();
+  if (!dense_on(a[2], device, type, 2) || !dense_on(a[3], device, at::kFloat, 2)) Py_RETURN_NONE;
+  const at::Tensor& s = THPVariable_Unpack(a[3]);
+  const int64_t B = s.size(0), N = s.size(1);
+  int64_t keep = 2 * N;
+  if (a[4] != Py_None) {
+    int over = 0;
+    if (!PyLong_CheckExact(a[4])) Py_RETURN_NONE;
+    keep = PyLong_AsLongLongAndOverflow(a[4], &over);
+    if (over) Py_RETURN_NONE;
+  }
+  if (B < 1 || N < 1 || B > 1024 || N > 32 || x.size(0) != B * N || x.size(1) < 1 || x.size(1) > (1 << 30) || keep < 1 || keep > 64) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  const cudaStream_t st = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+  cudaStreamCaptureStatus status;
+  unsigned long long capture = 0;
+  if (cudaStreamGetCaptureInfo(st, &status, &capture) != cudaSuccess || status == cudaStreamCaptureStatusInvalidated) Py_RETURN_NONE;
+  if (status == cudaStreamCaptureStatusNone) capture = 0;
+  const auto opt = at::TensorOptions().device(at::Device(at::kCUDA, (c10::DeviceIndex)device));
+  at::Tensor scores = at::empty({B, keep}, opt.dtype(at::kFloat)), beams = at::empty({B, keep}, opt.dtype(at::kInt)), tokens = at::empty({B, keep}, opt.dtype(at::kLong));
+  pbs_beam_select_t g = {};
+  g.dtype = type == at::kBFloat16 ? PBS_BF16 : type == at::kHalf ? PBS_FP16 : PBS_FP32;
+  g.batch = (int32_t)B;
+  g.beams = (int32_t)N;
+  g.vocab = (int32_t)x.size(1);
+  g.keep = (int32_t)keep;
+  g.logits = x.data_ptr();
+  g.logits_stride = x.stride(0);
+  g.scores = static_cast<const float*>(s.data_ptr());
+  g.scores_stride = s.stride(0);
+  g.out_scores = static_cast<float*>(scores.data_ptr());
+  g.out_beams = static_cast<int32_t*>(beams.data_ptr());
+  g.out_tokens = static_cast<int64_t*>(tokens.data_ptr());
+  at::Tensor& space = space_of(kBeams, device, st, capture);
+  int rc = PBS_ERR_SHAPE;
+  for (int round = 0; rc == PBS_ERR_SHAPE && round < 2; ++round) {
+    if (round == 1 || !space.defined()) {                          // too small, perhaps
+      int64_t need = 0;
+      if (ws(&g, &need) != PBS_OK || (space.defined() && need <= space.numel())) Py_RETURN_NONE;
+      space = at::zeros({need}, opt.dtype(at::kByte));
+    }
+    rc = fn(&g, space.data_ptr(), space.numel(), st);
+  }
+  if (rc != PBS_OK) Py_RETURN_NONE;
+  THPObjectPtr o0(THPVariable_Wrap(std::move(scores))), o1(THPVariable_Wrap(std::move(beams))), o2(THPVariable_Wrap(std::move(tokens)));
+  if (!o0 || !o1 || !o2) return nullptr;
+  return PyTuple_Pack(3, o0.get(), o1.get(), o2.get());
+  END_HANDLE_TH_ERRORS
+}
+
 // paged_forget(): the next calls make new workspaces
 PyObject* py_forget(PyObject*, PyObject*) {
   spaces().clear();
@@ -331,5 +428,7 @@ PyMethodDef pbs_decode_methods[] = {
     {"paged_append", fast(py_append), METH_FASTCALL, "paged_append(cache, k, v, table, lens, new_lens, cos, sin, q, q_out): the rotated queries, True, or None where Python has to do it"},
     {"paged_gather", fast(py_gather), METH_FASTCALL, "paged_gather(cache, table, lens, count, new_lens): (keys, values), or None where Python has to do it"},
     {"paged_attn", fast(py_attn), METH_FASTCALL, "paged_attn(cache, q, table, lens, new_lens, scale, out): the result, or None where Python has to do it"},
+    {"paged_reorder", fast(py_reorder), METH_FASTCALL, "paged_reorder(function, caches, table, lens, beams): True, or False where Python has to do it"},
+    {"beam_select", fast(py_beams), METH_FASTCALL, "beam_select(function, workspace_function, logits, scores, keep): (scores, beams, tokens), or None where Python has to do it"},
     {"process_logits", fast(py_logits), METH_FASTCALL, "process_logits(function, logits, ...): the result, or None where Python has to do it"},
     {nullptr, nullptr, 0, nullptr}};

@@ -68,6 +68,27 @@ int check_count(const PagedArgs& a, int64_t heads) {
   return PBS_OK;
 }
 
+int check_beams(const pbs_beam_select_t* a) {
+  PBS_NONNULL(a);
+  if (a->dtype < PBS_BF16 || a->dtype > PBS_FP32) { set_error("dtype %d is not bf16/fp16/fp32", a->dtype); return PBS_ERR_ARG; }
+  if (a->batch < 1 || a->batch > 1024 || a->beams < 1 || a->beams > 32 || a->vocab < 1 || a->vocab > (1 << 30)) {
+    set_error("beam selection: %d entries (1 .. 1024) of %d beams (1 .. 32) of %d tokens", a->batch, a->beams, a->vocab);
+    return PBS_ERR_SHAPE;
+  }
+  if (a->keep < 1 || a->keep > 64 || a->keep > (int64_t)a->beams * a->vocab) { set_error("beam selection: keep %d, need 1 .. 64 and no more than there are", a->keep); return PBS_ERR_SHAPE; }
+  PBS_NONNULL(a->logits);
+  PBS_NONNULL(a->scores);
+  PBS_NONNULL(a->out_scores);
+  PBS_NONNULL(a->out_beams);
+  PBS_NONNULL(a->out_tokens);
+  if ((uintptr_t)a->logits % elem_bytes(a->dtype) || a->logits_stride < 0 || a->scores_stride < 0 || ((uintptr_t)a->scores | (uintptr_t)a->out_scores | (uintptr_t)a->out_beams) % 4 ||
+      (uintptr_t)a->out_tokens % 8) {
+    set_error("beam selection: pointers must be aligned to their elements, strides must not be negative");
+    return PBS_ERR_LAYOUT;
+  }
+  return PBS_OK;
+}
+
 int check_q_heads(const PagedArgs& a, int q_heads) {
   if (q_heads < 1 || q_heads % a.c.kv_heads) { set_error("kv_heads %d does not divide q_heads %d", a.c.kv_heads, q_heads); return PBS_ERR_SHAPE; }
   return check_count(a, q_heads);
@@ -147,6 +168,51 @@ int pbs_paged_attn(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* batc
   PBS_TRY(paged_attn_workspace(a, q_heads, &need));
   if (workspace_bytes < need) { set_error("workspace: %lld bytes, need %lld", (long long)workspace_bytes, (long long)need); return PBS_ERR_SHAPE; }
   return launch_paged_attn(a, q_heads, qt, ot, scale, workspace, (cudaStream_t)stream);
+}
+
+int pbs_paged_reorder(const pbs_paged_cache_t* const* caches, int32_t layers, const pbs_paged_batch_t* batch, int32_t* block_table, int32_t beams,
+                      const int32_t* parents, int64_t parents_stride, void* stream) {
+  PBS_NONNULL(caches);
+  PBS_NONNULL(batch);
+  PBS_NONNULL(block_table);
+  PBS_NONNULL(parents);
+  if (layers < 1) { set_error("%d layers", layers); return PBS_ERR_SHAPE; }
+  if (beams < 1 || beams > 32 || batch->batch % beams) { set_error("%d rows in groups of %d: need 1 .. 32 that divide them", batch->batch, beams); return PBS_ERR_SHAPE; }
+  if (parents_stride < 0 || (batch->batch > 1 && batch->table_stride < batch->max_pages)) { set_error("rows of the block table share memory, or a negative stride"); return PBS_ERR_LAYOUT; }
+  PagedArgs a;
+  pbs_paged_batch_t b = *batch;
+  b.block_table = block_table;
+  b.new_tokens = 1;
+  b.new_lens = nullptr;
+  for (int32_t l = layers - 1; l >= 0; --l) {              // (the first stays in a)
+    PBS_TRY(check_paged(caches[l], &b, &a));
+    const pbs_paged_cache_t &c = *caches[l], &d = *caches[0];
+    bool same = c.num_pages == d.num_pages && c.page_size == d.page_size && c.kv_heads == d.kv_heads && c.head_dim == d.head_dim && c.bits == d.bits;
+    same = same && (c.bits != 4 || c.group_size == d.group_size) && (c.bits != 8 || c.block_size == d.block_size) && (c.bits == 16 || c.dtype == d.dtype);
+    for (int i = 0; i < 3; ++i) {
+      same = same && c.k_strides[i] == d.k_strides[i] && c.v_strides[i] == d.v_strides[i];
+      same = same && (c.bits == 16 || (c.k_params_strides[i] == d.k_params_strides[i] && c.v_params_strides[i] == d.v_params_strides[i]));
+    }
+    if (!same) { set_error("the caches of a call have one layout: that of layer %d differs from the first's", l); return PBS_ERR_SHAPE; }
+  }
+  if (a.c.kv_heads > (INT_MAX >> 1)) { set_error("%d heads", a.c.kv_heads); return PBS_ERR_SHAPE; }
+  return launch_paged_reorder(a, caches, layers, block_table, parents, parents_stride, beams, (cudaStream_t)stream);
+}
+
+int pbs_beam_select_workspace(const pbs_beam_select_t* args, int64_t* bytes) {
+  PBS_NONNULL(bytes);
+  PBS_TRY(check_beams(args));
+  return beam_select_workspace(*args, bytes);
+}
+
+int pbs_beam_select(const pbs_beam_select_t* args, void* workspace, int64_t workspace_bytes, void* stream) {
+  PBS_TRY(check_beams(args));
+  PBS_NONNULL(workspace);
+  if ((uintptr_t)workspace % 16) { set_error("workspace: 16-byte alignment"); return PBS_ERR_LAYOUT; }
+  int64_t need;
+  PBS_TRY(beam_select_workspace(*args, &need));
+  if (workspace_bytes < need) { set_error("workspace: %lld bytes, need %lld", (long long)workspace_bytes, (long long)need); return PBS_ERR_SHAPE; }
+  return launch_beam_select(*args, workspace, (cudaStream_t)stream);
 }
 
 int pbs_process_logits(const pbs_logits_t* args, void* stream) {

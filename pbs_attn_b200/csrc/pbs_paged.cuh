@@ -52,6 +52,10 @@ int launch_paged_append(const PagedArgs& a, const RowTensor& k, const RowTensor&
 int launch_paged_gather(const PagedArgs& a, const RowTensor& k, const RowTensor& v, cudaStream_t st);
 int paged_attn_workspace(const PagedArgs& a, int q_heads, int64_t* bytes);
 int launch_paged_attn(const PagedArgs& a, int q_heads, const RowTensor& q, const RowTensor& out, float scale, void* workspace, cudaStream_t st);
+int launch_paged_reorder(const PagedArgs& a, const pbs_paged_cache_t* const* caches, int layers, int32_t* table, const int32_t* beams, int64_t beams_stride, int n,
+                         cudaStream_t st);
+int beam_select_workspace(const pbs_beam_select_t& a, int64_t* bytes);
+int launch_beam_select(const pbs_beam_select_t& a, void* workspace, cudaStream_t st);
 int launch_process_logits(const pbs_logits_t& a, cudaStream_t st);
 
 }  // namespace pbs

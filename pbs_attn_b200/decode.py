@@ -3,6 +3,7 @@
     cache = PagedKVCache(num_pages, page_size, kv_heads, head_dim, torch.bfloat16, "cuda", bits=4)     # one per layer
     q = paged_kv_append(cache, k, v, block_table, seq_lens, cos=cos, sin=sin, query_states=q)
     o = paged_attn_fwd(q, cache, block_table, seq_lens)
+    paged_kv_reorder(caches, block_table, seq_lens, beams)                                             # beams: rows go on from other rows
 
 ``block_table`` (B, pages) int32 names the pages of each sequence, ``seq_lens`` (B,) int32 counts its tokens, those of the call
 among them: token i of the S new ones of sequence b is at position ``seq_lens[b] - S + i`` (with ``new_lens``, (B,) int32, the
@@ -17,7 +18,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from typing import Optional
+from typing import Optional, Sequence, Union
 
 import torch
 
@@ -26,13 +27,14 @@ from .prefill import _ptr, _readable, _strides
 
 _DTYPES = {torch.bfloat16: _cabi.BF16, torch.float16: _cabi.FP16}
 _FAULTS = {1: "a page number in block_table is outside the pool", 2: "a sequence is longer than its row of block_table",
-           3: "a position is behind the rotary tables"}
+           3: "a position is behind the rotary tables", 5: "a beam goes on from one outside its group, or of another length"}
 _TIMEOUT = 4
 
 # One word a device that kernels report a fault in: pinned host memory, looked at without a copy, and never given back, since a kernel
 # may still be on its way when the cache it works on is gone.
 _STATUS: dict = {}
 _ADDRESSES: list = []                   # of the library's functions, as the native calls take them
+_REORDER: list = []                     # that of pbs_paged_reorder
 
 
 def _status_word(device: torch.device) -> C.c_int32:
@@ -278,17 +280,50 @@ def paged_kv_gather(cache: PagedKVCache, block_table: torch.Tensor, seq_lens: to
     return k, v
 
 
-# Memory for partial results, one piece a stream: calls on a stream come after one another.
+def paged_kv_reorder(caches: Union[PagedKVCache, Sequence[PagedKVCache]], block_table: torch.Tensor, seq_lens: torch.Tensor, beams: torch.Tensor):
+    """Rows of groups of N neighbours go on from other rows of their group, all at once: row b * N + i from row b * N + ``beams[b, i]``
+    (``beams`` (B, N) int32, as ``beam_select`` names them; N up to 32), in the caches of all layers, which have one layout.
+
+    ``block_table`` (B * N, pages) is changed in place: full pages are shared with the parent from then on.  The page under way (that of position
+    ``seq_lens``, the tokens that the caches hold) is each row's own, which no other row uses, and takes a copy of the parent's tokens.  A row
+    and its parent have one length.  So with N pages of its own for every page that a group has come to, nothing needs counting of
+    references: pages that rows share are full, and full pages are not written.
+    One kernel for up to 64 layers on the current stream, without synchronising."""
+    caches = (caches,) if isinstance(caches, PagedKVCache) else caches
+    if not len(caches):
+        return
+    first = caches[0]
+    if not _REORDER:
+        _REORDER.append(C.cast(first.lib.pbs_paged_reorder, C.c_void_p).value)
+    if first._native is not None and first._host.paged_reorder(_REORDER[0], [c._native for c in caches], block_table, seq_lens, beams):
+        return
+    rows = block_table.shape[0]
+    batch = _batch(first, rows, 1, block_table, seq_lens, None)
+    if beams.dtype != torch.int32 or beams.device != first.device:
+        raise TypeError(f"beams must be an int32 tensor on {first.device}")
+    if beams.dim() != 2 or beams.shape[0] * beams.shape[1] != rows or beams.stride(1) != 1 and beams.shape[1] > 1:
+        raise ValueError(f"beams must be (groups, rows of a group) for {rows} rows, its last dimension dense")
+    if any(c.device != first.device for c in caches):
+        raise ValueError("the caches of a call are on one device")
+    if rows == 0:
+        return
+    pointers = (C.POINTER(_cabi.PagedCache) * len(caches))(*(C.pointer(c._c) for c in caches))
+    with torch.cuda.device(first.device):
+        _cabi.check(first.lib.pbs_paged_reorder(pointers, len(caches), C.byref(batch), _ptr(block_table), beams.shape[1], _ptr(beams), beams.stride(0),
+                                                _stream(first.device)), "pbs_paged_reorder")
+
+
+# Memory for partial results, one piece a stream and kind of call: calls on a stream come after one another.
 _WORKSPACES: dict = {}
 _MAX_WORKSPACES = 8
 
 
-def _workspace(device: torch.device, need: int) -> torch.Tensor:
+def _workspace(device: torch.device, need: int, kind: str = "attention") -> torch.Tensor:
     if torch.cuda.is_current_stream_capturing():           # a graph is replayed at times and on streams unknown here: it has its own
         space = torch.empty(need, dtype=torch.uint8, device=device)
         space[:_cabi.PAGED_COUNTER_BYTES].zero_()
         return space
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
+    key = (kind, device.index, torch.cuda.current_stream(device).cuda_stream)
     space = _WORKSPACES.pop(key, None)                     # (back in behind the others: what was used longest ago goes first)
     if space is None or space.numel() < need:
         while len(_WORKSPACES) >= _MAX_WORKSPACES:
