@@ -146,11 +146,11 @@ def measure_prefill_latency(model, input_ids) -> float:
     return a.elapsed_time(b) / 1000.0
 
 
-def measure_decode(model, input_ids, tokens: int, bits: int) -> float:
+def measure_decode(model, input_ids, tokens: int, bits: int, beams: int = 1) -> float:
     """Milliseconds per token of ``generate`` behind the prompt, one graph replay each (model patched)."""
     from .generate import generate
     timings = {}
-    generate(model, input_ids, tokens + 2, bits=bits, repetition_penalty=1.1, timings=timings)
+    generate(model, input_ids, tokens + 2, bits=bits, repetition_penalty=1.1, timings=timings, num_beams=beams)
     return timings["ms_per_token"]
 
 
@@ -187,7 +187,8 @@ def main(argv=None):
                     help="time the model a second time with attention replaced by a no-op and report the share")
     ap.add_argument("--decode", type=int, default=0, metavar="N",
                     help="also generate N tokens through the paged cache (generate.py) and report the time of one")
-    ap.add_argument("--cache-bits", type=int, default=4, choices=[4, 16], help="what the paged cache holds keys and values in")
+    ap.add_argument("--cache-bits", type=int, default=4, choices=[4, 8, 16], help="what the paged cache holds keys and values in")
+    ap.add_argument("--num-beams", type=int, default=1, help="beams of the generated tokens")
     ap.add_argument("--out", default=None, help="append the JSON lines to this file (rank 0)")
     args = ap.parse_args(argv)
     if not torch.cuda.is_available():
@@ -256,8 +257,8 @@ def main(argv=None):
         if args.decode:
             remove_patch(model)                                  # (the no-op arm came last)
             apply_patch_with_prefill(model, prefill_function(args.method, args.block_size, args.segment_size, args.threshold))
-            rec.update(decode_tokens=args.decode, cache_bits=args.cache_bits,
-                       decode_ms_per_token=measure_decode(model, ids, args.decode, args.cache_bits))
+            rec.update(decode_tokens=args.decode, cache_bits=args.cache_bits, num_beams=args.num_beams,
+                       decode_ms_per_token=measure_decode(model, ids, args.decode, args.cache_bits, args.num_beams))
         line = json.dumps(rec)
         print(line, flush=True)
         if args.out:
