@@ -3,12 +3,13 @@
 // Within a beam the order of the scores is the order of the logits, so one pass over the logits gives both what the softmax needs (their maximum and
 // the sum of exponentials) and each slice's K largest; scores are formed for these few only, in 64 bits, when a batch entry's slices meet.
 //
-// A CTA keeps its slice of a row in registers (up to kMost 16-byte pieces a thread, all loads under way at once).  The K-th largest of a warp's
-// 32 largest-of-a-lane is a bound that K of the slice's logits reach; what reaches the best warp's bound (some tens of logits) is listed in shared
-// memory and ranked by counting.  Order: (logit, then lower token) as one 64-bit number, so that ties need no case of their own.
-// The CTA that finishes an entry last merges the sorted lists of its rows and slices: K times the best of their heads.
+// A CTA takes a segment of a row, in chunks of two 16-byte pieces a thread; the chunks ahead are on their way to shared memory meanwhile (each
+// thread's own pieces: nobody waits for anybody).  A thread keeps its sum, and the largest logits of its three best chunks.  At the end the
+// threads' largest give a bound that K logits reach, and few more: the chunks that do are looked at once more, their logits listed and ranked by
+// counting.  Order: (logit, then lower token) as one 64-bit number, so that ties need no case of their own.  (With lists kept while streaming,
+// cut down to K now and then, the CTA's warps waited for one another and branched: 76 us for 512 rows of 152064 in fp32.)
+// The CTA that finishes an entry last merges the sorted lists of its segments in the same way, by score.
 #include <climits>
-#include <type_traits>
 
 #include "pbs_paged.cuh"
 
@@ -16,25 +17,39 @@ namespace pbs {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kMost = 8;                  // 16-byte pieces a thread
+constexpr int P = 2, kStages = 4;          // 16-byte pieces of a thread in a chunk; chunks in shared memory, all but one of them on their way
 constexpr int kResident = 4;              // CTAs a SM
-constexpr int kListed = 1024;             // logits that reach the bound; more of them are gone through K times instead
+constexpr int kListed = 1024;             // logits that reach the bound; more of them at a time are gone through K times instead
+constexpr int kFound = 320;               // continuations that do
 constexpr int kMaxBeams = 32;
 constexpr float kFltMax = 3.402823466e38f;
 constexpr float kLog2e = 1.44269504f;
 
 struct BeamArgs {
   pbs_beam_select_t a;
-  int slices, pieces;                     // of a row; of a thread's share of a slice
-  unsigned* counters;                     // by batch entry: slices that are done
-  float2* sums;                           // [row][slice]: maximum, sum of exponentials
-  unsigned long long* lists;              // [row][slice][keep]
+  int slices, chunks, share;              // segments of a row; chunks of a row, and of a segment
+  unsigned* counters;                     // by batch entry: segments that are done
+  float2* sums;                           // by segment: maximum, sum of exponentials
+  unsigned long long* lists;              // by segment: its K largest
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n.reg .b64 a, b, c, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\nfma.rn.f32x2 d, a, b, c;\nmov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 
 // A number whose order is that of (value, then lower token); 0 is none.
@@ -52,22 +67,26 @@ __device__ __forceinline__ double value_of(unsigned long long key) {
   return __longlong_as_double((long long)(key ^ ((long long)key < 0 ? 1ull << 63 : ~0ull)));
 }
 
-// The elements of a 16-byte piece, as floats.
+// The elements of a 16-byte piece, as floats and back.
 template <class T>
 struct Piece;
 template <>
 struct Piece<float> {
   static constexpr int N = 4;
-  static constexpr uint32_t kNever = 0xff800000u;          // -infinity
   static __device__ __forceinline__ void get(const uint4& w, float (&x)[4]) {
     x[0] = __uint_as_float(w.x); x[1] = __uint_as_float(w.y); x[2] = __uint_as_float(w.z); x[3] = __uint_as_float(w.w);
   }
-  static __device__ __forceinline__ uint32_t bits(const float* p) { return __float_as_uint(*p); }
+  static __device__ __forceinline__ uint4 put(const float (&x)[4]) {
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  }
+  static __device__ __forceinline__ float one(const float* p) { return *p; }
+  static __device__ __forceinline__ float most(const uint4& w) {
+    return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+  }
 };
 template <>
 struct Piece<__nv_bfloat16> {
   static constexpr int N = 8;
-  static constexpr uint32_t kNever = 0xff80ff80u;
   static __device__ __forceinline__ void get(const uint4& w, float (&x)[8]) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -76,11 +95,22 @@ struct Piece<__nv_bfloat16> {
       x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
     }
   }
+  static __device__ __forceinline__ uint4 put(const float (&x)[8]) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(x[2 * i]) >> 16 | (__float_as_uint(x[2 * i + 1]) & 0xffff0000u);
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  static __device__ __forceinline__ float most(const uint4& w) {
+    const __nv_bfloat162 m = __hmax2(__hmax2(pair(w.x), pair(w.y)), __hmax2(pair(w.z), pair(w.w)));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ __nv_bfloat162 pair(const uint32_t& u) { return *reinterpret_cast<const __nv_bfloat162*>(&u); }
 };
 template <>
 struct Piece<__half> {
   static constexpr int N = 8;
-  static constexpr uint32_t kNever = 0xfc00fc00u;
   static __device__ __forceinline__ void get(const uint4& w, float (&x)[8]) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -90,21 +120,69 @@ struct Piece<__half> {
       x[2 * i + 1] = f.y;
     }
   }
+  static __device__ __forceinline__ uint4 put(const float (&x)[8]) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+      u[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
+  static __device__ __forceinline__ float most(const uint4& w) {
+    const __half2 m = __hmax2(__hmax2(pair(w.x), pair(w.y)), __hmax2(pair(w.z), pair(w.w)));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ __half2 pair(const uint32_t& u) { return *reinterpret_cast<const __half2*>(&u); }
 };
 
-__device__ __forceinline__ unsigned long long shfl64(unsigned long long x, int lane) { return __shfl_sync(0xffffffffu, x, lane); }
+// What a logit counts as.
+__device__ __forceinline__ float counted(float x) { return x == x ? x : -CUDART_INF_F; }
 
-// Lane k gets the (k + 1)-th largest of the warp's numbers.
-__device__ __forceinline__ unsigned long long sorted(unsigned long long x, int lane) {
+__device__ __forceinline__ unsigned long long warp_most(unsigned long long x) {
 #pragma unroll
-  for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      const unsigned long long y = __shfl_xor_sync(0xffffffffu, x, j);
-      const bool larger = ((lane & j) == 0) == ((lane & k) == 0 || k == 32);
-      x = larger ? (x > y ? x : y) : (x < y ? x : y);
-    }
+  for (int o = 16; o > 0; o >>= 1) {
+    const unsigned long long y = __shfl_xor_sync(0xffffffffu, x, o);
+    x = y > x ? y : x;
+  }
   return x;
+}
+
+// A number that K of the CTA's (one a thread) reach, and few more where warps' numbers are alike: what ceil(K / warps) of every warp do.
+// (Short, and not inlined: in a kernel of this size code that is not there yet takes longer than what it does.  The exact K-th largest, by the places of
+// the warps' sorted numbers among all, took 3000 cycles more.)
+__device__ __noinline__ float bound_of(float x, int K, float* meet) {
+  uint32_t left = key_of(x), top = 0;
+  for (int i = (K - 1) / kWarps; i >= 0; --i) {            // (equal ones go one by one, so that K are K)
+    top = __reduce_max_sync(0xffffffffu, left);
+    if ((int)(threadIdx.x % 32) == __ffs(__ballot_sync(0xffffffffu, left == top)) - 1) left = 0;
+  }
+  if (threadIdx.x % 32 == 0) meet[threadIdx.x / 32] = value_of(top);
+  __syncthreads();
+  float least = meet[0];
+#pragma unroll
+  for (int i = 1; i < kWarps; ++i) least = fminf(least, meet[i]);
+  return least;
+}
+
+// The same where they may differ: what K of one warp reach, or of two for K above 32.  meet: not that of the other.
+__device__ __noinline__ float bound_of_one(float x, int K, float* meet) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll 1
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll 1
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      const float y = __shfl_xor_sync(0xffffffffu, x, j);
+      x = ((lane & j) == 0) == ((lane & k) == 0 || k == 32) ? fmaxf(x, y) : fminf(x, y);
+    }
+  const float kth = __shfl_sync(0xffffffffu, x, min(K, 32) - 1);
+  if (lane == 0) meet[threadIdx.x / 32] = kth;
+  __syncthreads();
+  float most = -CUDART_INF_F;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) most = fmaxf(most, K <= 32 ? meet[i] : fminf(meet[i], meet[i ^ 1]));
+  return most;
 }
 
 // A continuation: its score's order, its beam, and its place in the beam (logit and token).
@@ -129,164 +207,241 @@ __device__ __forceinline__ int first_lane(const Next& x) {
   return __ffs(among) - 1;
 }
 
-template <class T, int P>
+// A row of logits.  Pieces are cut where addresses are multiples of 16.
+template <class T>
+struct Row {
+  static constexpr int N = Piece<T>::N, CHUNK = kThreads * P * N;
+  const T* in;
+  int vocab, lead;                        // elements between a boundary and the row's first
+  bool alive;                             // (a beam that is not has no order but the tokens')
+
+  __device__ __forceinline__ Row(const pbs_beam_select_t& a, int row)
+      : in((const T*)a.logits + row * a.logits_stride), vocab(a.vocab), lead((int)(((uintptr_t)in & 15) / sizeof(T))), alive(true) {}
+  __device__ __forceinline__ bool has(int v) const { return (unsigned)v < (unsigned)vocab; }
+  __device__ __forceinline__ float one(int v) const { return alive ? counted(Piece<T>::one(in + v)) : -CUDART_INF_F; }
+  // Token of element i of a thread's piece k of a chunk, the first and last whole pieces, and whether a chunk has no others.
+  __device__ __forceinline__ int token(int chunk, int k, int i, int thread) const { return chunk * CHUNK - lead + (k * kThreads + thread) * N + i; }
+  __device__ __forceinline__ int token(int chunk, int k, int i) const { return token(chunk, k, i, (int)threadIdx.x); }
+  __device__ __forceinline__ int whole0() const { return lead ? N - lead : 0; }
+  __device__ __forceinline__ int whole1() const { return (vocab + lead) / N * N - lead - N; }
+  __device__ __forceinline__ bool inner(int chunk) const { return chunk * CHUNK - lead >= whole0() && (chunk + 1) * CHUNK - lead - N <= whole1(); }
+
+  // Copies of this thread's pieces, or, of those that are an end of the row or beyond it, of some other; ends() puts those right.
+  __device__ __forceinline__ void copy(int chunk, uint4* to) const {
+    const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+    const bool plain = inner(chunk);
+    if (plain) {
+      const T* const from = in + token(chunk, 0, 0);
+#pragma unroll
+      for (int k = 0; k < P; ++k) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + k * kThreads * 16), "l"(from + k * kThreads * N) : "memory");
+      return;
+    }
+    const int w0 = whole0(), w1 = whole1();
+    if (w1 < w0) return;
+#pragma unroll
+    for (int k = 0; k < P; ++k)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + k * kThreads * 16), "l"(in + min(max(token(chunk, k, 0), w0), w1)) : "memory");
+  }
+  __device__ __forceinline__ void ends(int chunk, uint4 (&w)[P], int thread, bool all = false) const {
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      const int v = token(chunk, k, 0, thread);
+      if (!all && alive && v >= whole0() && v <= whole1()) continue;
+      float x[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = alive && has(v + i) ? Piece<T>::one(in + v + i) : -CUDART_INF_F;
+      w[k] = Piece<T>::put(x);
+    }
+  }
+};
+
+// A thread's logits so far: their maximum, and the sum of exp(logit - maximum).
+struct Sum {
+  float top = -kFltMax, sum = 0.f;
+
+  // Takes in P pieces (a NaN among them becomes -infinity) and returns the largest of their logits.
+  template <class T>
+  __device__ __forceinline__ float add(uint4 (&w)[P]) {
+    using E = Piece<T>;
+    constexpr int N = E::N;
+    float most = E::most(w[0]);
+#pragma unroll
+    for (int k = 1; k < P; ++k) most = fmaxf(most, E::most(w[k]));       // (a NaN gives way)
+    if (!(most >= -kFltMax)) most = -CUDART_INF_F;
+    const float higher = fmaxf(top, fminf(most, kFltMax)), shift = -higher * kLog2e;
+    const float2 scale = make_float2(kLog2e, kLog2e), by = make_float2(shift, shift);
+    float2 both = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      float x[N];
+      E::get(w[k], x);
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const float2 y = fma2(make_float2(x[i], x[i + 1]), scale, by);
+        both = add2(both, make_float2(exp2_fast(y.x), exp2_fast(y.y)));
+      }
+    }
+    float more = both.x + both.y;
+    more *= exp2_fast(-fmaf(higher, kLog2e, shift));       // (what the rounding of the shift has made of them all)
+    // Where logits are so large that this rounding matters, and where any is not a number or infinite: +infinity counts as the largest number.
+    if (__any_sync(0xffffffffu, !(more <= kFltMax) || fabsf(higher) > 1e5f)) {
+      more = 0.f;
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        float x[N];
+        E::get(w[k], x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          x[i] = counted(x[i]);
+          more += exp2_fast((fminf(x[i], kFltMax) - higher) * kLog2e);
+        }
+        w[k] = E::put(x);
+      }
+    }
+    sum = sum * exp2_fast((top - higher) * kLog2e) + more;
+    top = higher;
+    return most;
+  }
+};
+
+// The K largest of a segment one after the other, from memory: for the few that hold more large logits in few threads than there is room for.
+template <class T>
+__device__ __noinline__ void largest_one_by_one(const Row<T>& row, int chunk0, int chunk1, int K, unsigned long long* out, unsigned long long* meet) {
+  unsigned long long lower = ~0ull;
+  for (int r = 0; r < K; ++r) {
+    unsigned long long mine = 0;
+    for (int c = chunk0; c < chunk1; ++c)
+      for (int e = 0; e < P * Row<T>::N; ++e) {
+        const int v = row.token(c, e / Row<T>::N, e % Row<T>::N);
+        if (!row.has(v)) continue;
+        const unsigned long long o = ordered(row.one(v), v);
+        if (o < lower && o > mine) mine = o;
+      }
+    mine = warp_most(mine);
+    if (threadIdx.x % 32 == 0) meet[threadIdx.x / 32] = mine;
+    __syncthreads();
+    mine = meet[0];
+#pragma unroll
+    for (int i = 1; i < kWarps; ++i) mine = meet[i] > mine ? meet[i] : mine;
+    if (threadIdx.x == 0) out[r] = mine;
+    lower = mine;
+    __syncthreads();
+  }
+}
+
+template <class T>
 __global__ void __launch_bounds__(kThreads, kResident) beam_select_kernel(const __grid_constant__ BeamArgs p) {
   using E = Piece<T>;
+  using R = Row<T>;
   constexpr int N = E::N;
+  __shared__ __align__(16) uint4 ring[kStages][P][kThreads];
+  __shared__ unsigned long long list[kListed];
+  __shared__ unsigned long long found_score[kFound], found_place[kFound];
+  __shared__ uint32_t found_beam[kFound];
+  __shared__ Next heads[kWarps];
+  __shared__ float2 part[kWarps];
+  __shared__ float bounds[kWarps], bounds_of_one[kWarps];
+  __shared__ unsigned long long meet[kWarps];
+  __shared__ int listed, last;
+  __shared__ double norm[kMaxBeams];                       // of a beam: its score, less the logarithm of its sum
+  __shared__ float peak[kMaxBeams];
   const pbs_beam_select_t& a = p.a;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, K = a.keep;
-  const int row = blockIdx.x / p.slices, slice = blockIdx.x % p.slices, entry = row / a.beams;
-  __shared__ unsigned long long list[kListed];
-  __shared__ unsigned long long bounds[kWarps];
-  __shared__ float2 part[kWarps];
-  __shared__ int listed, last;
+  const int r = blockIdx.x / p.slices, entry = r / a.beams;
   {
-    const T* const in = (const T*)a.logits + row * a.logits_stride;
-    // pieces are cut where the row's addresses are multiples of 16: `lead` elements before its first
-    const int lead = (int)(((uintptr_t)in & 15) / sizeof(T));
-    const int first = (slice * P * kThreads + tid) * N - lead;             // vocabulary index of this thread's first piece
-    const float own = a.scores[entry * a.scores_stride + row % a.beams];
-    const bool alive = own > -CUDART_INF_F;                // (a beam that is not has no order but the tokens')
-    uint4 w[P];
+    const int chunk0 = (int)(blockIdx.x - r * p.slices) * p.share, chunk1 = min(p.chunks, chunk0 + p.share);
+    R row(a, r);
+    int ahead = chunk0, slot = 0;
+    auto issue = [&] {
+      if (ahead < chunk1) row.copy(ahead, &ring[(ahead - chunk0) % kStages][0][tid]);
+      ++ahead;
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
 #pragma unroll
-    for (int k = 0; k < P; ++k) {
-      const int v = first + k * kThreads * N;
-      w[k] = make_uint4(E::kNever, E::kNever, E::kNever, E::kNever);
-      if (!alive) continue;
-      if (v >= 0 && v + N <= a.vocab) {
-        w[k] = *reinterpret_cast<const uint4*>(in + v);
-      } else if (v + N > 0 && v < a.vocab) {
-        T* const x = reinterpret_cast<T*>(&w[k]);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (v + i >= 0 && v + i < a.vocab) x[i] = in[v + i];
-      }
-    }
+    for (int i = 0; i < kStages - 1; ++i) issue();
+    row.alive = a.scores[entry * a.scores_stride + r % a.beams] > -CUDART_INF_F;
     if (tid == 0) listed = 0;
-    // this thread's largest, the first of equals, and its sum of exponentials
-    float most = -CUDART_INF_F;
-    int at = -1;
+    Sum sum;
+    float best[3] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};         // of this thread's chunks, and where the first two are
+    int where[2] = {-1, -1};
+    for (int c = chunk0; c < chunk1; ++c) {
+      uint4 w[P];
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
 #pragma unroll
-    for (int k = 0; k < P; ++k) {
-      float x[N], m;
-      E::get(w[k], x);
-      m = x[0];
-#pragma unroll
-      for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
-      if (m > most) most = m;
+      for (int k = 0; k < P; ++k) w[k] = ring[slot][k][tid];
+      slot = (slot + 1) % kStages;
+      issue();                                             // (into the place that was read before)
+      if (!__all_sync(0xffffffffu, row.alive && row.inner(c))) row.ends(c, w, tid);
+      const float most = sum.add<T>(w);
+      const bool first = most > best[0], second = most > best[1];
+      best[2] = second ? best[1] : fmaxf(best[2], most);
+      best[1] = first ? best[0] : second ? most : best[1];
+      where[1] = first ? where[0] : second ? c : where[1];
+      best[0] = first ? most : best[0];
+      where[0] = first ? c : where[0];
     }
-    const float top = fminf(fmaxf(most, -kFltMax), kFltMax);
-    float sum = 0.f;
+    // K logits reach the bound.  Where there are no K to reach anything, all that is not -infinity does, and the first K tokens of the segment,
+    // enough of which are -infinity to fill up.
+    float bound = bound_of(best[0], K, bounds);
+    if (bound == -CUDART_INF_F) bound = bound_of_one(best[0], K, bounds_of_one);            // (a segment of few tokens, or most of them banned)
+    const int filled = bound == -CUDART_INF_F ? max(chunk0 * R::CHUNK - row.lead, 0) + K : -1;
+    auto enlist = [&](int c, int thread) {                 // a thread's pieces of a chunk
+      const bool plain = row.alive && row.inner(c);
+      uint4 w[P];
 #pragma unroll
-    for (int k = 0; k < P; ++k) {
-      float x[N];
-      E::get(w[k], x);
-#pragma unroll
-      for (int i = 0; i < N; ++i) sum += exp2_fast((x[i] - top) * kLog2e);
-    }
-    if (!(sum <= kFltMax)) {                               // a NaN counts as -infinity, +infinity as the largest number
-      sum = 0.f;
-#pragma unroll
-      for (int k = 0; k < P; ++k) {
-        T* const raw = reinterpret_cast<T*>(&w[k]);
-        float x[N];
-        E::get(w[k], x);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          if (x[i] != x[i]) raw[i] = T(-CUDART_INF_F);
-          sum += exp2_fast((fminf(fmaxf(x[i], -kFltMax), kFltMax) - top) * kLog2e);
-        }
-      }
-    }
-    unsigned long long best = 0;
-#pragma unroll
-    for (int k = P - 1; k >= 0; --k) {
-      float x[N];
-      E::get(w[k], x);
-#pragma unroll
-      for (int i = N - 1; i >= 0; --i) {
-        const int v = first + k * kThreads * N + i;
-        if (x[i] == most && v >= 0 && v < a.vocab) at = v;
-      }
-    }
-    if (at >= 0) best = ordered(most, at);
-    // the slice's maximum and sum
-    const float wide = warp_max(top);
-    sum = warp_sum(sum * exp2_fast((top - wide) * kLog2e));
-    if (lane == 0) part[warp] = make_float2(wide, sum);
-    // bound: K of a warp's lanes, or of two warps', hold a logit that reaches it
-    const unsigned long long order = sorted(best, lane), kth = shfl64(order, min(K, 32) - 1);
-    if (lane == 0) bounds[warp] = kth;
-    __syncthreads();
-    unsigned long long bound = 0;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      const unsigned long long b = K <= 32 ? bounds[i] : bounds[i] < bounds[i ^ 1] ? bounds[i] : bounds[i ^ 1];
-      bound = b > bound ? b : bound;
-    }
-    const float least = bound ? value_of((uint32_t)(bound >> 32)) : -CUDART_INF_F;
-    if (best >= bound && best != 0) {
+      for (int k = 0; k < P; ++k) w[k] = plain ? __ldcg(reinterpret_cast<const uint4*>(row.in + row.token(c, k, 0, thread))) : make_uint4(0, 0, 0, 0);
+      if (!plain) row.ends(c, w, thread, true);
+      uint32_t reach = 0;
 #pragma unroll
       for (int k = 0; k < P; ++k) {
         float x[N];
         E::get(w[k], x);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const int v = first + k * kThreads * N + i;
-          if (!(x[i] >= least) || v < 0 || v >= a.vocab) continue;
-          const unsigned long long o = ordered(x[i], v);
-          if (o < bound) continue;
-          const int n = atomicAdd(&listed, 1);
-          if (n < kListed) list[n] = o;
+          const int v = row.token(c, k, i, thread);
+          if ((x[i] >= bound && x[i] > -CUDART_INF_F) || (v < filled && c == chunk0)) reach |= row.has(v) ? 1u << (k * N + i) : 0;
         }
       }
-    }
-    __syncthreads();
-    unsigned long long* const out = p.lists + (int64_t)blockIdx.x * K;
-    if (tid == 0) {
-      float2 all = part[0];
-#pragma unroll
-      for (int i = 1; i < kWarps; ++i) {
-        const float m = fmaxf(all.x, part[i].x);
-        all = make_float2(m, all.y * exp2_fast((all.x - m) * kLog2e) + part[i].y * exp2_fast((part[i].x - m) * kLog2e));
+      for (; reach; reach &= reach - 1) {
+        const int bit = __ffs(reach) - 1, v = row.token(c, bit / N, bit % N, thread), n = atomicAdd(&listed, 1);
+        if (n < kListed) list[n] = ordered(row.one(v), v);
       }
-      p.sums[blockIdx.x] = all;
+    };
+    // (in three or more chunks of a thread: rarely, and then the warp looks through all of them)
+    const uint32_t everywhere = __ballot_sync(0xffffffffu, best[2] >= bound && best[2] > -CUDART_INF_F);
+    for (uint32_t left = everywhere; left; left &= left - 1)
+      for (int c = chunk0 + lane; c < chunk1; c += 32) enlist(c, warp * 32 + __ffs(left) - 1);
+    if (!(everywhere >> lane & 1)) {
+      const bool fills = row.token(chunk0, 0, 0) < filled;
+      if (fills) enlist(chunk0, tid);
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        const int c = i == 0 ? where[0] : where[1];
+        if ((i == 0 ? best[0] : best[1]) >= bound && c >= 0 && !(fills && c == chunk0)) enlist(c, tid);
+      }
     }
+    // the segment's maximum and sum, and its list
+    const float wide = warp_max(sum.top), scaled = warp_sum(sum.sum * exp2_fast((sum.top - wide) * kLog2e));
+    if (lane == 0) part[warp] = make_float2(wide, scaled);
+    __syncthreads();
     const int n = listed;
+    unsigned long long* const out = p.lists + (int64_t)blockIdx.x * K;
     if (n <= kListed) {
       for (int i = tid; i < n; i += kThreads) {
         const unsigned long long mine = list[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += list[j] > mine;
-        if (rank < K) out[rank] = mine;
+        int at = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) at += list[j] > mine;
+        if (at < K) out[at] = mine;
       }
-      for (int i = n + tid; i < K; i += kThreads) out[i] = 0;              // (a slice of fewer tokens)
-    } else {                                               // very many in few lanes: the largest, the one after it, ...
-      unsigned long long lower = ~0ull;
-      for (int r = 0; r < K; ++r) {
-        unsigned long long mine = 0;
-#pragma unroll
-        for (int k = 0; k < P; ++k) {
-          float x[N];
-          E::get(w[k], x);
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const int v = first + k * kThreads * N + i;
-            if (v < 0 || v >= a.vocab) continue;
-            const unsigned long long o = ordered(x[i], v);
-            if (o < lower && o > mine) mine = o;
-          }
-        }
-        mine = shfl64(sorted(mine, lane), 0);
-        if (lane == 0) list[warp] = mine;
-        __syncthreads();
-        mine = list[0];
-#pragma unroll
-        for (int i = 1; i < kWarps; ++i) mine = list[i] > mine ? list[i] : mine;
-        if (tid == 0) out[r] = mine;
-        lower = mine;
-        __syncthreads();
-      }
+      for (int i = n + tid; i < K; i += kThreads) out[i] = 0;              // (a segment of fewer tokens)
+    } else {
+      largest_one_by_one(row, chunk0, chunk1, K, out, meet);
+    }
+    if (warp == 1) {
+      const float2 x = lane < kWarps ? part[lane] : make_float2(-kFltMax, 0.f);
+      const float m = warp_max(x.x), total = warp_sum(x.y * exp2_fast((x.x - m) * kLog2e));
+      if (lane == 0) p.sums[blockIdx.x] = make_float2(m, total);
     }
   }
   __syncthreads();
@@ -297,128 +452,157 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_select_kernel(const 
       p.counters[entry] = 0;                               // for the next call
       __threadfence();
     }
+    listed = 0;
   }
   __syncthreads();
   if (!last) return;
 
-  // the entry's rows and slices meet: lists of one entry are neighbours
-  __shared__ double norm[kMaxBeams];                       // of a beam: its score, less the logarithm of its sum
-  __shared__ float peak[kMaxBeams];
-  __shared__ Next heads[kWarps];
-  const int rows = a.beams, lists = rows * p.slices;
-  const int64_t base = (int64_t)entry * lists;
-  for (int r = warp; r < rows; r += kWarps) {
-    float m = -kFltMax;
-    for (int s = lane; s < p.slices; s += 32) m = fmaxf(m, __ldcg(&p.sums[base + r * p.slices + s]).x);
-    m = warp_max(m);
-    double sum = 0.0;
-    for (int s = lane; s < p.slices; s += 32) {
-      const float2 x = __ldcg(&p.sums[base + r * p.slices + s]);
-      sum += (double)x.y * (double)exp2_fast((x.x - m) * kLog2e);
-    }
+  // The entry's segments meet.  A thread looks through a segment's sorted list, or several, or every g-th place of one where they are few.
+  const int rows = a.beams, lists = rows * p.slices, number0 = entry * lists;
+  const int g = lists >= kThreads ? 1 : min(K, kThreads / lists), together = kThreads / g;      // threads of a list; lists at a time
+  const int list0 = tid / g < together ? tid / g : lists, place0 = tid % g;
+  auto place_of = [&](int l, int i) { return __ldcg(p.lists + (int64_t)(number0 + l) * K + i); };
+  const unsigned long long early = list0 < lists ? place_of(list0, place0) : 0;          // (on its way while the sums are added up)
+  const int share = rows < kWarps ? kWarps / rows : 1;   // warps of a row, which all do the same
+  constexpr int A = 4;                                   // loads under way
+  for (int i = warp / share; i < rows; i += kWarps / share) {
+    const float2* const sums = p.sums + number0 + i * p.slices;
+    float2 x[A];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) {
-      const float own = a.scores[entry * a.scores_stride + r];
-      norm[r] = own > -CUDART_INF_F ? (double)own - log(sum) : -CUDART_INF;
-      peak[r] = m;
+    for (int u = 0; u < A; ++u) x[u] = lane + u * 32 < p.slices ? __ldcg(sums + lane + u * 32) : make_float2(-kFltMax, 0.f);
+    float m = -kFltMax, total = 0.f;
+#pragma unroll 1
+    for (int at = lane;;) {
+      float wide = m;
+#pragma unroll
+      for (int u = 0; u < A; ++u) wide = fmaxf(wide, x[u].x);
+      total *= exp2_fast((m - wide) * kLog2e);
+#pragma unroll
+      for (int u = 0; u < A; ++u) total += x[u].y * exp2_fast((x[u].x - wide) * kLog2e);
+      m = wide;
+      at += A * 32;
+      if (at - lane >= p.slices) break;
+#pragma unroll
+      for (int u = 0; u < A; ++u) x[u] = at + u * 32 < p.slices ? __ldcg(sums + at + u * 32) : make_float2(-kFltMax, 0.f);
+    }
+    const float top = warp_max(m);
+    total = warp_sum(total * exp2_fast((m - top) * kLog2e));
+    if (lane == 0) {                                     // (warps that share a row write the same)
+      const float s = a.scores[entry * a.scores_stride + i];
+      // the logarithm of the sum's mantissa, 0.7 to 1.4, so that its rounding is one of a small number
+      const int up = (int)(__float_as_uint(total * 1.41421356f) >> 23) - 127;
+      const float part_of = logf(total * __uint_as_float((uint32_t)(127 - up) << 23));
+      norm[i] = s > -CUDART_INF_F ? (double)s - (0.69314718055994531 * up + (double)part_of) : -CUDART_INF;
+      peak[i] = top;
     }
   }
   __syncthreads();
-  auto next = [&](int l, int i) {                          // entry i of list l
-    Next x{0, 0, 0xffffffffu};
-    if (i < K) x.place = __ldcg(p.lists + (base + l) * K + i);
-    if (x.place) {
-      x.beam = l / p.slices;
-      const float v = value_of((uint32_t)(x.place >> 32));
-      // (the largest number stands for infinity)
-      const double score = v == -CUDART_INF_F ? -CUDART_INF : norm[x.beam] + ((double)fminf(v, kFltMax) - (double)peak[x.beam]);
-      x.score = key_of(score);
-    }
-    return x;
+  auto score_of = [&](int i, uint32_t key) {             // in 64 bits
+    const float v = value_of(key);
+    return v == -CUDART_INF_F ? -CUDART_INF : norm[i] + ((double)fminf(v, kFltMax) - (double)peak[i]);
   };
-  // a thread's lists l = tid, tid + kThreads, ...: how far each has been taken, in shared memory
-  uint8_t* const taken = reinterpret_cast<uint8_t*>(list);
-  const bool many = lists > kListed * 8;                   // (more lists than there is room for are looked through anew each time)
-  if (!many)
-    for (int l = tid; l < lists; l += kThreads) taken[l] = 0;
-  Next mine{0, 0, 0xffffffffu}, floor_{~0ull, ~0ull, 0};
-  int mine_list = -1;
-  auto look = [&] {                                        // the best of this thread's lists
-    mine = Next{0, 0, 0xffffffffu};
-    for (int l = tid; l < lists; l += kThreads) {
-      Next x{0, 0, 0xffffffffu};
-      if (!many) {
-        x = next(l, taken[l]);
-      } else {
-        for (int i = 0; i < K; ++i) {
-          x = next(l, i);
-          if (!x.place || before(floor_, x)) break;
+  auto every = [&](auto&& take) {                        // this thread's places, as continuations, list by list while take() says so
+    for (int l = list0; l < lists; l += together) {
+      const int i = l / p.slices;
+      for (int at = place0; at < K; at += g) {
+        const unsigned long long place = l == list0 && at == place0 ? early : place_of(l, at);
+        if (!place || !take(Next{key_of(score_of(i, (uint32_t)(place >> 32))), place, (uint32_t)i})) break;
+      }
+    }
+  };
+  // (bounds are of scores rounded to 32 bits, an order that the rounding keeps)
+  float leads = -CUDART_INF_F;
+  every([&](const Next& x) {
+    leads = fmaxf(leads, (float)value_of(x.score));
+    return false;
+  });
+  float reached = fmaxf(bound_of(leads, K, bounds), bound_of_one(leads, K, bounds_of_one));
+  int count;
+  for (int i = 0;; ++i) {
+    if (leads >= reached && leads > -CUDART_INF_F)
+      every([&](const Next& x) {
+        const float s = (float)value_of(x.score);
+        if (s < reached || s == -CUDART_INF_F) return false;
+        const int at = atomicAdd(&listed, 1);
+        if (at < kFound) {
+          found_score[at] = x.score;
+          found_place[at] = x.place;
+          found_beam[at] = x.beam;
         }
-      }
-      if (x.place && (!mine.place || before(x, mine))) {
-        mine = x;
-        mine_list = l;
-      }
-    }
-  };
-  auto head = [&] {                                        // the best of the warp's
-    const int l = first_lane(mine);
-    if (lane == l) heads[warp] = mine;
-  };
-  look();
-  head();
-  __syncthreads();
-  for (int r = 0; r < K; ++r) {
-    int w = 0;
-    Next x = heads[0];
-#pragma unroll
-    for (int i = 1; i < kWarps; ++i)
-      if (before(heads[i], x)) {
-        x = heads[i];
-        w = i;
-      }
+        return true;
+      });
     __syncthreads();
-    if (tid == 0) {
-      const int64_t o = (int64_t)entry * K + r;
-      a.out_scores[o] = (float)value_of(x.score);
-      a.out_beams[o] = (int)x.beam;
-      a.out_tokens[o] = (long long)(uint32_t)~(uint32_t)x.place;
+    count = listed;
+    if (count <= kFound || i == 2) break;
+    // too many (a beam far ahead of the others, whose best lie in few hands): the K-th of those that found room is a better bound
+    for (int e = tid; e < kFound; e += kThreads) {
+      const unsigned long long mine = found_score[e];
+      int at = 0;
+#pragma unroll 4
+      for (int j = 0; j < kFound; ++j) at += found_score[j] > mine || (found_score[j] == mine && j < e);
+      if (at == K - 1) bounds[0] = (float)value_of(mine);
     }
-    floor_ = x;
-    if (warp == w) {
-      if (mine.place == x.place && mine.beam == x.beam && mine_list >= 0) {
-        if (!many) ++taken[mine_list];
-        look();
-      }
-      __syncwarp();
-      head();
-    }
+    __syncthreads();
+    reached = bounds[0];
+    if (tid == 0) listed = 0;
     __syncthreads();
   }
-}
-
-template <class T>
-constexpr int elements() { return 16 / (int)sizeof(T); }
-
-// Pieces of a thread (a power of two) and slices of a row: as many slices as are resident at a time, though no smaller than a piece a
-// thread, and as many more as it takes to keep them in registers.
-template <class T>
-void cut(const pbs_beam_select_t& a, int* slices, int* pieces) {
-  const int64_t per = (int64_t)kThreads * elements<T>(), total = ((int64_t)a.vocab + elements<T>() - 1 + per - 1) / per;
-  const int64_t rows = (int64_t)a.batch * a.beams, fit = (int64_t)kResident * device_sms() / rows;
-  int64_t p = (total + (fit > 1 ? fit : 1) - 1) / (fit > 1 ? fit : 1);
-  *pieces = p <= 1 ? 1 : p <= 2 ? 2 : p <= 4 ? 4 : kMost;
-  *slices = (int)((total + *pieces - 1) / *pieces);
+  auto put = [&](int at, const Next& x) {
+    const int64_t o = (int64_t)entry * K + at;
+    a.out_scores[o] = (float)value_of(x.score);
+    a.out_beams[o] = (int)x.beam;
+    a.out_tokens[o] = (long long)(uint32_t)~(uint32_t)x.place;
+  };
+  if (count >= K && count <= kFound) {
+    for (int i = tid; i < count; i += kThreads) {
+      const Next x{found_score[i], found_place[i], found_beam[i]};
+      int at = 0;
+#pragma unroll 4
+      for (int j = 0; j < count; ++j) at += found_score[j] > x.score;
+      for (int j = 0; j < count; ++j)                    // (equal scores, which a short loop is enough to find)
+        if (found_score[j] == x.score && j != i) at += before(Next{x.score, found_place[j], found_beam[j]}, x);
+      if (at < K) put(at, x);
+    }
+  } else {
+    // too few that are not -infinity, or too many that are equal: the first, the one after it, ...
+    Next passed{~0ull, ~0ull, 0}, next{0, 0, 0xffffffffu};
+    bool look = true;
+    for (int i = 0; i < K; ++i) {
+      if (look) {
+        next = Next{0, 0, 0xffffffffu};
+        every([&](const Next& x) {
+          if (!before(passed, x)) return true;
+          if (!next.score || before(x, next)) next = x;
+          return false;                                  // (the rest of the list comes after it)
+        });
+      }
+      const int from = first_lane(next);
+      if (lane == from) heads[warp] = next;
+      __syncthreads();
+      passed = heads[0];
+#pragma unroll
+      for (int u = 1; u < kWarps; ++u)
+        if (before(heads[u], passed)) passed = heads[u];
+      if (tid == 0) put(i, passed);
+      look = next.place == passed.place && next.beam == passed.beam;
+      __syncthreads();
+    }
+  }
 }
 
 template <class T>
 int launch(const pbs_beam_select_t& a, void* workspace, int64_t* bytes, cudaStream_t st) {
+  constexpr int N = Piece<T>::N, CHUNK = Row<T>::CHUNK;
   BeamArgs p{};
   p.a = a;
-  cut<T>(a, &p.slices, &p.pieces);
-  const int64_t ctas = (int64_t)a.batch * a.beams * p.slices;
-  if (ctas > INT_MAX) { set_error("beam selection: %lld rows of %d", (long long)a.batch * a.beams, a.vocab); return PBS_ERR_SHAPE; }
+  p.chunks = (int)(((int64_t)a.vocab + N - 1 + CHUNK - 1) / CHUNK);        // (a row may start inside a piece)
+  // Segments: so many that all are resident at a time; where there are more rows than that, so short that the CTAs that come last are a small part.
+  const int64_t rows = (int64_t)a.batch * a.beams, resident = (int64_t)kResident * device_sms(), whole = 4 * resident / rows;
+  const int64_t slices = rows <= resident ? resident / rows : whole > 1 ? whole : 1;
+  p.share = (int)((p.chunks + slices - 1) / slices);
+  p.slices = (p.chunks + p.share - 1) / p.share;
+  const int64_t ctas = rows * p.slices;
+  if (ctas > INT_MAX || (int64_t)p.chunks * CHUNK > INT_MAX) { set_error("beam selection: %lld rows of %d", (long long)rows, a.vocab); return PBS_ERR_SHAPE; }
   if (bytes) {
     *bytes = PBS_PAGED_COUNTER_BYTES + ctas * (8 + 8 * (int64_t)a.keep);
     return PBS_OK;
@@ -426,13 +610,7 @@ int launch(const pbs_beam_select_t& a, void* workspace, int64_t* bytes, cudaStre
   p.counters = (unsigned*)workspace;
   p.sums = (float2*)((uint8_t*)workspace + PBS_PAGED_COUNTER_BYTES);
   p.lists = (unsigned long long*)(p.sums + ctas);
-  const dim3 grid((unsigned)ctas);
-  switch (p.pieces) {
-    case 1: beam_select_kernel<T, 1><<<grid, kThreads, 0, st>>>(p); break;
-    case 2: beam_select_kernel<T, 2><<<grid, kThreads, 0, st>>>(p); break;
-    case 4: beam_select_kernel<T, 4><<<grid, kThreads, 0, st>>>(p); break;
-    default: beam_select_kernel<T, kMost><<<grid, kThreads, 0, st>>>(p); break;
-  }
+  beam_select_kernel<T><<<(unsigned)ctas, kThreads, 0, st>>>(p);
   PBS_CUDA_CHECK_LAUNCH("beam_select_kernel");
   return PBS_OK;
 }

@@ -28,7 +28,7 @@ struct ReorderArgs {
   int64_t beams_stride;
   int n;                                  // rows of a group
   int layers, layers_cta;
-  int row_pieces, row_words;              // of a token's row: 16-byte pieces; 4-byte words of params (4 bits)
+  int piece_shift, word_shift;            // of a token's row, as powers of two: 16-byte pieces; 4-byte words of params (4 bits)
   Pools pools[kLayers];
 };
 
@@ -37,26 +37,31 @@ struct Move {
   int row, parent, to, from, fill, full;  // rows of the batch; pages under way (-1: nothing to copy) and their tokens; full pages
 };
 
-// Brings units `u` of a page, for all moves, from the parents' pages: F(layer, unit) is where a unit lies in page 0, UNIT its type.
-template <class UNIT, int MAXN, int U, class F>
+// Brings units of a page, for all moves, from the parents' pages: per_layer of them at most in each of `layers`, units[m] of move m.  at(layer, u) is
+// where unit u lies in page 0.  M: the most moves; U units are under way in a thread.
+template <class UNIT, int M, int U, class F>
 __device__ __forceinline__ void copy(const Move* moves, int count, int layers, int per_layer, int64_t page_bytes, F at, const int* units) {
-  for (int i0 = threadIdx.x; i0 < layers * per_layer; i0 += U * kThreads) {
-    UNIT v[U][MAXN];
+  const float inverse = 1.f / (float)per_layer;
+  const int total = layers * per_layer;
+  for (int i0 = threadIdx.x; i0 < total; i0 += U * kThreads) {
+    UNIT v[U][M];
     uint8_t* where[U];
     int unit[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * kThreads, layer = i / per_layer;
-      unit[u] = i < layers * per_layer ? i - layer * per_layer : INT_MAX;
-      where[u] = unit[u] == INT_MAX ? nullptr : at(layer, unit[u]);
+      const int i = i0 + u * kThreads;
+      int layer = (int)((float)i * inverse);               // (of up to 2^21 units: off by one at most)
+      layer += (i >= (layer + 1) * per_layer) - (i < layer * per_layer);
+      unit[u] = i < total ? i - layer * per_layer : INT_MAX;
+      where[u] = i < total ? at(layer, unit[u]) : nullptr;
 #pragma unroll
-      for (int m = 0; m < MAXN; ++m)
+      for (int m = 0; m < M; ++m)
         if (m < count && unit[u] < units[m]) v[u][m] = *reinterpret_cast<const UNIT*>(where[u] + moves[m].from * page_bytes);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int m = 0; m < MAXN; ++m)
+      for (int m = 0; m < M; ++m)
         if (m < count && unit[u] < units[m]) *reinterpret_cast<UNIT*>(where[u] + moves[m].to * page_bytes) = v[u][m];
   }
 }
@@ -88,8 +93,8 @@ __global__ void __launch_bounds__(kThreads) paged_reorder_kernel(const __grid_co
     }
     const uint32_t all = __ballot_sync(0xffffffffu, moves_);
     const int at = __popc(all & ((1u << tid) - 1));
-    const int n_pieces = moves_ && m.fill && m.to != m.from ? m.fill * p.row_pieces : 0;
-    const int n_words = n_pieces == 0 || c.bits == 16 ? 0 : c.bits == 8 ? (m.fill + c.block_size - 1) >> p.a.block_shift : m.fill * p.row_words;
+    const int n_pieces = moves_ && m.fill && m.to != m.from ? m.fill << p.piece_shift : 0;
+    const int n_words = n_pieces == 0 || c.bits == 16 ? 0 : c.bits == 8 ? (m.fill + c.block_size - 1) >> p.a.block_shift : m.fill << p.word_shift;
     if (moves_) {
       moves[at] = m;
       pieces[at] = n_pieces;
@@ -122,16 +127,20 @@ __global__ void __launch_bounds__(kThreads) paged_reorder_kernel(const __grid_co
   const int64_t(&st)[3] = is_v ? c.v_strides : c.k_strides;
   const int64_t(&pst)[3] = is_v ? c.v_params_strides : c.k_params_strides;
   const Pools* const pools = p.pools + layer0;
-  constexpr int U = MAXN <= 4 ? 4 : MAXN <= 8 ? 2 : 1;
-  if (most_pieces)
-    copy<uint4, MAXN, U>(moves, n, layers, most_pieces, st[0] * es, [&](int layer, int u) {
-      return (is_v ? pools[layer].v : pools[layer].k) + (head * st[1] + u / p.row_pieces * st[2]) * es + u % p.row_pieces * 16;
-    }, pieces);
+  if (most_pieces) {
+    auto at = [&](int layer, int u) {
+      return (is_v ? pools[layer].v : pools[layer].k) + (head * st[1] + (u >> p.piece_shift) * st[2]) * es + (u & ((1 << p.piece_shift) - 1)) * 16;
+    };
+    const int64_t page = st[0] * es;
+    // eight pieces under way in a thread, however many rows they are of
+    if (n <= 2) copy<uint4, 2, 4>(moves, n, layers, most_pieces, page, at, pieces);
+    else if (n <= 4) copy<uint4, 4, 2>(moves, n, layers, most_pieces, page, at, pieces);
+    else copy<uint4, MAXN, 1>(moves, n, layers, most_pieces, page, at, pieces);
+  }
   const int ps = c.bits == 8 ? 4 : 2;
   if (most_words)
     copy<uint32_t, MAXN, 1>(moves, n, layers, most_words, pst[0] * ps, [&](int layer, int u) {
-      const int slot = u / p.row_words;
-      return (is_v ? pools[layer].v_params : pools[layer].k_params) + (head * pst[1] + slot * pst[2]) * ps + (u - slot * p.row_words) * 4;
+      return (is_v ? pools[layer].v_params : pools[layer].k_params) + (head * pst[1] + (u >> p.word_shift) * pst[2]) * ps + (u & ((1 << p.word_shift) - 1)) * 4;
     }, words);
 }
 
@@ -152,8 +161,8 @@ int launch_paged_reorder(const PagedArgs& a, const pbs_paged_cache_t* const* cac
   p.beams = beams;
   p.beams_stride = beams_stride;
   p.n = n;
-  p.row_pieces = a.c.head_dim * a.c.bits / 128;
-  p.row_words = a.c.bits == 4 ? a.c.head_dim / a.c.group_size : 1;
+  while (128 << p.piece_shift < a.c.head_dim * a.c.bits) ++p.piece_shift;
+  while (a.c.bits == 4 && a.c.group_size << p.word_shift < a.c.head_dim) ++p.word_shift;
   const int groups = a.b.batch / n;
   for (int l0 = 0; l0 < layers; l0 += kLayers) {
     p.layers = layers - l0 < kLayers ? layers - l0 : kLayers;
@@ -165,7 +174,7 @@ int launch_paged_reorder(const PagedArgs& a, const pbs_paged_cache_t* const* cac
     const int64_t ctas = (int64_t)p.layers * groups * 2 * a.c.kv_heads, fill = (int64_t)device_sms() * 8;
     p.layers_cta = (int)((ctas + fill - 1) / fill);
     if (p.layers_cta > p.layers) p.layers_cta = p.layers;
-    PBS_TRY(n <= 4 ? launch<4>(p, groups, st) : n <= 8 ? launch<8>(p, groups, st) : n <= 16 ? launch<16>(p, groups, st) : launch<kMaxBeams>(p, groups, st));
+    PBS_TRY(n <= 8 ? launch<8>(p, groups, st) : n <= 16 ? launch<16>(p, groups, st) : launch<kMaxBeams>(p, groups, st));
     p.table = nullptr;                                     // (its full pages have been seen to)
   }
   return PBS_OK;
