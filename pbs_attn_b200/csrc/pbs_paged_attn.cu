@@ -147,13 +147,14 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
-// Signed bytes 0 and 2, or 1 and 3, of a word as two halves: 1024 + (byte + 128) by its bits, less 1152, which is exact.
-__device__ __forceinline__ uint32_t bytes02(uint32_t w) {
-  const uint32_t h = (w & 0x00ff00ffu) ^ 0x64806480u, b = 0x64806480u;
-  const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&d);
+// Integers: 16 x 32 signed bytes times 32 x 8.
+__device__ __forceinline__ void mma_bytes(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t bytes13(uint32_t w) { return bytes02(w >> 8); }
+// Signed bytes 0 and 2, or 1 and 3, of a word, plus 128 and times 2^-24: fp16 numbers by their bits.
+__device__ __forceinline__ uint32_t bytes02(uint32_t w) { return (w & 0x00ff00ffu) ^ 0x00800080u; }
+__device__ __forceinline__ uint32_t bytes13(uint32_t w) { return __byte_perm(w, 0, 0x4341) ^ 0x00800080u; }
 // Step (low half) and minimum (high half) of a word of params.
 template <class T>
 __device__ __forceinline__ float step_of(uint32_t w) {
@@ -236,6 +237,7 @@ struct Warp {
   static constexpr int kRoom = C::BITS == 16 && C::DT == PBS_BF16 ? 40 : 0;        // powers of 2 that weights are kept smaller by
   float o[C::D / 16][C::NT][4];
   float om[C::BITS == 4 ? C::NG : 1][C::NT][2];                    // sums of p * lo, this lane's tokens
+  [[maybe_unused]] float o128[C::BITS == 8 ? C::NT : 1][4];        // 8 bits: what o has to be less
   float l[C::NT][2], ref[C::NT][2];
   const uint4* qf;                                                 // this lane's query fragments, C::NT * 32 apart from chunk to chunk
   const float* qsum;
@@ -248,6 +250,12 @@ struct Warp {
     if constexpr (C::SHIFT > 0) {
       for (int i = lane; i < C::NG * C::COLS; i += 32) shift[i] = 0.f;
       __syncwarp();
+    }
+    if constexpr (C::BITS == 8) {
+#pragma unroll
+      for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o128[n][c] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < C::D / 16; ++i)
@@ -290,24 +298,34 @@ struct Warp {
         }
       }
     } else if constexpr (C::BITS == 8) {
+      int high[C::MT][C::NT][4], low[C::MT][C::NT][4];             // with the queries' high and low bytes
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) high[m][n][c] = low[m][n][c] = 0;
 #pragma unroll
       for (int j = 0; j < C::CH / 2; ++j) {
         uint32_t r[C::MT][4];
 #pragma unroll
         for (int m = 0; m < C::MT; ++m) load_matrices(r[m], k_at + piece<C>(16 * m + row, 2 * j + half));
 #pragma unroll
-        for (int jj = 0; jj < 2; ++jj)
+        for (int n = 0; n < C::NT; ++n) {
+          const uint4 q = qf[(j * C::NT + n) * 32];
 #pragma unroll
           for (int m = 0; m < C::MT; ++m) {
-            const uint32_t x = r[m][2 * jj], y = r[m][2 * jj + 1];
-            const uint32_t a0 = bytes02(x), a1 = bytes02(y), a2 = bytes13(x), a3 = bytes13(y);
-#pragma unroll
-            for (int n = 0; n < C::NT; ++n) {
-              const uint4 q = qf[(j * C::NT + n) * 32];
-              mma<PBS_FP16>(tot[m][n], a0, a1, a2, a3, jj ? q.z : q.x, jj ? q.w : q.y);
-            }
+            mma_bytes(high[m][n], r[m], q.x, q.y);
+            mma_bytes(low[m][n], r[m], q.z, q.w);
           }
+        }
       }
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tot[m][n][c] = (float)(high[m][n][c] * 256 + low[m][n][c]);
     } else {
       uint32_t kp[C::MT][2][C::NG];
       const uint8_t* params = stage + 2 * C::TILE * C::ROW;
@@ -410,6 +428,7 @@ struct Warp {
         if (ref[n][c] != old && old > -CUDART_INF_F) {             // (before the first reference nothing has been summed up)
           const float keep = factor_of<C>(old - ref[n][c]);
           l[n][c] = scaled<C>(l[n][c], keep);
+          if constexpr (C::BITS == 8) o128[n][c] = scaled<C>(o128[n][c], keep);
 #pragma unroll
           for (int i = 0; i < C::D / 16; ++i) {
             o[i][n][c] = scaled<C>(o[i][n][c], keep);
@@ -447,6 +466,21 @@ struct Warp {
   }
 
   __device__ __forceinline__ void move_sums() {
+    if constexpr (C::BITS == 8) {
+#pragma unroll
+      for (int n = 0; n < C::NT; ++n) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int i = 0; i < C::D / 16; ++i) {
+            o[i][n][c] -= o128[n][c];
+            o[i][n][c + 2] -= o128[n][c];
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o128[n][c] = 0.f;
+      }
+    }
     if constexpr (C::SHIFT > 0) {
 #pragma unroll
       for (int g = 0; g < C::NG; ++g)
@@ -651,6 +685,9 @@ struct Warp {
             for (int n = 0; n < C::NT; ++n) mma<PBS_FP16>(o[2 * j2 + jj][n], a0, a1, a2, a3, b[n][0], b[n][1]);
           }
         }
+        constexpr uint32_t k128 = 0x00800080u;
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n) mma<PBS_FP16>(o128[n], k128, k128, k128, k128, b[n][0], b[n][1]);
       }
     } else {
 #pragma unroll
@@ -701,6 +738,7 @@ struct Warp {
   // Sums, reference and weights' sum of this warp's tokens to shared memory, query by query.
   __device__ __forceinline__ void put(float* sums, float* refs, float* weights) {
     __syncwarp();
+    if constexpr (C::BITS == 8) move_sums();
 #pragma unroll
     for (int n = 0; n < C::NT; ++n)
 #pragma unroll
@@ -731,7 +769,7 @@ struct Warp {
           }
         } else if constexpr (C::BITS == 8) {
 #pragma unroll
-          for (int i = 0; i < C::D / 16; ++i) *reinterpret_cast<float2*>(row + 16 * i + 2 * (lane / 4)) = make_float2(o[i][n][c], o[i][n][c + 2]);
+          for (int i = 0; i < C::D / 16; ++i) *reinterpret_cast<float2*>(row + 16 * i + 2 * (lane / 4)) = make_float2(o[i][n][c] * 0x1p24f, o[i][n][c + 2] * 0x1p24f);
         } else {
 #pragma unroll
           for (int i = 0; i < C::D / 16; ++i) {
@@ -778,22 +816,41 @@ __device__ __forceinline__ void load_queries(const AttnArgs& p, const Item& it, 
       }
 #pragma unroll
       for (int s = PIECES / 2; s > 0; s >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
-      // most = 2^e * [1, 2): scaled by 2^k, k = 14 - e, kept where 2^k and the factor 2^(24 - k) are ordinary numbers
+      // most = 2^e * [1, 2): scaled by 2^k, k = 14 - e, kept where 2^k and the factor 2^-k or 2^(24 - k) are ordinary numbers
       int k = most > 0.f ? 14 - ((int)(__float_as_uint(most) >> 23) - 127) : 0;
+      if constexpr (C::BITS == 8) {                                // (two signed bytes hold up to 32639)
+        if ((__float_as_uint(most) & 0x7fffffu) > 0x7efe00u) --k;
+      }
       k = min(max(k, -90), 120);
       const float up = __uint_as_float((uint32_t)(k + 127) << 23);
       f *= __uint_as_float((uint32_t)((C::BITS == 4 ? 24 : 0) - k + 127) << 23);
-#pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        x[t] = __half2float(__float2half_rn(x[t] * up));
-        sum += x[t];
-      }
       if constexpr (C::BITS == 8) {
-        // codes 0 and 2, and 1 and 3, of a word meet in a register
-        uint8_t* const at = frag + (((pc / 4) * C::NT + col / 8) * 32 + (col % 8) * 4 + pc % 2 * 2) * 16 + pc / 2 % 2 * 8;
-        *reinterpret_cast<uint2*>(at) = make_uint2(pack_half(x[0], x[2]), pack_half(x[1], x[3]));
-        *reinterpret_cast<uint2*>(at + 16) = make_uint2(pack_half(x[4], x[6]), pack_half(x[5], x[7]));
+        // integers of two bytes: rounded by up to 2^-15 of the row's largest, which moves a score by as much of it times the sum of a key's
+        // magnitudes at most (bf16 queries lose nothing down to 2^-7 of the largest).  What no integer is makes the row NaN
+        uint32_t high[2] = {0, 0}, low[2] = {0, 0};
+        float none = 0.f;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) none += x[t] * 0.f;
+#pragma unroll
+        for (int s = PIECES / 2; s > 0; s >>= 1) none += __shfl_xor_sync(0xffffffffu, none, s);
+        f += none;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          const int i = __float2int_rn(x[t] * up), h = (i + 128) >> 8;
+          high[t / 4] |= (h & 0xff) << t % 4 * 8;
+          low[t / 4] |= ((i - h * 256) & 0xff) << t % 4 * 8;
+        }
+        uint32_t* const at = reinterpret_cast<uint32_t*>(frag + (((pc / 4) * C::NT + col / 8) * 32 + (col % 8) * 4 + pc % 2 * 2) * 16) + pc / 2 % 2;
+        at[0] = high[0];
+        at[2] = low[0];
+        at[4] = high[1];
+        at[6] = low[1];
       } else {
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          x[t] = __half2float(__float2half_rn(x[t] * up));
+          sum += x[t];
+        }
 #pragma unroll
         for (int s = C::G / 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
         if (pc % (C::G / 8) == 0) qsum[pc / (C::G / 8) * C::COLS + col] = sum * 0x1p-24f;
@@ -1019,7 +1076,7 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
       const uint32_t hole = holes >> slot * C::MT & ((1u << C::MT) - 1);
       if (t0 > plain || hole) w.template tile<true>(stage, t0, hole);
       else w.template tile<false>(stage, t0, 0);
-      if (C::SHIFT > 0 && i % kShiftEvery == kShiftEvery - 1) w.move_sums();
+      if ((C::SHIFT > 0 || C::BITS == 8) && i % kShiftEvery == kShiftEvery - 1) w.move_sums();
       slot = slot == C::STAGES - 1 ? 0 : slot + 1;
     }
     copy_wait<0>();

@@ -62,9 +62,9 @@ def values8(cache, codes, scales, table, b, n):
 def attention8(q, cache, table, lens, new=None, scale=None):
     """The result in 64 bits and a bound of the kernel's error, both (B, Hq, S, D).
 
-    Scores are sums of D exact products held in 32 bits, up to D / 16 + 4 of its roundings deep, each of them up to 2^-22 of the sum of
-    magnitudes; a score that is e off changes its weight by the factor exp(e), and so the result by up to 2 e times the weighted
-    magnitudes.  Weights times scales are rounded to fp16; where they are subnormal, by up to 2^-25, where the largest of them is at
+    Queries are rounded by up to 2^-15 of the row's largest, and scores, sums of D products of integers, a few times in 32 bits (taken as up to
+    D / 16 + 4 roundings of 2^-22 of the sum of magnitudes); a score that is e off changes its weight by the factor exp(e), and so the result by
+    up to 2 e times the weighted magnitudes.  Weights times scales are rounded to fp16; where they are subnormal, by up to 2^-25, where the largest of them is at
     least 2^7 and the codes are at most 127: over n tokens that comes to n 2^-32 of the largest magnitude that a block has room for."""
     B, Hq, S, D = q.shape
     scale = 1 / math.sqrt(D) if scale is None else scale
@@ -82,6 +82,7 @@ def attention8(q, cache, table, lens, new=None, scale=None):
             x = q[b, :, i].double().view(cache.kv_heads, -1, D)
             s = torch.einsum("hgd,htd->hgt", x, k[:, :end]) * scale
             e = torch.einsum("hgd,htd->hgt", x.abs(), k[:, :end].abs()).amax(-1, keepdim=True) * abs(scale) * (D / 16 + 4) * 2.0 ** -22
+            e = e + (x.abs().amax(-1, keepdim=True) * k[:, :end].abs().sum(-1).amax(-1)[:, None, None]) * abs(scale) * 2.0 ** -15
             p = torch.softmax(s, -1)
             o, a = torch.einsum("hgt,htd->hgd", p, v[:, :end]), torch.einsum("hgt,htd->hgd", p, v[:, :end].abs())
             want[b, :, i] = o.reshape(Hq, D)

@@ -161,6 +161,36 @@ def test_what_a_row_does_not_see_does_not_reach_it():
     assert paged_attn_fwd(q, cache, table, ints(100))[:, :, 26:].isnan().all()
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_queries_that_are_not_finite(bad):
+    """Their rows are NaN, and no others."""
+    from pbs_attn_b200.decode import paged_attn_fwd
+    lens = [90, 33]
+    q, cache, table = _case(lens, S=2)
+    want = paged_attn_fwd(q, cache, table, ints(*lens))
+    q = q.clone()
+    q[1, 3, 1, 77] = bad
+    got = paged_attn_fwd(q, cache, table, ints(*lens))
+    assert got[1, 3, 1].isnan().all()
+    got[1, 3, 1] = want[1, 3, 1]
+    assert torch.equal(got, want)
+
+
+def test_queries_of_very_different_sizes():
+    """One channel far above the others, mantissas next to the largest that two bytes hold, and rows of zeros."""
+    from pbs_attn_b200.decode import paged_attn_fwd
+    lens = [200]
+    for dtype in (torch.bfloat16, torch.float16):
+        q, cache, table = _case(lens, Hq=8, Hkv=1, dtype=dtype)
+        q = q.clone()
+        for i, x in enumerate((255 / 128, 127 / 64, 1.0, 1.9921264, 1.99999, 2.0 ** -10)):
+            q[0, i, 0, 5 * i] = 8 * x
+        q[0, 6] = 0
+        q[0, 7, 0, 1:] = 0
+        _run(q, cache, table, lens)
+        assert paged_attn_fwd(q, cache, table, ints(*lens))[0, 6].isfinite().all()
+
+
 def test_pages_that_are_not_there():
     from pbs_attn_b200 import _cabi
     from pbs_attn_b200.decode import paged_attn_fwd
