@@ -792,79 +792,95 @@ struct Item {
 // Brings the queries of an item into the order of the product's second operand (in 8 and 4 bits scaled by a power of two to a maximum in
 // [2^14, 2^15), which fp16 holds to 2^-38 of it), and what belongs to each.
 template <class C>
-__device__ __forceinline__ void load_queries(const AttnArgs& p, const Item& it, uint8_t* frag, float* qsum, float* factor, int* limit) {
+struct Queries {
   using T = typename C::T;
-  constexpr int PIECES = C::D / 8;
-  for (int e = threadIdx.x; e < C::COLS * PIECES; e += C::THREADS) {
-    const int col = e / PIECES, pc = e % PIECES, r = it.row0 + col, i = r / p.group;
-    const bool valid = i < it.n;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (valid) raw = *reinterpret_cast<const uint4*>((const T*)p.q.p + it.seq * p.q.st.b + (it.head * p.group + r % p.group) * p.q.st.h + i * p.q.st.s + 8 * pc);
-    float f = p.scale;
-    if constexpr (C::BITS == 16) {
-      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  static constexpr int PIECES = C::D / 8, EACH = (C::COLS * PIECES + C::THREADS - 1) / C::THREADS;     // 16-byte pieces of a row; of a thread
+  uint4 raws[EACH];
+
+  __device__ __forceinline__ void load(const AttnArgs& p, const Item& it) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-        *reinterpret_cast<uint32_t*>(frag + (((pc / 4) * C::NT + col / 8) * 32 + (col % 8) * 4 + t) * 16 + (pc / 2 % 2 * 2 + pc % 2) * 4) = w[t];
-    } else {
-      const T* raw8 = reinterpret_cast<const T*>(&raw);
-      float x[8], most = 0.f, sum = 0.f;
-#pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        x[t] = Elem<C::DT>::ld(raw8 + t);
-        most = fmaxf(most, fabsf(x[t]));
-      }
-#pragma unroll
-      for (int s = PIECES / 2; s > 0; s >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
-      // most = 2^e * [1, 2): scaled by 2^k, k = 14 - e, kept where 2^k and the factor 2^-k or 2^(24 - k) are ordinary numbers
-      int k = most > 0.f ? 14 - ((int)(__float_as_uint(most) >> 23) - 127) : 0;
-      if constexpr (C::BITS == 8) {                                // (two signed bytes hold up to 32639)
-        if ((__float_as_uint(most) & 0x7fffffu) > 0x7efe00u) --k;
-      }
-      k = min(max(k, -90), 120);
-      const float up = __uint_as_float((uint32_t)(k + 127) << 23);
-      f *= __uint_as_float((uint32_t)((C::BITS == 4 ? 24 : 0) - k + 127) << 23);
-      if constexpr (C::BITS == 8) {
-        // integers of two bytes: rounded by up to 2^-15 of the row's largest, which moves a score by as much of it times the sum of a key's
-        // magnitudes at most (bf16 queries lose nothing down to 2^-7 of the largest).  What no integer is makes the row NaN
-        uint32_t high[2] = {0, 0}, low[2] = {0, 0};
-        float none = 0.f;
-#pragma unroll
-        for (int t = 0; t < 8; ++t) none += x[t] * 0.f;
-#pragma unroll
-        for (int s = PIECES / 2; s > 0; s >>= 1) none += __shfl_xor_sync(0xffffffffu, none, s);
-        f += none;
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          const int i = __float2int_rn(x[t] * up), h = (i + 128) >> 8;
-          high[t / 4] |= (h & 0xff) << t % 4 * 8;
-          low[t / 4] |= ((i - h * 256) & 0xff) << t % 4 * 8;
-        }
-        uint32_t* const at = reinterpret_cast<uint32_t*>(frag + (((pc / 4) * C::NT + col / 8) * 32 + (col % 8) * 4 + pc % 2 * 2) * 16) + pc / 2 % 2;
-        at[0] = high[0];
-        at[2] = low[0];
-        at[4] = high[1];
-        at[6] = low[1];
-      } else {
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          x[t] = __half2float(__float2half_rn(x[t] * up));
-          sum += x[t];
-        }
-#pragma unroll
-        for (int s = C::G / 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-        if (pc % (C::G / 8) == 0) qsum[pc / (C::G / 8) * C::COLS + col] = sum * 0x1p-24f;
-        // codes i and i + 4 of a word meet in one register; those of bits 4-7 are 16 times too large
-        *reinterpret_cast<uint4*>(frag + (((pc / 4) * C::NT + col / 8) * 32 + (col % 8) * 4 + pc % 4) * 16) =
-            make_uint4(pack_half(x[0], x[4]), pack_half(x[1] * 0.0625f, x[5] * 0.0625f), pack_half(x[2], x[6]), pack_half(x[3] * 0.0625f, x[7] * 0.0625f));
-      }
-    }
-    if (pc == 0) {
-      factor[col] = f;
-      limit[col] = valid ? max(0, min(it.len, it.full - it.n + i + 1)) : INT_MAX;
+    for (int u = 0; u < EACH; ++u) {
+      const int e = threadIdx.x + u * C::THREADS, col = e / PIECES, pc = e % PIECES, r = it.row0 + col, i = r / p.group;
+      raws[u] = make_uint4(0, 0, 0, 0);
+      if (e < C::COLS * PIECES && i < it.n)
+        raws[u] = *reinterpret_cast<const uint4*>((const T*)p.q.p + it.seq * p.q.st.b + (it.head * p.group + r % p.group) * p.q.st.h + i * p.q.st.s + 8 * pc);
     }
   }
-}
+
+  __device__ __forceinline__ void put(const AttnArgs& p, const Item& it, uint8_t* frag, float* qsum, float* factor, int* limit) const {
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+      const int e = threadIdx.x + u * C::THREADS;
+      if (e >= C::COLS * PIECES) break;                              // (whole warps: shuffles are among the lanes of a row)
+      const int col = e / PIECES, pc = e % PIECES, r = it.row0 + col, i = r / p.group;
+      const bool valid = i < it.n;
+      const uint4 raw = raws[u];
+      float f = p.scale;
+      if constexpr (C::BITS == 16) {
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          *reinterpret_cast<uint32_t*>(frag + (((pc / 4) * C::NT + col / 8) * 32 + (col % 8) * 4 + t) * 16 + (pc / 2 % 2 * 2 + pc % 2) * 4) = w[t];
+      } else {
+        const T* raw8 = reinterpret_cast<const T*>(&raw);
+        float x[8], most = 0.f, sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          x[t] = Elem<C::DT>::ld(raw8 + t);
+          most = fmaxf(most, fabsf(x[t]));
+        }
+#pragma unroll
+        for (int s = PIECES / 2; s > 0; s >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
+        // most = 2^e * [1, 2): scaled by 2^k, k = 14 - e, kept where 2^k and the factor 2^-k or 2^(24 - k) are ordinary numbers
+        int k = most > 0.f ? 14 - ((int)(__float_as_uint(most) >> 23) - 127) : 0;
+        if constexpr (C::BITS == 8) {                                // (two signed bytes hold up to 32639)
+          if ((__float_as_uint(most) & 0x7fffffu) > 0x7efe00u) --k;
+        }
+        k = min(max(k, -90), 120);
+        const float up = __uint_as_float((uint32_t)(k + 127) << 23);
+        f *= __uint_as_float((uint32_t)((C::BITS == 4 ? 24 : 0) - k + 127) << 23);
+        if constexpr (C::BITS == 8) {
+          // integers of two bytes: rounded by up to 2^-15 of the row's largest, which moves a score by as much of it times the sum of a key's
+          // magnitudes at most (bf16 queries lose nothing down to 2^-7 of the largest).  What no integer is makes the row NaN
+          uint32_t high[2] = {0, 0}, low[2] = {0, 0};
+          float none = 0.f;
+#pragma unroll
+          for (int t = 0; t < 8; ++t) none += x[t] * 0.f;
+#pragma unroll
+          for (int s = PIECES / 2; s > 0; s >>= 1) none += __shfl_xor_sync(0xffffffffu, none, s);
+          f += none;
+#pragma unroll
+          for (int t = 0; t < 8; ++t) {
+            const int i = __float2int_rn(x[t] * up), h = (i + 128) >> 8;
+            high[t / 4] |= (h & 0xff) << t % 4 * 8;
+            low[t / 4] |= ((i - h * 256) & 0xff) << t % 4 * 8;
+          }
+          uint32_t* const at = reinterpret_cast<uint32_t*>(frag + (((pc / 4) * C::NT + col / 8) * 32 + (col % 8) * 4 + pc % 2 * 2) * 16) + pc / 2 % 2;
+          at[0] = high[0];
+          at[2] = low[0];
+          at[4] = high[1];
+          at[6] = low[1];
+        } else {
+#pragma unroll
+          for (int t = 0; t < 8; ++t) {
+            x[t] = __half2float(__float2half_rn(x[t] * up));
+            sum += x[t];
+          }
+#pragma unroll
+          for (int s = C::G / 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+          if (pc % (C::G / 8) == 0) qsum[pc / (C::G / 8) * C::COLS + col] = sum * 0x1p-24f;
+          // codes i and i + 4 of a word meet in one register; those of bits 4-7 are 16 times too large
+          *reinterpret_cast<uint4*>(frag + (((pc / 4) * C::NT + col / 8) * 32 + (col % 8) * 4 + pc % 4) * 16) =
+              make_uint4(pack_half(x[0], x[4]), pack_half(x[1] * 0.0625f, x[5] * 0.0625f), pack_half(x[2], x[6]), pack_half(x[3] * 0.0625f, x[7] * 0.0625f));
+        }
+      }
+      if (pc == 0) {
+        factor[col] = f;
+        limit[col] = valid ? max(0, min(it.len, it.full - it.n + i + 1)) : INT_MAX;
+      }
+    }
+  }
+};
 
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __grid_constant__ AttnArgs p) {
@@ -981,13 +997,12 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
       paged_fault(p.a, PBS_PAGED_BAD_PAGE);
       return -1;
     };
-    auto fetch = [&] {                                             // pages of the next tile
+    auto fetch = [&](int (&page)[C::MT]) {                         // pages of the next tile
       page[0] = lookup(next);
       if constexpr (C::MT == 2) page[1] = p.a.shift > 4 ? page[0] : lookup(next + 16);   // (tiles start at multiples of 32)
       next += C::UNIT;
     };
-    auto issue = [&](int slot) {                                   // its copies, to this place in the ring, once its pages are here
-      const int t0 = next - C::UNIT;
+    auto issue = [&](int slot, int t0, const int (&page)[C::MT]) { // the copies of a tile, to this place in the ring, once its pages are here
       const uint32_t at = ring_at + slot * C::STAGE;
       if constexpr (C::BITS == 8) {                                // scales: a lane one
         const int m = lane >> 1, pg = C::MT == 2 && m == 1 ? page[C::MT - 1] : page[0], first = t0 + 16 * m;
@@ -1054,14 +1069,19 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
         }
       }
     };
-    fetch();
+    // the queries and the pages of the first tiles on their way together: one after the other they took 5 us under load
+    Queries<C> queries;
+    queries.load(p, it);
+    int first_pages[C::STAGES - 1][C::MT];
+#pragma unroll
+    for (int s = 0; s < C::STAGES - 1; ++s) fetch(first_pages[s]);
+    fetch(page);
 #pragma unroll
     for (int s = 0; s < C::STAGES - 1; ++s) {
-      if (s < mine) issue(s);
-      fetch();
+      if (s < mine) issue(s, tok0 + warp * C::TILE + s * C::UNIT, first_pages[s]);
       copy_commit();
     }
-    load_queries<C>(p, it, frag, qsum, factor, limit);
+    queries.put(p, it, frag, qsum, factor, limit);
     w.start();
     __syncthreads();
     int slot = 0, t0 = tok0 + warp * C::TILE;
@@ -1069,8 +1089,8 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
     for (int i = 0; i < mine; ++i, t0 += C::UNIT) {
       copy_wait<C::STAGES - 2>();
       __syncwarp();                                                // (the place read last is free in all lanes, too)
-      if (i + C::STAGES - 1 < mine) issue(slot == 0 ? C::STAGES - 1 : slot - 1);
-      fetch();
+      if (i + C::STAGES - 1 < mine) issue(slot == 0 ? C::STAGES - 1 : slot - 1, t0 + (C::STAGES - 1) * C::UNIT, page);
+      fetch(page);
       copy_commit();
       const uint8_t* stage = ring + slot * C::STAGE;
       const uint32_t hole = holes >> slot * C::MT & ((1u << C::MT) - 1);
