@@ -9,6 +9,7 @@
 // TB/s; 75 % of the issue slots are taken: some 170 instructions for eight channels), back out 11 us; 64 sequences' next tokens, 32 query
 // heads rotated, 2.5 us.
 #include <climits>
+#include <type_traits>
 
 #include "pbs_paged.cuh"
 
@@ -246,94 +247,118 @@ __device__ __forceinline__ void signed4(uint32_t w, float (&x)[4]) {
 
 constexpr float kLeastScale = 7.52316385e-37f;             // 2^-120: its reciprocal is an ordinary number
 
-// blocks: of tokens that a sequence's new ones may lie in; kv_ctas: CTAs that write keys and values, the others turn queries
+// Queries, rotated: group g of lanes takes a token, and p.chunk of its heads.
+template <class T, int D>
+__device__ __forceinline__ void turn_queries(const AppendArgs& p, int g) {
+  constexpr int LPR = D / 8;
+  const pbs_paged_batch_t& bt = p.a.b;
+  const int lane = threadIdx.x % LPR, token = g / p.q_chunks, head0 = g % p.q_chunks * p.chunk;
+  const bool active = token < bt.batch * bt.new_tokens;    // (the other lanes go along: a warp's shuffles take all of them)
+  const int n = min(p.chunk, p.q_heads - head0), seq = active ? token / bt.new_tokens : 0, i = active ? token % bt.new_tokens : 0;
+  int pos = active ? new_position(bt, seq, i) : -1;
+  uint4 cs = make_uint4(0, 0, 0, 0), sn = cs;
+  if (pos >= 0) {
+    if (p.table_rows > 0 && pos >= p.table_rows) {
+      paged_fault(p.a, PBS_PAGED_BAD_ROTARY);
+      pos = -1;
+    } else {
+      const int64_t at = (p.table_rows > 0 ? pos * p.cs_s : seq * p.cs_b + i * p.cs_s) + 8 * lane;
+      cs = *reinterpret_cast<const uint4*>((const T*)p.cosp + at);
+      sn = *reinterpret_cast<const uint4*>((const T*)p.sinp + at);
+    }
+  }
+  const T* in = (const T*)p.q.p + seq * p.q.st.b + head0 * p.q.st.h + i * p.q.st.s + 8 * lane;
+  T* out = (T*)p.qo.p + seq * p.qo.st.b + head0 * p.qo.st.h + i * p.qo.st.s + 8 * lane;
+  for (int r = 0; r < p.chunk; ++r) {
+    uint4 w = r < n ? *reinterpret_cast<const uint4*>(in + r * p.q.st.h) : make_uint4(0, 0, 0, 0);
+    float x[8];
+    turned8<T, LPR>(w, cs, sn, lane, x);
+    w = pack8<T>(x);
+    if (pos < 0) w = make_uint4(0, 0, 0, 0);               // (a row that is left out)
+    if (active && r < n) *reinterpret_cast<uint4*>(out + r * p.qo.st.h) = w;
+  }
+}
+
+// A block of a sequence's tokens, of a head's keys or values, that new ones come into.
+struct Block {
+  int seq, head, shift, first, end, begin;                 // first .. end - 1: positions of its new tokens; shift: of the call's first row; begin: of the block
+  bool is_v, covers;                                       // covers: there are any
+};
+
+// Unit u of the call's: heads go fastest, then keys and values, then the `blocks` that a sequence's new tokens may lie in.
+__device__ __forceinline__ Block block_of(const AppendArgs& p, int u, int blocks) {
+  const pbs_paged_batch_t& bt = p.a.b;
+  Block b;
+  b.head = u % p.a.c.kv_heads;
+  int rest = u / p.a.c.kv_heads;
+  b.is_v = rest % 2;
+  rest /= 2;
+  b.seq = rest / blocks;
+  const int n = bt.new_lens ? min(max(bt.new_lens[b.seq], 0), bt.new_tokens) : bt.new_tokens, len = bt.seq_lens[b.seq];
+  b.shift = len - n;
+  b.end = len;
+  if (p.cosp && p.table_rows > 0 && len > p.table_rows && n > 0) {
+    paged_fault(p.a, PBS_PAGED_BAD_ROTARY);
+    b.end = p.table_rows;
+  }
+  const int start = max(0, b.shift), block = (start >> p.a.block_shift) + rest % blocks;
+  b.covers = n > 0 && b.end > start && block <= (b.end - 1) >> p.a.block_shift;
+  b.begin = block << p.a.block_shift;
+  b.first = max(start, b.begin);
+  b.end = min(b.end, b.begin + p.a.c.block_size);
+  return b;
+}
+
+// A block's scale with new tokens of magnitudes up to `most` in it; old: of the tokens that it holds, 0 for none.
+__device__ __forceinline__ float scale_of(float most, float old) {
+  const float scale = most <= 3.402823466e38f ? fmaxf(__fmul_rn(most, 1.f / 127.f), kLeastScale) : CUDART_NAN_F;
+  return max_nan(scale, old);
+}
+
+__device__ __forceinline__ uint2 scaled8(const uint2& w, float ratio) {
+  float a[4], b[4], y[8];
+  signed4(w.x, a);
+  signed4(w.y, b);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    y[j] = a[j];
+    y[j + 4] = b[j];
+  }
+  return codes8(y, ratio);
+}
+
+// Prompts: a warp takes 16 tokens of a block, blocks of 32 and 64 are several warps'.
 template <int DT, int D, int W, bool ROPE>
-__global__ void __launch_bounds__(kThreads, ROPE && D == 256 ? 1 : 2) paged_append8_kernel(const __grid_constant__ AppendArgs p, int blocks, int units, int kv_ctas) {
+__global__ void __launch_bounds__(kThreads, D == 256 ? ROPE ? 1 : 2 : ROPE ? 2 : 4) paged_append8_kernel(const __grid_constant__ AppendArgs p, int blocks, int units) {
   using T = typename Elem<DT>::T;
   constexpr int LPR = D / 8, RPI = 32 / LPR, NI = 16 / RPI;  // lanes a row; rows at a time, and times, of a warp's 16
   const pbs_paged_cache_t& c = p.a.c;
-  const pbs_paged_batch_t& bt = p.a.b;
-  if (ROPE && (int)blockIdx.x >= kv_ctas) {                // queries: a token, and p.chunk of its heads, a group of lanes
-    const int lane = threadIdx.x % LPR, g = ((int)blockIdx.x - kv_ctas) * (kThreads / LPR) + threadIdx.x / LPR;
-    const int token = g / p.q_chunks, head0 = g % p.q_chunks * p.chunk;
-    const bool active = token < bt.batch * bt.new_tokens;    // (the other lanes go along: a warp's shuffles take all of them)
-    const int n = min(p.chunk, p.q_heads - head0), seq = active ? token / bt.new_tokens : 0, i = active ? token % bt.new_tokens : 0;
-    int pos = active ? new_position(bt, seq, i) : -1;
-    uint4 cs = make_uint4(0, 0, 0, 0), sn = cs;
-    if (pos >= 0) {
-      if (p.table_rows > 0 && pos >= p.table_rows) {
-        paged_fault(p.a, PBS_PAGED_BAD_ROTARY);
-        pos = -1;
-      } else {
-        const int64_t at = (p.table_rows > 0 ? pos * p.cs_s : seq * p.cs_b + i * p.cs_s) + 8 * lane;
-        cs = *reinterpret_cast<const uint4*>((const T*)p.cosp + at);
-        sn = *reinterpret_cast<const uint4*>((const T*)p.sinp + at);
-      }
-    }
-    const T* in = (const T*)p.q.p + seq * p.q.st.b + head0 * p.q.st.h + i * p.q.st.s + 8 * lane;
-    T* out = (T*)p.qo.p + seq * p.qo.st.b + head0 * p.qo.st.h + i * p.qo.st.s + 8 * lane;
-    for (int r = 0; r < p.chunk; ++r) {
-      uint4 w = r < n ? *reinterpret_cast<const uint4*>(in + r * p.q.st.h) : make_uint4(0, 0, 0, 0);
-      float x[8];
-      turned8<T, LPR>(w, cs, sn, lane, x);
-      w = pack8<T>(x);
-      if (pos < 0) w = make_uint4(0, 0, 0, 0);             // (a row that is left out)
-      if (active && r < n) *reinterpret_cast<uint4*>(out + r * p.qo.st.h) = w;
-    }
-    return;
-  }
-  // the warp's 16 tokens: positions t0 .. of a head's keys or values, of them first .. end - 1 new
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, col = lane % LPR;
-  const int unit = (int)blockIdx.x * (kThreads / 32 / W) + warp / W;
-  int head = 0, seq = 0, first = 0, end = 0, shift_i = 0, begin = 0, page = -1;
-  bool is_v = false;
-  if (unit < units) {
-    head = unit % c.kv_heads;
-    int rest = unit / c.kv_heads;
-    is_v = rest % 2;
-    rest /= 2;
-    seq = rest / blocks;
-    const int n = bt.new_lens ? min(max(bt.new_lens[seq], 0), bt.new_tokens) : bt.new_tokens, len = bt.seq_lens[seq];
-    shift_i = len - n;                                     // position of the first row
-    first = max(0, shift_i);
-    end = len;
-    if (p.cosp && p.table_rows > 0 && end > p.table_rows && n > 0) {
-      paged_fault(p.a, PBS_PAGED_BAD_ROTARY);
-      end = p.table_rows;
-    }
-    const int block = (first >> p.a.block_shift) + rest % blocks;
-    if (n > 0 && end > first && block <= (end - 1) >> p.a.block_shift) {
-      begin = block << p.a.block_shift;
-      page = page_of(p.a, seq, begin);
-    }
-  }
-  const bool active = page >= 0;
-  first = max(first, begin);
-  const int t0 = begin + warp % W * 16 + lane / LPR;       // this lane's first token, RPI apart
-  const RowTensor& src = is_v ? p.v : p.k;
-  const T* in = (const T*)src.p + seq * src.st.b + head * src.st.h + 8 * col;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, col = lane % LPR, unit = (int)blockIdx.x * (kThreads / 32 / W) + warp / W;
+  Block b{};
+  if (unit < units) b = block_of(p, unit, blocks);
+  const int t0 = b.begin + warp % W * 16 + lane / LPR;     // this lane's first token, RPI apart
+  const RowTensor& src = b.is_v ? p.v : p.k;
+  const T* in = (const T*)src.p + b.seq * src.st.b + b.head * src.st.h + 8 * col;
+  auto fresh = [&](int k) { return b.covers && t0 + k * RPI >= b.first && t0 + k * RPI < b.end; };
   uint4 raw[NI];
 #pragma unroll
-  for (int k = 0; k < NI; ++k) {
-    const int t = t0 + k * RPI;
-    raw[k] = make_uint4(0, 0, 0, 0);
-    if (active && t >= first && t < end) raw[k] = *reinterpret_cast<const uint4*>(in + (int64_t)(t - shift_i) * src.st.s);
-  }
-  const bool older = active && first > begin;              // the block holds tokens already
-  const int slot = begin & (c.page_size - 1);
-  float* const scale_at = (float*)(is_v ? c.v_params : c.k_params) +
-                          (active ? slot_offset(is_v ? c.v_params_strides : c.k_params_strides, page, head, slot >> p.a.block_shift) : 0);
+  for (int k = 0; k < NI; ++k)
+    raw[k] = fresh(k) ? *reinterpret_cast<const uint4*>(in + (int64_t)(t0 + k * RPI - b.shift) * src.st.s) : make_uint4(0, 0, 0, 0);
+  const int page = b.covers ? page_of(p.a, b.seq, b.begin) : -1, slot = b.begin & (c.page_size - 1);
+  const bool active = page >= 0, older = active && b.first > b.begin;      // older: the block holds tokens already
+  float* const scale_at = (float*)(b.is_v ? c.v_params : c.k_params) +
+                          (active ? slot_offset(b.is_v ? c.v_params_strides : c.k_params_strides, page, b.head, slot >> p.a.block_shift) : 0);
   const float old = older ? *scale_at : 0.f;
   float most = 0.f;
   float x[ROPE ? NI : 1][8];
-  const bool turn = ROPE && !is_v;
+  const bool turn = ROPE && !b.is_v;
   if (turn) {
 #pragma unroll
     for (int k = 0; k < (ROPE ? NI : 0); ++k) {
       const int t = t0 + k * RPI;
       uint4 cs = make_uint4(0, 0, 0, 0), sn = cs;
-      if (active && t >= first && t < end) {
-        const int64_t at = (p.table_rows > 0 ? t * p.cs_s : seq * p.cs_b + (t - shift_i) * p.cs_s) + 8 * col;
+      if (fresh(k)) {
+        const int64_t at = (p.table_rows > 0 ? t * p.cs_s : b.seq * p.cs_b + (t - b.shift) * p.cs_s) + 8 * col;
         cs = *reinterpret_cast<const uint4*>((const T*)p.cosp + at);
         sn = *reinterpret_cast<const uint4*>((const T*)p.sinp + at);
       }
@@ -356,31 +381,16 @@ __global__ void __launch_bounds__(kThreads, ROPE && D == 256 ? 1 : 2) paged_appe
     for (int k = 1; k < W; ++k) most = max_nan(most, meet[warp / W * W + k]);
   }
   if (!active) return;
-  float scale = fmaxf(__fmul_rn(most, 1.f / 127.f), kLeastScale);
-  if (!(most <= 3.402823466e38f)) scale = CUDART_NAN_F;
-  if (older) scale = max_nan(scale, old);
+  const float scale = scale_of(most, old), inv = __fdiv_rn(1.f, scale);
   const bool grown = older && scale != old;                // (of one that is NaN the codes are nothing)
-  const float inv = __fdiv_rn(1.f, scale), ratio = grown ? __fdiv_rn(old, scale) : 1.f;
-  int8_t* const out = (int8_t*)(is_v ? c.v : c.k) + slot_offset(is_v ? c.v_strides : c.k_strides, page, head, 0) + 8 * col;
-  const int64_t step = (is_v ? c.v_strides : c.k_strides)[2];
+  int8_t* const out = (int8_t*)(b.is_v ? c.v : c.k) + slot_offset(b.is_v ? c.v_strides : c.k_strides, page, b.head, 0) + 8 * col;
+  const int64_t step = (b.is_v ? c.v_strides : c.k_strides)[2];
 #pragma unroll
   for (int k = 0; k < NI; ++k) {
     const int t = t0 + k * RPI;
-    if (t < first ? !grown : t >= end) continue;
     uint2* const at = reinterpret_cast<uint2*>(out + (t & (c.page_size - 1)) * step);
-    float y[8];
-    if (t < first) {
-      const uint2 w = *at;
-      float a[4], b[4];
-      signed4(w.x, a);
-      signed4(w.y, b);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        y[j] = a[j];
-        y[j + 4] = b[j];
-      }
-      *at = codes8(y, ratio);
-    } else {
+    if (t >= b.first && t < b.end) {
+      float y[8];
       if (turn) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] = x[ROPE ? k : 0][j];
@@ -390,7 +400,92 @@ __global__ void __launch_bounds__(kThreads, ROPE && D == 256 ? 1 : 2) paged_appe
       *at = codes8(y, inv);
     }
   }
+  if (grown) {
+    const float ratio = __fdiv_rn(old, scale);
+#pragma unroll 1
+    for (int k = 0; k < NI; ++k) {
+      const int t = t0 + k * RPI;
+      uint2* const at = reinterpret_cast<uint2*>(out + (t & (c.page_size - 1)) * step);
+      if (t < b.first) *at = scaled8(*at, ratio);
+    }
+  }
   if (lane == 0 && warp % W == 0) *scale_at = scale;
+}
+
+constexpr int kFew = 4;                                    // rows of a lane
+
+// A few tokens a sequence: a warp takes all of a block, its new tokens in registers.  Latency is all there is: lengths, then rows and the page's
+// number, then the scale and what is written, in little code (with the kernel above, unrolled for 16 tokens a warp, one token took 5.2 us).
+// The CTAs behind kv_ctas turn queries.
+template <int DT, int D, bool ROPE>
+__global__ void __launch_bounds__(kThreads) paged_append8_few_kernel(const __grid_constant__ AppendArgs p, int blocks, int units, int kv_ctas) {
+  using T = typename Elem<DT>::T;
+  constexpr int LPR = D / 8, RPI = 32 / LPR;
+  if (ROPE && (int)blockIdx.x >= kv_ctas) {
+    turn_queries<T, D>(p, ((int)blockIdx.x - kv_ctas) * (kThreads / LPR) + threadIdx.x / LPR);
+    return;
+  }
+  const pbs_paged_cache_t& c = p.a.c;
+  const int lane = threadIdx.x % 32, col = lane % LPR, unit = (int)blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
+  if (unit >= units) return;
+  const Block b = block_of(p, unit, blocks);
+  if (!b.covers) return;
+  const RowTensor& src = b.is_v ? p.v : p.k;
+  const T* in = (const T*)src.p + b.seq * src.st.b + b.head * src.st.h + 8 * col;
+  const int t0 = b.first + lane / LPR;
+  const bool turn = ROPE && !b.is_v;
+  uint4 raw[kFew], cs[kFew], sn[kFew];
+#pragma unroll
+  for (int k = 0; k < kFew; ++k) {
+    const int t = t0 + k * RPI;
+    raw[k] = cs[k] = sn[k] = make_uint4(0, 0, 0, 0);
+    if (t >= b.end) continue;
+    raw[k] = *reinterpret_cast<const uint4*>(in + (int64_t)(t - b.shift) * src.st.s);
+    if (turn) {
+      const int64_t at = (p.table_rows > 0 ? t * p.cs_s : b.seq * p.cs_b + (t - b.shift) * p.cs_s) + 8 * col;
+      cs[k] = *reinterpret_cast<const uint4*>((const T*)p.cosp + at);
+      sn[k] = *reinterpret_cast<const uint4*>((const T*)p.sinp + at);
+    }
+  }
+  const int page = page_of(p.a, b.seq, b.begin), slot = b.begin & (c.page_size - 1);
+  if (page < 0) return;                                    // (the whole warp's)
+  const bool older = b.first > b.begin;
+  float* const scale_at = (float*)(b.is_v ? c.v_params : c.k_params) + slot_offset(b.is_v ? c.v_params_strides : c.k_params_strides, page, b.head, slot >> p.a.block_shift);
+  const float old = older ? *scale_at : 0.f;
+  float most = 0.f, x[kFew][8];
+#pragma unroll
+  for (int k = 0; k < kFew; ++k) {
+    if (b.first + k * RPI >= b.end) break;
+    if (turn) turned8<T, LPR>(raw[k], cs[k], sn[k], col, x[k]);
+    else unpack8<T>(raw[k], x[k]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) most = max_nan(most, fabsf(x[k][j]));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+  const float scale = scale_of(most, old), inv = __fdiv_rn(1.f, scale);
+  int8_t* const out = (int8_t*)(b.is_v ? c.v : c.k) + slot_offset(b.is_v ? c.v_strides : c.k_strides, page, b.head, 0) + 8 * col;
+  const int64_t step = (b.is_v ? c.v_strides : c.k_strides)[2];
+  auto at = [&](int t) { return reinterpret_cast<uint2*>(out + (t & (c.page_size - 1)) * step); };
+#pragma unroll
+  for (int k = 0; k < kFew; ++k) {
+    if (b.first + k * RPI >= b.end) break;
+    if (t0 + k * RPI < b.end) *at(t0 + k * RPI) = codes8(x[k], inv);
+  }
+  if (older && scale != old) {                             // (of one that is NaN the codes are nothing)
+    const float ratio = __fdiv_rn(old, scale);
+    constexpr int A = 4;                                   // rows under way
+    for (int t = b.begin + lane / LPR; t < b.first; t += A * RPI) {
+      uint2 w[A];
+#pragma unroll
+      for (int k = 0; k < A; ++k)
+        if (t + k * RPI < b.first) w[k] = *at(t + k * RPI);
+#pragma unroll
+      for (int k = 0; k < A; ++k)
+        if (t + k * RPI < b.first) *at(t + k * RPI) = scaled8(w[k], ratio);
+    }
+  }
+  if (lane == 0) *scale_at = scale;
 }
 
 template <int DT, int D, int BITS, int G>
@@ -512,22 +607,40 @@ int launch(AppendArgs p, bool gather, cudaStream_t st) {
   return PBS_OK;
 }
 
-template <int DT, int D, int W>
+template <int DT, int D>
 int launch_append8(AppendArgs p, cudaStream_t st) {
-  constexpr int UPC = kThreads / 32 / W, RPB = kThreads / (D / 8);
-  const int S = p.a.b.new_tokens, bs = 16 * W;
+  constexpr int RPB = kThreads / (D / 8), RPI = 256 / D;
+  const int S = p.a.b.new_tokens, bs = p.a.c.block_size;
   const int64_t blocks = ((int64_t)S + 2 * bs - 2) / bs;   // that S tokens reach into, wherever they begin
-  const int64_t units = blocks * p.a.b.batch * 2 * p.a.c.kv_heads, kv_ctas = (units + UPC - 1) / UPC;
-  // heads of a token's queries share its rotary factors: as many as leave every group of lanes something to do
-  const int64_t tokens = (int64_t)p.a.b.batch * S, groups = (int64_t)device_sms() * 4 * RPB;
-  const int64_t chunk = (tokens * p.q_heads + groups - 1) / groups;
-  p.chunk = (int)(chunk < 1 ? 1 : chunk < 8 ? chunk : 8);
-  p.q_chunks = (p.q_heads + p.chunk - 1) / p.chunk;
-  const int64_t ctas = kv_ctas + (tokens * p.q_chunks + RPB - 1) / RPB;
-  if (units > INT_MAX - 1024 || ctas > INT_MAX) { set_error("paged append: too many blocks of tokens in a call"); return PBS_ERR_SHAPE; }
-  if (p.cosp) paged_append8_kernel<DT, D, W, true><<<(unsigned)ctas, kThreads, 0, st>>>(p, (int)blocks, (int)units, (int)kv_ctas);
-  else paged_append8_kernel<DT, D, W, false><<<(unsigned)kv_ctas, kThreads, 0, st>>>(p, (int)blocks, (int)units, (int)kv_ctas);
+  const int64_t units = blocks * p.a.b.batch * 2 * p.a.c.kv_heads, tokens = (int64_t)p.a.b.batch * S;
+  if (units > INT_MAX - 1024) { set_error("paged append: too many blocks of tokens in a call"); return PBS_ERR_SHAPE; }
+  if (S <= kFew * RPI) {
+    // heads of a token's queries share its rotary factors: as many as leave every group of lanes something to do
+    const int64_t groups = (int64_t)device_sms() * 4 * RPB, chunk = (tokens * p.q_heads + groups - 1) / groups, kv_ctas = (units + kThreads / 32 - 1) / (kThreads / 32);
+    p.chunk = (int)(chunk < 1 ? 1 : chunk < 8 ? chunk : 8);
+    p.q_chunks = (p.q_heads + p.chunk - 1) / p.chunk;
+    const unsigned ctas = (unsigned)(kv_ctas + (tokens * p.q_chunks + RPB - 1) / RPB);
+    if (p.cosp) paged_append8_few_kernel<DT, D, true><<<ctas, kThreads, 0, st>>>(p, (int)blocks, (int)units, (int)kv_ctas);
+    else paged_append8_few_kernel<DT, D, false><<<(unsigned)kv_ctas, kThreads, 0, st>>>(p, (int)blocks, (int)units, (int)kv_ctas);
+    PBS_CUDA_CHECK_LAUNCH("paged_append8_few_kernel");
+    return PBS_OK;
+  }
+  auto prompt = [&](auto warps) {
+    constexpr int W = decltype(warps)::value, UPC = kThreads / 32 / W;
+    const unsigned ctas = (unsigned)((units + UPC - 1) / UPC);
+    if (p.cosp) paged_append8_kernel<DT, D, W, true><<<ctas, kThreads, 0, st>>>(p, (int)blocks, (int)units);
+    else paged_append8_kernel<DT, D, W, false><<<ctas, kThreads, 0, st>>>(p, (int)blocks, (int)units);
+  };
+  if (bs == 16) prompt(std::integral_constant<int, 1>());
+  else if (bs == 32) prompt(std::integral_constant<int, 2>());
+  else prompt(std::integral_constant<int, 4>());
   PBS_CUDA_CHECK_LAUNCH("paged_append8_kernel");
+  if (p.q_heads) {                                         // the queries, which cost as much as keys and values, by the kernel that is made for them
+    dim3 grid = deal<D>(p);
+    grid.y = p.q_chunks;
+    paged_append_kernel<DT, D, 16, 0><<<grid, kThreads, 0, st>>>(p, (int)tokens);
+    PBS_CUDA_CHECK_LAUNCH("paged_append_kernel");
+  }
   return PBS_OK;
 }
 
@@ -536,7 +649,7 @@ int by_bits(const AppendArgs& p, bool gather, cudaStream_t st) {
   if (p.a.c.bits == 16) return launch<DT, D, 16, 0>(p, gather, st);
   if (p.a.c.bits == 8) {
     if (gather) return launch_gather<DT, D, 8, 0>(p, st);
-    return p.a.block_shift == 4 ? launch_append8<DT, D, 1>(p, st) : p.a.block_shift == 5 ? launch_append8<DT, D, 2>(p, st) : launch_append8<DT, D, 4>(p, st);
+    return launch_append8<DT, D>(p, st);
   }
   return p.a.c.group_size == 32 ? launch<DT, D, 4, 32>(p, gather, st) : launch<DT, D, 4, 64>(p, gather, st);
 }

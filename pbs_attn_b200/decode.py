@@ -208,7 +208,7 @@ def paged_kv_append(cache: PagedKVCache, key_states: torch.Tensor, value_states:
     ``query_states`` (B, Hq, S, D), if given, into ``query_out`` (a new tensor by default; may be ``query_states``).  The tables
     are (positions, D), looked up by position, or (B or 1, S, D), one row per token as a model hands them over; of the cache's
     dtype.  Without them keys are taken as they are and None is returned.  Padding rows of ``query_out`` are 0.
-    One kernel on the current stream, without synchronising."""
+    One kernel on the current stream (two for a prompt with queries and 8 bits), without synchronising."""
     if cache._native is not None:
         done = cache._host.paged_append(cache._native, key_states, value_states, block_table, seq_lens, new_lens, cos, sin, query_states, query_out)
         if done is not None:
