@@ -17,7 +17,7 @@ namespace pbs {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int P = 2, kStages = 4;          // 16-byte pieces of a thread in a chunk; chunks in shared memory, all but one of them on their way
+constexpr int P = 2, kStages = 3;          // 16-byte pieces of a thread in a chunk; chunks in shared memory, all but one of them on their way
 constexpr int kResident = 4;              // CTAs a SM
 constexpr int kListed = 1024;             // logits that reach the bound; more of them at a time are gone through K times instead
 constexpr int kFound = 320;               // continuations that do
@@ -597,7 +597,7 @@ int launch(const pbs_beam_select_t& a, void* workspace, int64_t* bytes, cudaStre
   p.a = a;
   p.chunks = (int)(((int64_t)a.vocab + N - 1 + CHUNK - 1) / CHUNK);        // (a row may start inside a piece)
   // Segments: so many that all are resident at a time; where there are more rows than that, so short that the CTAs that come last are a small part.
-  const int64_t rows = (int64_t)a.batch * a.beams, resident = (int64_t)kResident * device_sms(), whole = 4 * resident / rows;
+  const int64_t rows = (int64_t)a.batch * a.beams, resident = (int64_t)kResident * device_sms(), whole = 3 * resident / rows;
   const int64_t slices = rows <= resident ? resident / rows : whole > 1 ? whole : 1;
   p.share = (int)((p.chunks + slices - 1) / slices);
   p.slices = (p.chunks + p.share - 1) / p.share;
