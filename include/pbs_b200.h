@@ -356,7 +356,8 @@ int pbs_paged_gather(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* ba
 
 /* Causal attention of the new tokens' queries, q (B, q_heads, S, D), over the cache: token i sees the positions up to its own.
  * out has q's shape; rows that see nothing, or scores of -infinity alone, are 0.  Softmax and sums are held in 32 bits.
- * Range for 16 bits: that of the type (bf16 values below 2^-90 may count as 0).  For 4 bits: in bf16 |q| up to 2^100 (what is 2^29 below
+ * Range for 16 bits: that of the type (bf16 values below 2^-90 may count as 0).  For 8 bits: |v| from 2^-66 to 2^100 in bf16 (what scales below
+ * 2^-70 stand for loses bits); queries are rounded to 2^-15 of the largest of their row.  For 4 bits: in bf16 |q| up to 2^100 (what is 2^29 below
  * the largest of a query's row counts as 0) and |v| from 2^-80 to 2^100; in both types, a group of channels whose steps are 2^20 below
  * those of another group of the head loses bits, and one 2^30 below it counts as its minima.
  * What a row does not see does not reach it, infinities and NaNs included: its bits do not change with the values of tokens behind it or
@@ -438,7 +439,7 @@ int pbs_beam_select(const pbs_beam_select_t* args, void* workspace, int64_t work
  * beams (1 .. 32), and seq_lens the tokens that their caches hold; new_tokens and new_lens are not looked at.  In the table, which is
  * written, entries of full pages become those of the parent; tokens of the page under way are copied, in the caches of all layers, from the
  * parent's page into the row's own (which no other row uses), with what stands for them.  A row and its parent have one length.
- * The caches have one layout: their pages, params and status may differ, the other members not. */
+ * The caches have one layout: their pages, which have to, params and status may differ, the other members not. */
 int pbs_paged_reorder(const pbs_paged_cache_t* const* caches, int32_t layers, const pbs_paged_batch_t* batch, int32_t* block_table,
                       int32_t beams, const int32_t* parents, int64_t parents_stride, void* stream);
 

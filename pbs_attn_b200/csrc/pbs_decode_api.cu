@@ -193,6 +193,8 @@ int pbs_paged_reorder(const pbs_paged_cache_t* const* caches, int32_t layers, co
       same = same && c.k_strides[i] == d.k_strides[i] && c.v_strides[i] == d.v_strides[i];
       same = same && (c.bits == 16 || (c.k_params_strides[i] == d.k_params_strides[i] && c.v_params_strides[i] == d.v_params_strides[i]));
     }
+    for (int32_t m = 0; m < l; ++m)
+      if (caches[m] && caches[m]->k == c.k) { set_error("layers %d and %d are one cache", m, l); return PBS_ERR_ARG; }
     if (!same) { set_error("the caches of a call have one layout: that of layer %d differs from the first's", l); return PBS_ERR_SHAPE; }
   }
   if (a.c.kv_heads > (INT_MAX >> 1)) { set_error("%d heads", a.c.kv_heads); return PBS_ERR_SHAPE; }

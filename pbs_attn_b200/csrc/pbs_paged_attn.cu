@@ -837,7 +837,7 @@ struct Queries {
         if constexpr (C::BITS == 8) {                                // (two signed bytes hold up to 32639)
           if ((__float_as_uint(most) & 0x7fffffu) > 0x7efe00u) --k;
         }
-        k = min(max(k, -90), 120);
+        k = min(max(k, C::BITS == 8 ? -114 : -90), 120);
         const float up = __uint_as_float((uint32_t)(k + 127) << 23);
         f *= __uint_as_float((uint32_t)((C::BITS == 4 ? 24 : 0) - k + 127) << 23);
         if constexpr (C::BITS == 8) {

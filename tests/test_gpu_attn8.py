@@ -140,6 +140,19 @@ def test_blocks_of_zeros_and_values_near_the_ends_of_bf16():
         _run(q, cache, table, [n])
 
 
+@pytest.mark.parametrize("q_size,k_size", [(2.0 ** 120, 2.0 ** -115), (1.99 * 2.0 ** 127, 2.0 ** -116), (2.0 ** -110, 2.0 ** 118), (2.0 ** 60, 2.0 ** -60)])
+def test_queries_and_keys_at_the_ends_of_bf16(q_size, k_size):
+    from pbs_attn_b200.decode import paged_kv_append
+    g = torch.Generator(device="cuda").manual_seed(9)
+    n, D, ps = 300, 64, 16
+    cache = make_cache8(20, ps, 1, D, torch.bfloat16, 16)
+    x = torch.randn(2, 1, 1, n, D, generator=g, device="cuda").clamp(-4, 4)
+    q = (torch.rand(1, 4, 1, D, generator=g, device="cuda", dtype=torch.float64) * 2 - 1) * q_size
+    table = torch.arange(20, dtype=torch.int32, device="cuda")[None]
+    paged_kv_append(cache, (x[0].double() * k_size).bfloat16(), x[1].bfloat16(), table, ints(n))
+    _run(q.bfloat16(), cache, table, [n], scale=0.25 / (q_size * k_size))
+
+
 def test_what_a_row_does_not_see_does_not_reach_it():
     """Blocks behind a row's last token that are not finite, stale pages among them; a block that a row sees makes it NaN."""
     from pbs_attn_b200.decode import paged_attn_fwd, paged_kv_append
