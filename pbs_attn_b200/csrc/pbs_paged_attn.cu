@@ -782,6 +782,24 @@ struct Warp {
   }
 };
 
+// Quotients of numbers from 0 by one that does not change: the common ones are small and take an eighth of a division's time.
+struct Divisor {
+  int d;
+  float inverse;
+  __device__ __forceinline__ explicit Divisor(int n) : d(n), inverse(1.f / (float)n) {}
+  __device__ __forceinline__ int of(int a, int& rest) const {
+    int q = (int)((float)a * inverse);
+    rest = a - q * d;
+    for (; rest < 0; rest += d) --q;
+    for (; rest >= d; rest -= d) ++q;
+    return q;
+  }
+  __device__ __forceinline__ int of(int a) const {
+    int rest;
+    return of(a, rest);
+  }
+};
+
 // The part of an item that a CTA works on.
 struct Item {
   int seq, head, row0;                                             // row = new token * group + query head within the KV head
@@ -798,22 +816,24 @@ struct Queries {
   static constexpr int PIECES = C::D / 8, EACH = (C::COLS * PIECES + C::THREADS - 1) / C::THREADS;     // 16-byte pieces of a row; of a thread
   uint4 raws[EACH];
 
-  __device__ __forceinline__ void load(const AttnArgs& p, const Item& it) {
+  __device__ __forceinline__ void load(const AttnArgs& p, const Item& it, const Divisor& group) {
 #pragma unroll
     for (int u = 0; u < EACH; ++u) {
-      const int e = threadIdx.x + u * C::THREADS, col = e / PIECES, pc = e % PIECES, r = it.row0 + col, i = r / p.group;
+      const int e = threadIdx.x + u * C::THREADS, col = e / PIECES, pc = e % PIECES;
+      int h;
+      const int i = group.of(it.row0 + col, h);
       raws[u] = make_uint4(0, 0, 0, 0);
       if (e < C::COLS * PIECES && i < it.n)
-        raws[u] = *reinterpret_cast<const uint4*>((const T*)p.q.p + it.seq * p.q.st.b + (it.head * p.group + r % p.group) * p.q.st.h + i * p.q.st.s + 8 * pc);
+        raws[u] = *reinterpret_cast<const uint4*>((const T*)p.q.p + it.seq * p.q.st.b + (it.head * p.group + h) * p.q.st.h + i * p.q.st.s + 8 * pc);
     }
   }
 
-  __device__ __forceinline__ void put(const AttnArgs& p, const Item& it, uint8_t* frag, float* qsum, float* factor, int* limit) const {
+  __device__ __forceinline__ void put(const AttnArgs& p, const Item& it, const Divisor& group, uint8_t* frag, float* qsum, float* factor, int* limit) const {
 #pragma unroll
     for (int u = 0; u < EACH; ++u) {
       const int e = threadIdx.x + u * C::THREADS;
       if (e >= C::COLS * PIECES) break;                              // (whole warps: shuffles are among the lanes of a row)
-      const int col = e / PIECES, pc = e % PIECES, r = it.row0 + col, i = r / p.group;
+      const int col = e / PIECES, pc = e % PIECES, i = group.of(it.row0 + col);
       const bool valid = i < it.n;
       const uint4 raw = raws[u];
       float f = p.scale;
@@ -901,12 +921,15 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
 
   // 8 bits: where all sequences are short (two units at most) a unit is a whole one.  What splitting it saves on a tile goes on joining the parts:
   // 187 tokens take 6.9 us in two units a head, 5.9 in one (500 tokens 7.5 in four, 10.8 in one).
+  static_assert((C::UNIT & (C::UNIT - 1)) == 0, "units are a power of two");
   int unit_tokens = C::UNIT;
+  const int own_len = tid < bt.batch ? bt.seq_lens[tid] : 0;       // (of up to THREADS sequences all that is read of the lengths here)
   if constexpr (C::BITS == 8) {
-    bool any = false;
-    for (int b = tid; b < bt.batch; b += C::THREADS) any = any || bt.seq_lens[b] > kWhole * C::UNIT;
+    bool any = own_len > kWhole * C::UNIT;
+    for (int b = tid + C::THREADS; b < bt.batch; b += C::THREADS) any = any || bt.seq_lens[b] > kWhole * C::UNIT;
     if (!__syncthreads_or(any)) unit_tokens = kWhole * C::UNIT;
   }
+  const int unit_shift = __ffs(unit_tokens) - 1;
   // units of all sequences (an empty one has a unit too: its rows are written)
   const int per = p.row_tiles * c.kv_heads;
   int total = 0;
@@ -914,9 +937,9 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
     const int b = b0 + tid;
     int u = 0;
     if (b < bt.batch) {
-      const int len = bt.seq_lens[b];
+      const int len = b0 == 0 ? own_len : bt.seq_lens[b];
       if (len > table_tokens) paged_fault(p.a, PBS_PAGED_BAD_LENGTH);
-      u = max(1, (max(0, min(len, table_tokens)) + unit_tokens - 1) / unit_tokens) * per;
+      u = max(1, (max(0, min(len, table_tokens)) + unit_tokens - 1) >> unit_shift) * per;
     }
     int sum = u;
 #pragma unroll
@@ -936,6 +959,7 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
     __syncthreads();
   }
   const int share = (total + gridDim.x - 1) / gridDim.x;
+  const Divisor by_share(share), by_group(p.group);
   int unit = min(total, (int)blockIdx.x * share);
   const int unit_end = min(total, unit + share);
 
@@ -953,12 +977,13 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
   constexpr int Q4 = C::D / 4;
   constexpr int PART = C::COLS * (C::D + 2);                       // floats of a partial result
   auto write = [&](int col, int d, float4 x, float sum) {          // a piece of a row of the result
-    const int r = it.row0 + col, i = r / p.group;
+    int h;
+    const int i = by_group.of(it.row0 + col, h);
     const bool empty = i >= it.n || sum == 0.f;
     const float inv = empty ? 0.f : 1.f / sum;
     uint2 y = make_uint2(pack<T>(x.x * inv, x.y * inv), pack<T>(x.z * inv, x.w * inv));
     if (empty) y = make_uint2(0, 0);
-    *reinterpret_cast<uint2*>((T*)p.out.p + it.seq * p.out.st.b + (it.head * p.group + r % p.group) * p.out.st.h + i * p.out.st.s + d) = y;
+    *reinterpret_cast<uint2*>((T*)p.out.p + it.seq * p.out.st.b + (it.head * p.group + h) * p.out.st.h + i * p.out.st.s + d) = y;
   };
   int i0 = 0, i1 = 0;                                              // CTAs that share the item
   while (unit < unit_end) {
@@ -972,16 +997,16 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
     it.seq = lo;
     it.full = bt.seq_lens[lo];
     it.len = max(0, min(it.full, table_tokens));
-    const int units = max(1, (it.len + unit_tokens - 1) / unit_tokens);
-    const int within = unit - prefix[lo], index = within / units, start = within % units;
+    const int units = max(1, (it.len + unit_tokens - 1) >> unit_shift);
+    int start;
+    const int within = unit - prefix[lo], index = Divisor(units).of(within, start);
     const int item_first = unit - start;
     it.unit1 = item_first + units;
     const int stop = min(unit_end, it.unit1);
-    it.head = index % c.kv_heads;
-    it.row0 = index / c.kv_heads * C::COLS;
+    it.row0 = Divisor(c.kv_heads).of(index, it.head) * C::COLS;
     it.n = bt.new_lens ? min(max(bt.new_lens[lo], 0), bt.new_tokens) : bt.new_tokens;
     {
-      const int i0 = it.row0 / p.group, i1 = min((it.row0 + C::COLS - 1) / p.group, it.n - 1);
+      const int i0 = by_group.of(it.row0), i1 = min(by_group.of(it.row0 + C::COLS - 1), it.n - 1);
       it.first = max(0, min(it.len, it.full - it.n + i0 + 1));
       it.end = i0 <= i1 ? max(0, min(it.len, it.full - it.n + i1 + 1)) : 0;
     }
@@ -1080,7 +1105,7 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
     };
     // the queries and the pages of the first tiles on their way together: one after the other they took 5 us under load
     Queries<C> queries;
-    queries.load(p, it);
+    queries.load(p, it, by_group);
     int first_pages[C::STAGES - 1][C::MT];
 #pragma unroll
     for (int s = 0; s < C::STAGES - 1; ++s) fetch(first_pages[s]);
@@ -1090,7 +1115,7 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
       if (s < mine) issue(s, tok0 + warp * C::TILE + s * C::UNIT, first_pages[s]);
       copy_commit();
     }
-    queries.put(p, it, frag, qsum, factor, limit);
+    queries.put(p, it, by_group, frag, qsum, factor, limit);
     w.start();
     __syncthreads();
     int slot = 0, t0 = tok0 + warp * C::TILE;
@@ -1116,8 +1141,8 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
     w.put(sums + warp * C::COLS * C::OROW, refs + warp * C::COLS, weights + warp * C::COLS);
     __syncthreads();
 
-    i0 = item_first / share;
-    i1 = (it.unit1 - 1) / share;
+    i0 = by_share.of(item_first);
+    i1 = by_share.of(it.unit1 - 1);
     const int cols = min(C::COLS, bt.new_tokens * p.group - it.row0);
     float* const part = p.partials + ((int64_t)blockIdx.x * 2 + ((int)blockIdx.x == i0)) * PART;
     for (int e = tid; e < cols * Q4; e += C::THREADS) {
@@ -1295,7 +1320,8 @@ int launch(AttnArgs p, void* workspace, bool measure, int64_t* bytes, cudaStream
   }
   if (!fits) { set_error("paged attention: a pool of more than 64 GiB (params: 16 GiB)"); return PBS_ERR_SHAPE; }
   p.counters = (unsigned*)workspace;
-  const bool splits = (int64_t)p.a.b.max_pages * p.a.c.page_size > C::UNIT;    // an item may be long enough for several CTAs
+  // an item may be long enough for several CTAs
+  const bool splits = (int64_t)p.a.b.max_pages * p.a.c.page_size > (C::BITS == 8 ? kWhole : 1) * C::UNIT;
   p.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
   p.drop_arrive = g_drop_arrive.load(std::memory_order_relaxed);
   p.partials = (float*)((uint8_t*)workspace + PBS_PAGED_COUNTER_BYTES);
