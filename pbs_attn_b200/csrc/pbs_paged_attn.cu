@@ -1,4 +1,4 @@
-// Causal attention of new tokens over a paged cache of 16 or 4 bits: out = softmax(scale q K^T) V in one pass over the cache.
+// Causal attention of new tokens over a paged cache of 16, 8 or 4 bits: out = softmax(scale q K^T) V in one pass over the cache.
 //
 // Mathematics.  With values of 4 bits K = lo + code * step (step and lo per token and group g of channels)
 //   q . k_t  =  sum_g  step_{t,g} (q_g . code_{t,g})  +  lo_{t,g} sum(q_g)
@@ -8,7 +8,13 @@
 // tensor cores multiply exactly.  A word of eight codes costs four ANDs and a shift to become four operand registers, and the factors
 // 2^24 and 1/16 go into the queries and the final sums.
 //
-// What bounds it: the cache is read once, (D + 8 D / G) bytes a token and KV head in 4 bits, and a step of the batch has few queries a
+// With values of 8 bits K = code * scale, V too (a scale for a block of 16 to 64 tokens, so one for the 16 of a product)
+//   q . k_t  =  scale_t (q . code_t),        o_d  =  sum_t (p_t scale_t) code_{t,d}.
+// K's codes go into the tensor cores as the bytes that they are, m16n8k32, against queries of two bytes (high and low, two products whose sum
+// is that of integers): nothing is unpacked.  V's codes must meet weights, which have no two bytes' range, so a byte plus 128, a subnormal
+// fp16 number by its bits, meets fp16 weights, and one more product of 128 and the weights, for all channels, is what the sums are less.
+//
+// What bounds it: the cache is read once, 2 D bytes a token and KV head in 8 bits and (D + 8 D / G) in 4, and a step of the batch has few queries a
 // head, so HBM bounds long caches and latency short ones.  Tokens are the rows (M) of both products and the queries of a KV head the
 // columns (N = 8 NT), because a group of 8 or fewer queries then fills an m16n8k16 product; with queries as rows half of it would be
 // padding.  mma.sync and not tcgen05: the operand that changes is unpacked in registers, tcgen05 would take it back through shared
@@ -25,7 +31,9 @@
 // instructions for 32 tokens, half of them on the ALU pipe.)  One sequence of 131072: 41 us, 3.7 TB/s; of 32768 with 4 KV heads: 13 us.  Several
 // queries a head make it arithmetic: 20 (64 sequences of up to 4096) run at 25 % of the copy rate, 32 (8 of up to 8192) at 15; 8 heads of 64
 // channels at 38, two of 256 at 30.  Pages of 16 bits, 64 sequences of up to 4096: 121 us for 0.8 GB, the copy rate, under load too; one of
-// 131072: 89 us, 92 %; 20 queries a head, 8 of up to 8192: 40 us, 64 %.
+// 131072: 89 us, 92 %; 20 queries a head, 8 of up to 8192: 38 us, 67 %.  8 bits, 64 sequences of 12000 to 16384: 328 us for 1.86 GB, 86 % of the
+// copy rate, 336 under load (318 instructions for 16 tokens; with both products in fp16, codes less 1152 by an instruction each, 429, 327 us and 386
+// under load); one of 131072: 56 us, 73 %; 64 of 2000 to 4096: 75 us, 81 %; 16 of 2000 to 4096 with 8, 16 and 32 queries a head 52, 39 and 27 %.
 //
 // Within a CTA every warp takes every eighth (fourth) tile of 16 or 32 tokens through its own ring of cp.async stages, with its own running
 // reference and sums; warps meet once an item.
@@ -60,7 +68,8 @@ struct Cfg {
   static constexpr int PROW = BITS == 4 ? 4 * NG : 0;
   static constexpr int SCALES = BITS == 8 ? 16 : 0;                // bytes of a tile's scales: of keys and of values, for each 16 tokens
   static constexpr int STAGE = TILE * 2 * (ROW + PROW) + SCALES;
-  static constexpr int OCC = BITS != 16 && NT == 1 && D <= 128 ? 2 : 1;      // CTAs a SM
+  // CTAs a SM: two where registers allow (8 bits, two tiles of queries of 64 channels: 26 us against 31; of 128, spilling a little: no difference)
+  static constexpr int OCC = BITS == 8 ? NT * D <= 128 ? 2 : 1 : BITS == 4 && NT == 1 && D <= 128 ? 2 : 1;
   // (with two CTAs a SM a third stage of 128 channels gained nothing: 64 sequences of 16384 205 us with it, 203 without; and the batch's
   // prefix sums have room)
   static constexpr int BUDGET = (OCC == 2 ? BITS == 8 ? 97 : 96 : 200) * 1024;
@@ -223,6 +232,9 @@ __device__ __forceinline__ void load_params(uint32_t (&w)[C::NG], const uint8_t*
 //         code - 8 then and not on the code (3.1e-4, of which the result's own rounding is 2.1e-4);
 //   bf16: every kShiftEvery tiles the sums are moved by what one of each group's has come to, and that is kept aside (1.7e-3, the result's
 //         own rounding).  The other way costs 10 % of the time where it goes into arithmetic, this one 1.
+//
+// 8 bits: every kShiftEvery tiles the sums are made less what 128 and the weights, as they were rounded, have come to: what is left is that of the
+// codes, and rounded weights act on code and not on code + 128.  Within eight tiles the larger sums cost 2^-15 of a code.
 //
 // In bf16 a minimum may be much larger than any step (a group of equal values has none), up to 2^128, and 32 bits hold its products with weights if
 // it counts as a step of 2^-64 of it: they stay below 2^79.

@@ -5,7 +5,9 @@
 // group, reads what it needs of the rows that are continued, and only then writes: no buffer, no barrier, no order among threads.
 //
 // Bound by HBM: what moves is read once and written once.  One launch for up to kLayers layers; a CTA takes a group's keys or values of one head
-// in some of them, and looks up once what moves.
+// in some of them, and looks up once what moves.  32 layers of 8 KV heads of 128, pages of 64 tokens half full, half of the rows moving: 8 groups of
+// four in 16 bits 27.6 us for 134 MB (74 % of the copy rate), 32 of eight 167 us (98 %); one of four in 8 bits 7.0 us.  (Divisions by the units of a
+// page and four rows' pieces in registers whatever the number that moves, one CTA a SM: 65 us.)
 #include <climits>
 
 #include "pbs_paged.cuh"
