@@ -10,7 +10,7 @@ from . import _cabi
 from .decode import _workspace
 from .prefill import _DTYPES
 
-MAX_BEAMS, MAX_KEEP, MAX_BATCH = 32, 64, 1024
+MAX_BEAMS, MAX_KEEP, MAX_BATCH, MAX_VOCAB = 32, 64, 1024, 1 << 30
 _host = None
 _addresses: tuple = ()
 
@@ -46,6 +46,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, keep: Optional[int] 
     keep = 2 * N if keep is None else int(keep)
     if N < 1 or keep < 1:
         raise ValueError(f"{N} beams, keep={keep}: at least one of each is needed")
+    if B > MAX_BATCH or N > MAX_BEAMS or keep > MAX_KEEP or logits.shape[1] > MAX_VOCAB:
+        raise _cabi.PbsError(f"beam selection: {B} entries of {N} beams of {logits.shape[1]} tokens, keep={keep}: up to {MAX_BATCH}, {MAX_BEAMS}, {MAX_VOCAB} and {MAX_KEEP}")
     out = tuple(torch.empty(B, keep, dtype=dt, device=logits.device) for dt in (torch.float32, torch.int32, torch.int64))
     if B == 0:
         return out

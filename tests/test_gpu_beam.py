@@ -182,7 +182,7 @@ def test_refusals():
     logits, scores = _logits(2, 3, 50, torch.bfloat16)
     for error, args in ((TypeError, (logits.double(), scores)), (TypeError, (logits, scores.double())), (ValueError, (logits, scores[:1])), (ValueError, (logits, scores[0])),
                         (ValueError, (logits.t(), scores)), (ValueError, (logits, scores, 0)), (RuntimeError, (logits.cpu(), scores.cpu())), (TypeError, (logits, scores.cpu())),
-                        (ValueError, (logits[None], scores)), (_cabi.PbsError, (logits, scores, 65)), (_cabi.PbsError, (logits[:, :3], scores, 10)),
+                        (ValueError, (logits[None], scores)), (_cabi.PbsError, (logits, scores, 65)), (_cabi.PbsError, (logits, scores, 2 ** 32 + 4)), (_cabi.PbsError, (logits[:, :3], scores, 10)),
                         (_cabi.PbsError, (logits[:, :0], scores, 1)), (_cabi.PbsError, (logits.expand(6, 50)[:1].expand(33, 50), scores.new_zeros(1, 33), 4)),
                         (_cabi.PbsError, (logits[:1].expand(1025, 50), scores.new_zeros(1025, 1), 4)), (ValueError, (logits[:0], scores.new_zeros(2, 0)))):
         with pytest.raises(error):
