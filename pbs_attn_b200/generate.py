@@ -121,7 +121,7 @@ class _Beams:
     def __init__(self, input_ids: torch.Tensor, steps: int, beams: int, ends: Sequence[int], length_penalty: float):
         B, S = input_ids.shape
         device = input_ids.device
-        self.N, self.S, self.power = beams, S, length_penalty
+        self.N, self.S, self.power = beams, S, float(length_penalty)
         self.keep = beams * (1 + len(ends))                # (so many that N go on where each beam may end in every way)
         self.ends = torch.tensor(ends, device=device) if ends else None
         self.pad = ends[0] if ends else 0

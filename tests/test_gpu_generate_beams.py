@@ -91,6 +91,15 @@ def test_masks_reach_every_beam():
     assert ((out >= 100) & (out < 104)).all()
 
 
+def test_whole_numbers_as_length_penalties():
+    from pbs_attn_b200.generate import generate
+    model = _patched(_model())
+    ids = torch.randint(0, 300, (1, 40), device="cuda")
+    kw = dict(num_beams=3, eos_token_id=list(range(0, 60, 6)))
+    for power in (-1, 0, 2):
+        assert torch.equal(generate(model, ids, 8, length_penalty=power, **kw), generate(model, ids, 8, length_penalty=float(power), **kw))
+
+
 def test_refusals():
     from pbs_attn_b200.generate import generate
     model = _patched(_model())
