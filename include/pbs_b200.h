@@ -361,7 +361,7 @@ int pbs_paged_gather(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* ba
  * the largest of a query's row counts as 0) and |v| from 2^-80 to 2^100; in both types, a group of channels whose steps are 2^20 below
  * those of another group of the head loses bits, and one 2^30 below it counts as its minima.
  * What a row does not see does not reach it, infinities and NaNs included: its bits do not change with the values of tokens behind it or
- * of other sequences.  They may with the batch, the lengths in it, the table's width, the number of new tokens and the GPU, which decide
+ * of other sequences (8 bits: as the cache holds them; appending a token behind it may change the scale of a block that it sees).  They may with the batch, the lengths in it, the table's width, the number of new tokens and the GPU, which decide
  * where a sequence is cut and in what order its sums are added; with all of these alike they are the same every time.
  * The blocks of the kernel wait for one another (it is launched cooperatively) where a sequence may be worked on by several.
  * workspace: pbs_paged_attn_workspace bytes, the first PBS_PAGED_COUNTER_BYTES of them 0 before the first call (each call leaves

@@ -394,7 +394,7 @@ struct Warp {
   // What the weights of tokens meet, for the largest of their steps and minima; at least `least`, for weights to stay below 2^85.
   static __device__ __forceinline__ constexpr float least() { return C::DT == PBS_BF16 ? 0x1p-70f : 0x1p-40f; }
   static __device__ __forceinline__ float met(uint32_t w) {
-    if constexpr (C::BITS == 8) return fmaxf(__uint_as_float(w), least());
+    if constexpr (C::BITS == 8) return fmaxf(fabsf(__uint_as_float(w)), least());
     if constexpr (C::DT == PBS_BF16) return fmaxf(fmaxf(step_of<T>(w), low_of<T>(w) * 0x1p-64f), least());
     else return fmaxf(step_of<T>(w), least());
   }
@@ -937,8 +937,9 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
   int unit_tokens = C::UNIT;
   const int own_len = tid < bt.batch ? bt.seq_lens[tid] : 0;       // (of up to THREADS sequences all that is read of the lengths here)
   if constexpr (C::BITS == 8) {
-    bool any = own_len > kWhole * C::UNIT;
-    for (int b = tid + C::THREADS; b < bt.batch; b += C::THREADS) any = any || bt.seq_lens[b] > kWhole * C::UNIT;
+    // (as far as their rows of the table go: with a table that short the CTAs are not launched to wait for one another, so nothing may be split)
+    bool any = min(own_len, table_tokens) > kWhole * C::UNIT;
+    for (int b = tid + C::THREADS; b < bt.batch; b += C::THREADS) any = any || min(bt.seq_lens[b], table_tokens) > kWhole * C::UNIT;
     if (!__syncthreads_or(any)) unit_tokens = kWhole * C::UNIT;
   }
   const int unit_shift = __ffs(unit_tokens) - 1;

@@ -313,7 +313,7 @@ __device__ __forceinline__ Block block_of(const AppendArgs& p, int u, int blocks
 // A block's scale with new tokens of magnitudes up to `most` in it; old: of the tokens that it holds, 0 for none.
 __device__ __forceinline__ float scale_of(float most, float old) {
   const float scale = most <= 3.402823466e38f ? fmaxf(__fmul_rn(most, 1.f / 127.f), kLeastScale) : CUDART_NAN_F;
-  return max_nan(scale, old);
+  return max_nan(scale, fabsf(old));                       // (a pool that was not filled here may have negative ones)
 }
 
 __device__ __forceinline__ uint2 scaled8(const uint2& w, float ratio) {
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 4) paged_gather_kernel(const __grid_
           x[j] = a[j] * scale;
           x[j + 4] = b[j] * scale;
         }
-        if (127.f * scale > most) {                        // (a key that the rotation made larger than fp16 holds)
+        if (127.f * fabsf(scale) > most) {                        // (a key that the rotation made larger than fp16 holds)
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[j] = fminf(fmaxf(x[j], -most), most);
         }

@@ -42,7 +42,7 @@ def append8(cache, codes, scales, x, table, lens, new):
             scale = torch.where(most.isfinite(), scale, math.nan)
             if a > t0:
                 old = scales[page, :, slot // bs].clone()
-                scale = torch.where(old.isnan() | scale.isnan(), math.nan, torch.maximum(scale, old))
+                scale = torch.where(old.isnan() | scale.isnan(), math.nan, torch.maximum(scale, old.abs()))
                 ratio = (old / scale).double()[:, None, None]
                 kept = codes[page, :, slot:slot + a - t0]
                 codes[page, :, slot:slot + a - t0] = torch.where(ratio.isnan(), kept.double(), (kept.double() * ratio).round()).to(torch.int8)
@@ -56,7 +56,7 @@ def values8(cache, codes, scales, table, b, n):
     t = torch.arange(n, device="cuda")
     page, slot = table[b].long()[t // cache.page_size], t % cache.page_size
     scale = scales[page, :, slot // cache.block_size].double()
-    return torch.einsum("thd,th->htd", codes[page, :, slot].double(), scale), 127 * (scale.amax(0) if n else scale.sum(0))
+    return torch.einsum("thd,th->htd", codes[page, :, slot].double(), scale), 127 * (scale.abs().amax(0) if n else scale.sum(0))
 
 
 def attention8(q, cache, table, lens, new=None, scale=None):

@@ -218,6 +218,46 @@ def test_pages_that_are_not_there():
     assert_within(got, *attention8(q, cache, want, [84]))
 
 
+def test_lengths_beyond_a_short_table_split_nothing():
+    """Sequences of a table of two units are not split, so no CTA waits for another, whatever the lengths say."""
+    from pbs_attn_b200 import _cabi
+    from pbs_attn_b200.decode import paged_attn_fwd
+    q, cache, table = _case([256, 100], ps=64)
+    assert table.shape[1] == 4
+    lib = _cabi.load()
+    try:
+        lib.pbs_debug_set_attn_wait(5_000_000, 1)          # 5 ms, and one would not arrive
+        got = paged_attn_fwd(q, cache, table, ints(300, 100))
+        torch.cuda.synchronize()
+    finally:
+        lib.pbs_debug_set_attn_wait(0, 0)
+    with pytest.raises(_cabi.PbsError, match="longer than its row"):
+        cache.check_status()
+    assert_within(got, *attention8(q, cache, table, [256, 100]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_negative_scales_of_a_pool_that_was_filled_elsewhere(dtype):
+    from pbs_attn_b200.decode import paged_kv_append, paged_kv_gather
+    lens = [333, 40]
+    q, cache, table = _case(lens, dtype=dtype, ps=32)
+    want = paged_kv_gather(cache, table, ints(*lens), 333)
+    for codes, scales in ((cache.k, cache.k_params), (cache.v, cache.v_params)):
+        scales[:, :, ::2] *= -1
+        codes[:, :, :16] *= -1
+    assert all(torch.equal(a, b) for a, b in zip(want, paged_kv_gather(cache, table, ints(*lens), 333)))
+    _run(q, cache, table, lens)
+    # larger tokens behind the others of a block whose scale is negative
+    lens, new = [335, 42], 100 * torch.ones(2, 2, 2, 128, dtype=dtype, device="cuda")
+    before = want[0][1, :, -8:].double()                    # tokens 32 .. 39
+    paged_kv_append(cache, new, new, table, ints(*lens))
+    got = paged_kv_gather(cache, table, ints(*lens), 10)[0][1].double()
+    step = cache.k_params[table[1, 1].long(), :, 0].double()
+    assert (step > 0).all() and ((got[:, :8] - before).abs() <= step[:, None, None] * 0.51 + before.abs() * 2.0 ** -7).all()
+    assert ((got[:, 8:] - 100).abs() <= step[:, None, None] * 0.51 + 100 * 2.0 ** -8).all()
+    _run(q, cache, table, lens)
+
+
 def test_same_bits_through_python_and_again(monkeypatch):
     from pbs_attn_b200.decode import paged_attn_fwd, paged_kv_append, paged_kv_gather
     lens = [3000, 17]
