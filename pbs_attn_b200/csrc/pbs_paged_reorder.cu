@@ -6,8 +6,9 @@
 //
 // Bound by HBM: what moves is read once and written once.  One launch for up to kLayers layers; a CTA takes a group's keys or values of one head
 // in some of them, and looks up once what moves.  32 layers of 8 KV heads of 128, pages of 64 tokens half full, half of the rows moving: 8 groups of
-// four in 16 bits 27.6 us for 134 MB (74 % of the copy rate), 32 of eight 167 us (98 %); one of four in 8 bits 7.0 us.  (Divisions by the units of a
-// page and four rows' pieces in registers whatever the number that moves, one CTA a SM: 65 us.)
+// four in 16 bits 26.4 us for 134 MB (77 % of the copy rate), 32 of eight 156 us; one of four in 8 bits 4.9 us.  (Divisions by the units of a page and
+// four rows' pieces in registers whatever the number that moves, one CTA a SM: 65 us.  72 registers, three CTAs a SM, each taking twice as much:
+// 27.6, 166 and 7.0; 48 registers, five: 32, 156 and 6.3.)
 #include <climits>
 
 #include "pbs_paged.cuh"
@@ -69,7 +70,7 @@ __device__ __forceinline__ void copy(const Move* moves, int count, int layers, i
 }
 
 template <int MAXN>
-__global__ void __launch_bounds__(kThreads) paged_reorder_kernel(const __grid_constant__ ReorderArgs p) {
+__global__ void __launch_bounds__(kThreads, MAXN == 8 ? 4 : 1) paged_reorder_kernel(const __grid_constant__ ReorderArgs p) {
   const pbs_paged_cache_t& c = p.a.c;
   const int head = blockIdx.x >> 1, is_v = blockIdx.x & 1, group = blockIdx.y, tid = threadIdx.x;
   const int layer0 = blockIdx.z * p.layers_cta, layers = min(p.layers_cta, p.layers - layer0);
@@ -172,8 +173,8 @@ int launch_paged_reorder(const PagedArgs& a, const pbs_paged_cache_t* const* cac
       const pbs_paged_cache_t& c = *caches[l0 + l];
       p.pools[l] = Pools{(uint8_t*)c.k, (uint8_t*)c.v, (uint8_t*)c.k_params, (uint8_t*)c.v_params};
     }
-    // as many CTAs as it takes to fill the SMs some times over
-    const int64_t ctas = (int64_t)p.layers * groups * 2 * a.c.kv_heads, fill = (int64_t)device_sms() * 8;
+    // as many CTAs as it takes to fill the SMs some times over (four of the common kind run on each at a time)
+    const int64_t ctas = (int64_t)p.layers * groups * 2 * a.c.kv_heads, fill = (int64_t)device_sms() * 16;
     p.layers_cta = (int)((ctas + fill - 1) / fill);
     if (p.layers_cta > p.layers) p.layers_cta = p.layers;
     PBS_TRY(n <= 8 ? launch<8>(p, groups, st) : n <= 16 ? launch<16>(p, groups, st) : launch<kMaxBeams>(p, groups, st));
