@@ -7,7 +7,7 @@
 //
 // HBM bounds prompts, latency and the launch single tokens.  8191 tokens of 8 KV heads into 4 bits: 15 us (33.5 MB read, 9.4 MB written, 2.9
 // TB/s; 75 % of the issue slots are taken: some 170 instructions for eight channels), back out 11 us; 64 sequences' next tokens, 32 query
-// heads rotated, 2.5 us.  Into 8 bits 12.0 us (50 MB, 4.2 TB/s, 64 %: the last of 1024 CTAs on 592 places) and back 9.0 (86 %); one token 2.6 us,
+// heads rotated, 2.5 us.  Into 8 bits 11.5 us (50 MB, 4.4 TB/s, 67 %: instruction issue and the last CTAs) and back 9.0 (86 %); one token 2.6 us,
 // 64 sequences' 3.0, with drafts of up to four 3.2.
 #include <climits>
 #include <type_traits>
@@ -328,13 +328,16 @@ __device__ __forceinline__ uint2 scaled8(const uint2& w, float ratio) {
   return codes8(y, ratio);
 }
 
-// Prompts: a warp takes 16 tokens of a block, blocks of 32 and 64 are several warps'.
+constexpr int kPrompt = 128;
+
+// Prompts: a warp takes 16 tokens of a block, blocks of 32 and 64 are several warps'.  Four warps a CTA, ten CTAs a SM: 11.5 us for 8191 tokens, 11.1 in
+// blocks of 64, 12.3 of 64 channels (eight warps, four CTAs: 11.7, 12.7 and 13.5; twelve CTAs, spilling: 14.3, 12.7 and 11.8).
 template <int DT, int D, int W, bool ROPE>
-__global__ void __launch_bounds__(kThreads, D == 256 ? ROPE ? 1 : 2 : ROPE ? 2 : 4) paged_append8_kernel(const __grid_constant__ AppendArgs p, int blocks, int units) {
+__global__ void __launch_bounds__(kPrompt, D == 256 ? ROPE ? 2 : 4 : ROPE ? 4 : 10) paged_append8_kernel(const __grid_constant__ AppendArgs p, int blocks, int units) {
   using T = typename Elem<DT>::T;
   constexpr int LPR = D / 8, RPI = 32 / LPR, NI = 16 / RPI;  // lanes a row; rows at a time, and times, of a warp's 16
   const pbs_paged_cache_t& c = p.a.c;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, col = lane % LPR, unit = (int)blockIdx.x * (kThreads / 32 / W) + warp / W;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, col = lane % LPR, unit = (int)blockIdx.x * (kPrompt / 32 / W) + warp / W;
   Block b{};
   if (unit < units) b = block_of(p, unit, blocks);
   const int t0 = b.begin + warp % W * 16 + lane / LPR;     // this lane's first token, RPI apart
@@ -374,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? ROPE ? 1 : 2 : ROPE ? 2 :
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
   if constexpr (W > 1) {
-    __shared__ float meet[kThreads / 32];
+    __shared__ float meet[kPrompt / 32];
     if (lane == 0) meet[warp] = most;
     __syncthreads();                                       // (old scales have been read, too)
     most = meet[warp / W * W];
@@ -627,10 +630,10 @@ int launch_append8(AppendArgs p, cudaStream_t st) {
     return PBS_OK;
   }
   auto prompt = [&](auto warps) {
-    constexpr int W = decltype(warps)::value, UPC = kThreads / 32 / W;
+    constexpr int W = decltype(warps)::value, UPC = kPrompt / 32 / W;
     const unsigned ctas = (unsigned)((units + UPC - 1) / UPC);
-    if (p.cosp) paged_append8_kernel<DT, D, W, true><<<ctas, kThreads, 0, st>>>(p, (int)blocks, (int)units);
-    else paged_append8_kernel<DT, D, W, false><<<ctas, kThreads, 0, st>>>(p, (int)blocks, (int)units);
+    if (p.cosp) paged_append8_kernel<DT, D, W, true><<<ctas, kPrompt, 0, st>>>(p, (int)blocks, (int)units);
+    else paged_append8_kernel<DT, D, W, false><<<ctas, kPrompt, 0, st>>>(p, (int)blocks, (int)units);
   };
   if (bs == 16) prompt(std::integral_constant<int, 1>());
   else if (bs == 32) prompt(std::integral_constant<int, 2>());
