@@ -1037,20 +1037,21 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
     int page[C::MT];
     uint32_t holes = 0;                                            // 16 tokens without a page: bit (place in the ring) * MT + m
     int next = tok0 + warp * C::TILE;                              // first token of the tile whose pages are fetched next
-    auto lookup = [&](int t) {
-      if (t >= tok1) return -1;
-      const int x = table[t >> p.a.shift];
-      if ((unsigned)x < (unsigned)c.num_pages) return x;
-      paged_fault(p.a, PBS_PAGED_BAD_PAGE);
-      return -1;
-    };
-    auto fetch = [&](int (&page)[C::MT]) {                         // pages of the next tile
+    auto lookup = [&](int t) { return t < tok1 ? table[t >> p.a.shift] : -1; };
+    auto fetch = [&](int (&page)[C::MT]) {                         // pages of the next tile, which issue() looks at, so that nothing waits for them here
       page[0] = lookup(next);
       if constexpr (C::MT == 2) page[1] = p.a.shift > 4 ? page[0] : lookup(next + 16);   // (tiles start at multiples of 32)
       next += C::UNIT;
     };
-    auto issue = [&](int slot, int t0, const int (&page)[C::MT]) { // the copies of a tile, to this place in the ring, once its pages are here
+    auto issue = [&](int slot, int t0, const int (&fetched)[C::MT]) {        // the copies of a tile, to this place in the ring, once its pages are here
       const uint32_t at = ring_at + slot * C::STAGE;
+      int page[C::MT];
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m) {
+        const bool there = (unsigned)fetched[m] < (unsigned)c.num_pages;
+        if (!there && t0 + 16 * m < tok1) paged_fault(p.a, PBS_PAGED_BAD_PAGE);
+        page[m] = there ? fetched[m] : -1;
+      }
       if constexpr (C::BITS == 8) {                                // scales: a lane one
         const int m = lane >> 1, pg = C::MT == 2 && m == 1 ? page[C::MT - 1] : page[0], first = t0 + 16 * m;
         if (m < C::MT && pg >= 0 && first < tok1) {
