@@ -350,6 +350,7 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_select_kernel(const 
   __shared__ int listed, last;
   __shared__ double norm[kMaxBeams];                       // of a beam: its score, less the logarithm of its sum
   __shared__ float peak[kMaxBeams];
+  after_the_kernel_before();
   const pbs_beam_select_t& a = p.a;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, K = a.keep;
   const int r = blockIdx.x / p.slices, entry = r / a.beams;
@@ -616,7 +617,7 @@ int launch(const pbs_beam_select_t& a, void* workspace, int64_t* bytes, cudaStre
   p.counters = (unsigned*)workspace;
   p.sums = (float2*)((uint8_t*)workspace + PBS_PAGED_COUNTER_BYTES);
   p.lists = (unsigned long long*)(p.sums + ctas);
-  beam_select_kernel<T><<<(unsigned)ctas, kThreads, 0, st>>>(p);
+  PBS_LAUNCH_EARLY("beam_select_kernel", beam_select_kernel<T>, dim3((unsigned)ctas), kThreads, st, p);
   PBS_CUDA_CHECK_LAUNCH("beam_select_kernel");
   return PBS_OK;
 }

@@ -47,6 +47,36 @@ __device__ __forceinline__ int64_t slot_offset(const int64_t (&st)[3], int page,
   return page * st[0] + head * st[1] + slot * st[2];
 }
 
+// The kernels of a step are short, and between two of them in a stream 1 to 2 us pass that no kernel runs in.  So each may be put on the SMs while the one
+// before it ends: it starts by waiting for that one's results (all threads, before anything else), and lets the next be put there in turn.
+// Back to back: selection from four rows 11.2 us a call instead of 13.0, attention of 187 tokens 5.9 instead of 6.8.
+__device__ __forceinline__ void after_the_kernel_before() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+inline cudaLaunchAttribute early_launch() {
+  cudaLaunchAttribute a = {};
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  return a;
+}
+template <class... P, class... A>
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t st, const A&... args) {
+  cudaLaunchAttribute early = early_launch();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.stream = st;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+#define PBS_LAUNCH_EARLY(name, kernel, grid, threads, st, ...)                              \
+  do {                                                                                      \
+    const cudaError_t launched_ = launch_early(kernel, grid, threads, st, __VA_ARGS__);     \
+    if (launched_ != cudaSuccess) return cuda_fail(launched_, name);                        \
+  } while (0)
+
 int launch_paged_append(const PagedArgs& a, const RowTensor& k, const RowTensor& v, int q_heads, const RowTensor& q, const RowTensor& qo,
                         const void* cosp, const void* sinp, int64_t cs_b, int64_t cs_s, int table_rows, cudaStream_t st);
 int launch_paged_gather(const PagedArgs& a, const RowTensor& k, const RowTensor& v, cudaStream_t st);

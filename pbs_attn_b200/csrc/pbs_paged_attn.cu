@@ -930,6 +930,7 @@ __global__ void __launch_bounds__(C::THREADS, C::OCC) paged_attn_kernel(const __
   const pbs_paged_batch_t& bt = p.a.b;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int table_tokens = bt.max_pages << p.a.shift;
+  after_the_kernel_before();
 
   // 8 bits: where all sequences are short (two units at most) a unit is a whole one.  What splitting it saves on a tile goes on joining the parts:
   // 187 tokens take 6.9 us in two units a head, 5.9 in one (500 tokens 7.5 in four, 10.8 in one).
@@ -1356,8 +1357,9 @@ int launch(AttnArgs p, void* workspace, bool measure, int64_t* bytes, cudaStream
   cudaLaunchAttribute together = {};
   together.id = cudaLaunchAttributeCooperative;
   together.val.cooperative = 1;
-  cfg.attrs = &together;
-  cfg.numAttrs = splits ? 1 : 0;
+  cudaLaunchAttribute early = early_launch();
+  cfg.attrs = splits ? &together : &early;
+  cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, paged_attn_kernel<C>, p);
   if (e != cudaSuccess) return cuda_fail(e, "paged_attn_kernel");
   PBS_CUDA_CHECK_LAUNCH("paged_attn_kernel");

@@ -132,6 +132,7 @@ constexpr int kAhead = 2;                                  // rows that a lane h
 
 template <int DT, int D, int BITS, int G>
 __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(const __grid_constant__ AppendArgs p, int tokens) {
+  after_the_kernel_before();
   using T = typename Elem<DT>::T;
   constexpr int LPR = D / 8;                               // lanes a row
   const pbs_paged_cache_t& c = p.a.c;
@@ -334,6 +335,7 @@ constexpr int kPrompt = 128;
 // blocks of 64, 12.3 of 64 channels (eight warps, four CTAs: 11.7, 12.7 and 13.5; twelve CTAs, spilling: 14.3, 12.7 and 11.8).
 template <int DT, int D, int W, bool ROPE>
 __global__ void __launch_bounds__(kPrompt, D == 256 ? ROPE ? 2 : 4 : ROPE ? 4 : 10) paged_append8_kernel(const __grid_constant__ AppendArgs p, int blocks, int units) {
+  after_the_kernel_before();
   using T = typename Elem<DT>::T;
   constexpr int LPR = D / 8, RPI = 32 / LPR, NI = 16 / RPI;  // lanes a row; rows at a time, and times, of a warp's 16
   const pbs_paged_cache_t& c = p.a.c;
@@ -423,6 +425,7 @@ constexpr int kFew = 4;                                    // rows of a lane
 // The CTAs behind kv_ctas turn queries.
 template <int DT, int D, bool ROPE>
 __global__ void __launch_bounds__(kThreads) paged_append8_few_kernel(const __grid_constant__ AppendArgs p, int blocks, int units, int kv_ctas) {
+  after_the_kernel_before();
   using T = typename Elem<DT>::T;
   constexpr int LPR = D / 8, RPI = 32 / LPR;
   if (ROPE && (int)blockIdx.x >= kv_ctas) {
@@ -494,6 +497,7 @@ __global__ void __launch_bounds__(kThreads) paged_append8_few_kernel(const __gri
 
 template <int DT, int D, int BITS, int G>
 __global__ void __launch_bounds__(kThreads, 4) paged_gather_kernel(const __grid_constant__ AppendArgs p, int tokens) {
+  after_the_kernel_before();
   using T = typename Elem<DT>::T;
   constexpr int LPR = D / 8;
   const pbs_paged_cache_t& c = p.a.c;
@@ -597,7 +601,7 @@ dim3 deal(AppendArgs& p) {
 template <int DT, int D, int BITS, int G>
 int launch_gather(AppendArgs p, cudaStream_t st) {
   const dim3 grid = deal<D>(p);
-  paged_gather_kernel<DT, D, BITS, G><<<grid, kThreads, 0, st>>>(p, p.a.b.batch * p.a.b.new_tokens);
+  PBS_LAUNCH_EARLY("paged_gather_kernel", (paged_gather_kernel<DT, D, BITS, G>), grid, kThreads, st, p, p.a.b.batch * p.a.b.new_tokens);
   PBS_CUDA_CHECK_LAUNCH("paged_gather_kernel");
   return PBS_OK;
 }
@@ -606,7 +610,7 @@ template <int DT, int D, int BITS, int G>
 int launch(AppendArgs p, bool gather, cudaStream_t st) {
   if (gather) return launch_gather<DT, D, BITS, G>(p, st);
   const dim3 grid = deal<D>(p);
-  paged_append_kernel<DT, D, BITS, G><<<grid, kThreads, 0, st>>>(p, p.a.b.batch * p.a.b.new_tokens);
+  PBS_LAUNCH_EARLY("paged_append_kernel", (paged_append_kernel<DT, D, BITS, G>), grid, kThreads, st, p, p.a.b.batch * p.a.b.new_tokens);
   PBS_CUDA_CHECK_LAUNCH("paged_append_kernel");
   return PBS_OK;
 }
@@ -624,25 +628,26 @@ int launch_append8(AppendArgs p, cudaStream_t st) {
     p.chunk = (int)(chunk < 1 ? 1 : chunk < 8 ? chunk : 8);
     p.q_chunks = (p.q_heads + p.chunk - 1) / p.chunk;
     const unsigned ctas = (unsigned)(kv_ctas + (tokens * p.q_chunks + RPB - 1) / RPB);
-    if (p.cosp) paged_append8_few_kernel<DT, D, true><<<ctas, kThreads, 0, st>>>(p, (int)blocks, (int)units, (int)kv_ctas);
-    else paged_append8_few_kernel<DT, D, false><<<(unsigned)kv_ctas, kThreads, 0, st>>>(p, (int)blocks, (int)units, (int)kv_ctas);
+    if (p.cosp) PBS_LAUNCH_EARLY("paged_append8_few_kernel", (paged_append8_few_kernel<DT, D, true>), ctas, kThreads, st, p, (int)blocks, (int)units, (int)kv_ctas);
+    else PBS_LAUNCH_EARLY("paged_append8_few_kernel", (paged_append8_few_kernel<DT, D, false>), (unsigned)kv_ctas, kThreads, st, p, (int)blocks, (int)units, (int)kv_ctas);
     PBS_CUDA_CHECK_LAUNCH("paged_append8_few_kernel");
     return PBS_OK;
   }
-  auto prompt = [&](auto warps) {
+  auto prompt = [&](auto warps) -> int {
     constexpr int W = decltype(warps)::value, UPC = kPrompt / 32 / W;
     const unsigned ctas = (unsigned)((units + UPC - 1) / UPC);
-    if (p.cosp) paged_append8_kernel<DT, D, W, true><<<ctas, kPrompt, 0, st>>>(p, (int)blocks, (int)units);
-    else paged_append8_kernel<DT, D, W, false><<<ctas, kPrompt, 0, st>>>(p, (int)blocks, (int)units);
+    if (p.cosp) PBS_LAUNCH_EARLY("paged_append8_kernel", (paged_append8_kernel<DT, D, W, true>), ctas, kPrompt, st, p, (int)blocks, (int)units);
+    else PBS_LAUNCH_EARLY("paged_append8_kernel", (paged_append8_kernel<DT, D, W, false>), ctas, kPrompt, st, p, (int)blocks, (int)units);
+    return PBS_OK;
   };
-  if (bs == 16) prompt(std::integral_constant<int, 1>());
-  else if (bs == 32) prompt(std::integral_constant<int, 2>());
-  else prompt(std::integral_constant<int, 4>());
+  if (bs == 16) PBS_TRY(prompt(std::integral_constant<int, 1>()));
+  else if (bs == 32) PBS_TRY(prompt(std::integral_constant<int, 2>()));
+  else PBS_TRY(prompt(std::integral_constant<int, 4>()));
   PBS_CUDA_CHECK_LAUNCH("paged_append8_kernel");
   if (p.q_heads) {                                         // the queries, which cost as much as keys and values, by the kernel that is made for them
     dim3 grid = deal<D>(p);
     grid.y = p.q_chunks;
-    paged_append_kernel<DT, D, 16, 0><<<grid, kThreads, 0, st>>>(p, (int)tokens);
+    PBS_LAUNCH_EARLY("paged_append_kernel", (paged_append_kernel<DT, D, 16, 0>), grid, kThreads, st, p, (int)tokens);
     PBS_CUDA_CHECK_LAUNCH("paged_append_kernel");
   }
   return PBS_OK;

@@ -71,6 +71,7 @@ __device__ __forceinline__ void copy(const Move* moves, int count, int layers, i
 
 template <int MAXN>
 __global__ void __launch_bounds__(kThreads, MAXN == 8 ? 4 : 1) paged_reorder_kernel(const __grid_constant__ ReorderArgs p) {
+  after_the_kernel_before();
   const pbs_paged_cache_t& c = p.a.c;
   const int head = blockIdx.x >> 1, is_v = blockIdx.x & 1, group = blockIdx.y, tid = threadIdx.x;
   const int layer0 = blockIdx.z * p.layers_cta, layers = min(p.layers_cta, p.layers - layer0);
@@ -149,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, MAXN == 8 ? 4 : 1) paged_reorder_ker
 
 template <int MAXN>
 int launch(const ReorderArgs& p, int groups, cudaStream_t st) {
-  paged_reorder_kernel<MAXN><<<dim3(2 * p.a.c.kv_heads, groups, (p.layers + p.layers_cta - 1) / p.layers_cta), kThreads, 0, st>>>(p);
+  PBS_LAUNCH_EARLY("paged_reorder_kernel", paged_reorder_kernel<MAXN>, dim3(2 * p.a.c.kv_heads, groups, (p.layers + p.layers_cta - 1) / p.layers_cta), kThreads, st, p);
   PBS_CUDA_CHECK_LAUNCH("paged_reorder_kernel");
   return PBS_OK;
 }
