@@ -174,3 +174,55 @@ def test_append_attend_select_and_reorder_together(block):
                     off = (value - own[:, i].transpose(0, 1)).abs() / scale / ((0.5 + 2.0 ** -16) * (block - t % block)[:, None])
                     assert off.max() <= 1, (step, r, i, float(off.max()), (off > 1).nonzero()[:5].tolist())
     caches[0].check_status()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_calls_that_follow_one_another_see_what_the_one_before_wrote(captured):
+    """Kernels are put on the SMs while the one before ends: append, attend, read back, reorder and select on one stream, many times over without a
+    pause, give what they give with a pause after each."""
+    from pbs_attn_b200.beam import beam_select
+    from pbs_attn_b200.decode import PagedKVCache, paged_attn_fwd, paged_kv_append, paged_kv_gather, paged_kv_reorder
+    B, N, H, D, V = 2, 4, 2, 128, 4000
+    g = torch.Generator(device="cuda").manual_seed(21)
+    rows = torch.randn(3, B * N, H, 1, D, generator=g, device="cuda").bfloat16()
+    out = torch.randn(H * D, V, generator=g, device="cuda").bfloat16() / 4
+    results = []
+    for pause in (True, False):
+        cache = PagedKVCache(B * N * 4, 64, H, D, torch.bfloat16, "cuda", bits=8, block_size=16)
+        for t in (cache.k, cache.v, cache.k_params, cache.v_params):
+            t.zero_()
+        table = torch.arange(B * N * 4, dtype=torch.int32, device="cuda").view(B * N, 4)
+        lens, scores = torch.zeros(B * N, dtype=torch.int32, device="cuda"), torch.zeros(B, N, device="cuda")
+        last, back = torch.zeros(B * N, H, 1, D, dtype=torch.bfloat16, device="cuda"), torch.zeros(B * N, H, 1, D, dtype=torch.bfloat16, device="cuda")
+
+        def step():
+            wait = torch.cuda.synchronize if pause else lambda: None
+            lens.add_(1)
+            k, v, q = rows[0] + last, rows[1] - last, rows[2] + last
+            wait()
+            paged_kv_append(cache, k, v, table, lens)
+            wait()
+            o = paged_attn_fwd(q, cache, table, lens)
+            wait()
+            got, _ = paged_kv_gather(cache, table, lens, 1)
+            wait()
+            back.add_(got)
+            s, beams, tokens = beam_select(o.reshape(B * N, H * D) @ out, scores, N)
+            wait()
+            paged_kv_reorder(cache, table, lens, beams)
+            wait()
+            scores.copy_(s - s[:, :1])
+            last.copy_(((tokens % 13).view(-1, 1, 1, 1) / 13 + o).bfloat16())
+
+        step()
+        if captured and not pause:
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                step()
+        for _ in range(150):
+            graph.replay() if captured and not pause else step()
+        torch.cuda.synchronize()
+        cache.check_status()
+        results.append([x.clone() for x in (back, last, scores, table, lens, cache.k, cache.v, cache.k_params)])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
