@@ -5,7 +5,6 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_strided.h>
-#include <ATen/ops/zeros.h>
 
 #include <algorithm>
 #include <cmath>
@@ -91,7 +90,7 @@ struct Space {
   at::Tensor memory;
 };
 
-constexpr size_t kMaxSpaces = 8;
+constexpr int kMaxSpaces = 8;                                      // of a kind, so that one kind takes no other's
 
 // In the order of their last use.  (Never destroyed: the interpreter ends after the allocator that they would go back to.)
 std::vector<Space>& spaces() {
@@ -109,9 +108,17 @@ at::Tensor& space_of(Kind kind, int device, cudaStream_t st, unsigned long long 
     return s.back().memory;
   }
   s.erase(std::remove_if(s.begin(), s.end(), [&](const Space& x) { return x.capture != 0 && x.capture != capture; }), s.end());
-  if (s.size() >= kMaxSpaces) s.erase(s.begin());
+  const auto same = [&](const Space& x) { return x.kind == kind; };
+  if (std::count_if(s.begin(), s.end(), same) >= kMaxSpaces) s.erase(std::find_if(s.begin(), s.end(), same));
   s.push_back(Space{kind, device, st, capture, at::Tensor()});
   return s.back().memory;
+}
+
+// New memory of `need` bytes, its counters 0.  An undefined tensor where that failed.
+at::Tensor new_space(int64_t need, const at::TensorOptions& opt, cudaStream_t st) {
+  at::Tensor t = at::empty({need}, opt.dtype(at::kByte));
+  if (cudaMemsetAsync(t.data_ptr(), 0, PBS_PAGED_COUNTER_BYTES, st) != cudaSuccess) return at::Tensor();
+  return t;
 }
 
 // paged_attn(cache, q, table, lens, new_lens, scale, out): the result, or None
@@ -145,7 +152,8 @@ PyObject* py_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (round == 1 || !space.defined()) {                          // too small, perhaps
       int64_t need = 0;
       if (c->workspace(c->c, &batch, (int32_t)q.size(1), &need) != PBS_OK || (space.defined() && need <= space.numel())) Py_RETURN_NONE;
-      space = at::zeros({need}, at::TensorOptions().dtype(at::kByte).device(at::Device(at::kCUDA, (c10::DeviceIndex)c->device)));
+      space = new_space(need, at::TensorOptions().device(at::Device(at::kCUDA, (c10::DeviceIndex)c->device)), st);
+      if (!space.defined()) Py_RETURN_NONE;
     }
     rc = c->attn(c->c, &batch, (int32_t)q.size(1), q.data_ptr(), q.strides().data(), out.data_ptr(), out.strides().data(), (float)scale,
                  space.data_ptr(), space.numel(), st);
@@ -400,7 +408,8 @@ PyObject* py_beams(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (round == 1 || !space.defined()) {                          // too small, perhaps
       int64_t need = 0;
       if (ws(&g, &need) != PBS_OK || (space.defined() && need <= space.numel())) Py_RETURN_NONE;
-      space = at::zeros({need}, opt.dtype(at::kByte));
+      space = new_space(need, opt, st);
+      if (!space.defined()) Py_RETURN_NONE;
     }
     rc = fn(&g, space.data_ptr(), space.numel(), st);
   }

@@ -315,20 +315,24 @@ def paged_kv_reorder(caches: Union[PagedKVCache, Sequence[PagedKVCache]], block_
 
 # Memory for partial results, one piece a stream and kind of call: calls on a stream come after one another.
 _WORKSPACES: dict = {}
-_MAX_WORKSPACES = 8
+_MAX_WORKSPACES = 8                     # of a kind, so that one kind takes no other's
 
 
 def _workspace(device: torch.device, need: int, kind: str = "attention") -> torch.Tensor:
-    if torch.cuda.is_current_stream_capturing():           # a graph is replayed at times and on streams unknown here: it has its own
+    def make():
         space = torch.empty(need, dtype=torch.uint8, device=device)
         space[:_cabi.PAGED_COUNTER_BYTES].zero_()
         return space
+
+    if torch.cuda.is_current_stream_capturing():           # a graph is replayed at times and on streams unknown here: it has its own
+        return make()
     key = (kind, device.index, torch.cuda.current_stream(device).cuda_stream)
     space = _WORKSPACES.pop(key, None)                     # (back in behind the others: what was used longest ago goes first)
     if space is None or space.numel() < need:
-        while len(_WORKSPACES) >= _MAX_WORKSPACES:
-            _WORKSPACES.pop(next(iter(_WORKSPACES), None), None)
-        space = torch.zeros(need, dtype=torch.uint8, device=device)
+        held = [k for k in list(_WORKSPACES) if k[0] == kind]
+        for k in held[:max(0, len(held) + 1 - _MAX_WORKSPACES)]:
+            _WORKSPACES.pop(k, None)
+        space = make()
     _WORKSPACES[key] = space
     return space
 

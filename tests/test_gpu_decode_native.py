@@ -215,3 +215,30 @@ def test_dense_tensors_between_the_16_byte_boundaries():
     paged_kv_append(cache, past, past, table, lens, new_lens=lens)
     out = shifted(q)
     assert paged_attn(shifted(q), cache, table, lens, out=out) is out and torch.equal(out, paged_attn(q, cache, table, lens))
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_streams_that_attend_and_choose_beams_in_turn_keep_their_memory(native, monkeypatch):
+    """Eight streams, each with memory of both kinds: once they have it, no call allocates any."""
+    from pbs_attn_b200 import beam
+    q, cache, table, lens = _filled()
+    g = torch.Generator(device="cuda").manual_seed(2)
+    logits, scores = torch.randn(4, 3000, generator=g, device="cuda"), torch.zeros(1, 4, device="cuda")
+    if not native:
+        cache._native = None
+        monkeypatch.setattr(beam, "_host", False)
+    want, chosen = paged_attn(q, cache, table, lens), beam.beam_select(logits, scores)
+    torch.cuda.synchronize()
+    streams, outs, count = [torch.cuda.Stream() for _ in range(8)], [], []
+    for _ in range(3):
+        before = torch.cuda.memory_stats()["allocation.all.allocated"]
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append((paged_attn(q, cache, table, lens), beam.beam_select(logits, scores)))
+        count.append(torch.cuda.memory_stats()["allocation.all.allocated"] - before)
+    torch.cuda.synchronize()
+    for o, b in outs:
+        assert torch.equal(o, want) and all(torch.equal(x, y) for x, y in zip(b, chosen))
+    # of each call its result, and three
+    assert count[1:] == [8 * 4, 8 * 4]
+    cache.check_status()
