@@ -188,3 +188,47 @@ def test_refusals():
         with pytest.raises(error):
             beam_select(*args)
     assert beam_select(logits[:0], scores[:0], 4)[0].shape == (0, 4)
+
+
+def _time_of(call, rounds=15):
+    """Median of a call's time on the device, among others."""
+    for _ in range(3):
+        call()
+    times = []
+    for _ in range(rounds):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        torch.cuda.synchronize()
+        start.record()
+        for _ in range(8):
+            call()
+        end.record()
+        end.synchronize()
+        times.append(start.elapsed_time(end))
+    return sorted(times)[rounds // 2]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_first_step_takes_no_longer_than_a_later_one(dtype):
+    """Of beams that are not alive nothing is looked at; what comes out is the order of their tokens."""
+    from pbs_attn_b200.beam import beam_select
+    logits, scores = _logits(64, 8, 100003, dtype, 12)
+    first, dead = scores.clone(), torch.full_like(scores, -math.inf)
+    first[:, 1:] = -math.inf
+    _check(logits, first)
+    got, beams, tokens = _check(logits, dead)
+    assert got.isneginf().all() and (beams == 0).all() and (tokens == torch.arange(16, device="cuda")).all()
+    later = _time_of(lambda: beam_select(logits, scores))
+    assert _time_of(lambda: beam_select(logits, first)) <= later and _time_of(lambda: beam_select(logits, dead)) <= later
+
+
+@pytest.mark.parametrize("N,V,keep", [(1, 5, 5), (1, 64, 64), (4, 3, 12), (2, 4099, 64), (3, 130001, 64)])
+def test_beams_that_are_all_dead(N, V, keep):
+    """The first tokens of the first beams, whatever the logits are, at the ends of segments and of rows that start anywhere."""
+    for dtype in (torch.bfloat16, torch.float32):
+        for shift in (0, 1, 3):
+            memory = torch.full((2 * N * V + 8,), math.nan, dtype=dtype, device="cuda")
+            from pbs_attn_b200.beam import beam_select
+            got, beams, tokens = beam_select(memory[shift:shift + 2 * N * V].view(2 * N, V), torch.full((2, N), -math.inf, device="cuda"), keep)
+            assert got.isneginf().all()
+            place = beams.long() * V + tokens
+            assert torch.equal(place, torch.arange(keep, device="cuda").expand(2, -1))
