@@ -24,7 +24,8 @@ namespace {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int P = 2, kStages = 3;          // 16-byte pieces of a thread in a chunk; chunks in shared memory, all but one of them on their way
 constexpr int kResident = 4;              // CTAs a SM
-constexpr int kListed = 1024;             // logits that reach the bound; more of them at a time are gone through K times instead
+constexpr int kListed = 1024;             // logits that reach the bound; of more the K-th of those that found room is a better bound
+constexpr int kSample = 512;              // of these
 constexpr int kFound = 320;               // continuations that do
 constexpr int kMaxBeams = 32;
 constexpr float kFltMax = 3.402823466e38f;
@@ -144,15 +145,6 @@ struct Piece<__half> {
 
 // What a logit counts as.
 __device__ __forceinline__ float counted(float x) { return x == x ? x : -CUDART_INF_F; }
-
-__device__ __forceinline__ unsigned long long warp_most(unsigned long long x) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long y = __shfl_xor_sync(0xffffffffu, x, o);
-    x = y > x ? y : x;
-  }
-  return x;
-}
 
 // A number that K of the CTA's (one a thread) reach, and few more where warps' numbers are alike: what ceil(K / warps) of every warp do.
 // (Short, and not inlined: in a kernel of this size code that is not there yet takes longer than what it does.  The exact K-th largest, by the places of
@@ -309,31 +301,6 @@ struct Sum {
   }
 };
 
-// The K largest of a segment one after the other, from memory: for the few that hold more large logits in few threads than there is room for.
-template <class T>
-__device__ __noinline__ void largest_one_by_one(const Row<T>& row, int chunk0, int chunk1, int K, unsigned long long* out, unsigned long long* meet) {
-  unsigned long long lower = ~0ull;
-  for (int r = 0; r < K; ++r) {
-    unsigned long long mine = 0;
-    for (int c = chunk0; c < chunk1; ++c)
-      for (int e = 0; e < P * Row<T>::N; ++e) {
-        const int v = row.token(c, e / Row<T>::N, e % Row<T>::N);
-        if (!row.has(v)) continue;
-        const unsigned long long o = ordered(row.one(v), v);
-        if (o < lower && o > mine) mine = o;
-      }
-    mine = warp_most(mine);
-    if (threadIdx.x % 32 == 0) meet[threadIdx.x / 32] = mine;
-    __syncthreads();
-    mine = meet[0];
-#pragma unroll
-    for (int i = 1; i < kWarps; ++i) mine = meet[i] > mine ? meet[i] : mine;
-    if (threadIdx.x == 0) out[r] = mine;
-    lower = mine;
-    __syncthreads();
-  }
-}
-
 template <class T>
 __global__ void __launch_bounds__(kThreads, kResident) beam_select_kernel(const __grid_constant__ BeamArgs p) {
   using E = Piece<T>;
@@ -346,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_select_kernel(const 
   __shared__ Next heads[kWarps];
   __shared__ float2 part[kWarps];
   __shared__ float bounds[kWarps], bounds_of_one[kWarps];
-  __shared__ unsigned long long meet[kWarps];
+  __shared__ unsigned long long kth;
   __shared__ int listed, last;
   __shared__ double norm[kMaxBeams];                       // of a beam: its score, less the logarithm of its sum
   __shared__ float peak[kMaxBeams];
@@ -397,7 +364,8 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_select_kernel(const 
       asm volatile("cp.async.wait_all;" ::: "memory");
       __syncthreads();                                     // (for `listed`, as in bound_of)
     }
-    const int filled = bound == -CUDART_INF_F ? max(chunk0 * R::CHUNK - row.lead, 0) + K : -1;
+    int filled = bound == -CUDART_INF_F ? max(chunk0 * R::CHUNK - row.lead, 0) + K : -1;
+    int tie = INT_MAX;                                     // tokens up to this one reach the bound by being equal to it
     auto enlist = [&](int c, int thread) {                 // a thread's pieces of a chunk
       const bool plain = row.alive && row.inner(c);
       uint4 w[P];
@@ -412,18 +380,20 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_select_kernel(const 
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const int v = row.token(c, k, i, thread);
-          if ((x[i] >= bound && x[i] > -CUDART_INF_F) || (v < filled && c == chunk0)) reach |= row.has(v) ? 1u << (k * N + i) : 0;
+          if ((x[i] >= bound && x[i] > -CUDART_INF_F && (v <= tie || x[i] > bound)) || (v < filled && c == chunk0)) reach |= row.has(v) ? 1u << (k * N + i) : 0;
         }
       }
       for (; reach; reach &= reach - 1) {
-        const int bit = __ffs(reach) - 1, v = row.token(c, bit / N, bit % N, thread), n = atomicAdd(&listed, 1);
-        if (n < kListed) list[n] = ordered(row.one(v), v);
+        const int bit = __ffs(reach) - 1, v = row.token(c, bit / N, bit % N, thread);
+        const int n = atomicAdd(&listed, 1);
+        if (n >= kListed) break;
+        list[n] = ordered(row.one(v), v);
       }
     };
     // (in three or more chunks of a thread: rarely, and then the warp looks through all of them)
     const uint32_t everywhere = __ballot_sync(0xffffffffu, best[2] >= bound && best[2] > -CUDART_INF_F);
     for (uint32_t left = everywhere; left; left &= left - 1)
-      for (int c = chunk0 + lane; c < chunk1; c += 32) enlist(c, warp * 32 + __ffs(left) - 1);
+      for (int c = chunk0 + lane; c < chunk1 && *(volatile int*)&listed <= kListed; c += 32) enlist(c, warp * 32 + __ffs(left) - 1);
     if (!(everywhere >> lane & 1)) {
       const bool fills = row.token(chunk0, 0, 0) < filled;
       if (fills) enlist(chunk0, tid);
@@ -437,20 +407,36 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_select_kernel(const 
     const float wide = warp_max(sum.top), scaled = warp_sum(sum.sum * exp2_fast((sum.top - wide) * kLog2e));
     if (lane == 0) part[warp] = make_float2(wide, scaled);
     __syncthreads();
-    const int n = listed;
-    unsigned long long* const out = p.lists + (int64_t)blockIdx.x * K;
-    if (n <= kListed) {
-      for (int i = tid; i < n; i += kThreads) {
+    // Too many (equal ones, as where a mask is of the lowest finite number, or large ones in few threads' hands): the K-th of some that found room is a
+    // better bound, which so many fewer reach, and of a sample of them a small part.  (512 rows of 152064 with five tokens that are not banned: 274 us,
+    // four to five times as long as usual; gone through once for each of K = 16, as it was, 2820.)
+    while (listed > kListed) {
+      for (int i = tid; i < kSample; i += kThreads) {
         const unsigned long long mine = list[i];
         int at = 0;
 #pragma unroll 4
-        for (int j = 0; j < n; ++j) at += list[j] > mine;
-        if (at < K) out[at] = mine;
+        for (int j = 0; j < kSample; ++j) at += list[j] > mine;
+        if (at == K - 1) kth = mine;
       }
-      for (int i = n + tid; i < K; i += kThreads) out[i] = 0;              // (a segment of fewer tokens)
-    } else {
-      largest_one_by_one(row, chunk0, chunk1, K, out, meet);
+      __syncthreads();
+      bound = value_of((uint32_t)(kth >> 32));
+      tie = (int)~(uint32_t)kth;
+      filled = -1;                                         // (more than K are not -infinity)
+      if (tid == 0) listed = 0;
+      __syncthreads();
+      for (int c = chunk0; c < chunk1; ++c) enlist(c, tid);
+      __syncthreads();
     }
+    const int n = listed;
+    unsigned long long* const out = p.lists + (int64_t)blockIdx.x * K;
+    for (int i = tid; i < n; i += kThreads) {
+      const unsigned long long mine = list[i];
+      int at = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) at += list[j] > mine;
+      if (at < K) out[at] = mine;
+    }
+    for (int i = n + tid; i < K; i += kThreads) out[i] = 0;                // (a segment of fewer tokens)
     if (warp == 1) {
       const float2 x = lane < kWarps ? part[lane] : make_float2(-kFltMax, 0.f);
       const float m = warp_max(x.x), total = warp_sum(x.y * exp2_fast((x.x - m) * kLog2e));

@@ -232,3 +232,25 @@ def test_beams_that_are_all_dead(N, V, keep):
             assert got.isneginf().all()
             place = beams.long() * V + tokens
             assert torch.equal(place, torch.arange(keep, device="cuda").expand(2, -1))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("left", [0, 1, 5, 16, 2000])
+def test_masks_of_the_lowest_finite_number(dtype, left):
+    """More logits that are equal than there is room for, beside the few that are not banned, in long segments and short ones."""
+    for B, N, V, keep in ((64, 8, 20011, 16), (1, 2, 150001, 64), (200, 2, 6000, 33)):
+        logits, scores = _logits(B, N, V, dtype, left, 2.0)
+        g = torch.Generator(device="cuda").manual_seed(left)
+        banned = torch.rand(B * N, V, generator=g, device="cuda").argsort(1) >= left
+        logits[banned] = torch.finfo(dtype).min
+        _check(logits, scores, keep)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_equal_logits_do_not_take_many_times_as_long(dtype):
+    """Rows of one segment each, all but five tokens banned by the lowest finite number: a few passes over them, not one for each that is kept."""
+    from pbs_attn_b200.beam import beam_select
+    logits, scores = _logits(64, 8, 100003, dtype, 13)
+    usual = _time_of(lambda: beam_select(logits, scores))
+    logits[:, 5:] = torch.finfo(dtype).min
+    assert _time_of(lambda: beam_select(logits, scores)) <= 8 * usual
