@@ -256,9 +256,9 @@ struct Row {
 struct Sum {
   float top = -kFltMax, sum = 0.f;
 
-  // Takes in P pieces (a NaN among them becomes -infinity) and returns the largest of their logits.
+  // Takes in P pieces and returns the largest of their logits (a NaN counts as -infinity).
   template <class T>
-  __device__ __forceinline__ float add(uint4 (&w)[P]) {
+  __device__ __forceinline__ float add(const uint4 (&w)[P]) {
     using E = Piece<T>;
     constexpr int N = E::N;
     float most = E::most(w[0]);
@@ -288,11 +288,7 @@ struct Sum {
         float x[N];
         E::get(w[k], x);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          x[i] = counted(x[i]);
-          more += exp2_fast((fminf(x[i], kFltMax) - higher) * kLog2e);
-        }
-        w[k] = E::put(x);
+        for (int i = 0; i < N; ++i) more += exp2_fast((fminf(counted(x[i]), kFltMax) - higher) * kLog2e);
       }
     }
     sum = sum * exp2_fast((top - higher) * kLog2e) + more;
