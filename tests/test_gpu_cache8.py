@@ -280,3 +280,75 @@ def test_gather_within_the_rounding_of_the_type():
     got = paged_kv_gather(cache, ints(1, 0)[None], ints(20), 20)[0][0]
     want = values8(cache, cache.k, cache.k_params, ints(1, 0)[None], 0, 20)[0]
     assert_within(got, want, want.abs() * (2.0 ** -8 + 2.0 ** -23) + 2.0 ** -134)
+
+
+def _guarded(pages, page_size, heads, dim, dtype, block, seed):
+    """A cache of codes and scales that are all different, and finite, inside of memory that is none of its own on every side."""
+    from pbs_attn_b200.decode import PagedKVCache
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    codes = [torch.randint(-127, 128, (pages + 2, heads + 2, page_size + 2, dim + 32), generator=g, device="cuda", dtype=torch.int8) for _ in "kv"]
+    scales = [torch.rand(pages + 2, heads + 2, page_size // block + 2, generator=g, device="cuda") / 8 for _ in "kv"]
+    inside = lambda memory: ([t[1:-1, 1:-1, 1:-1, 16:-16] for t in memory[:2]] + [t[1:-1, 1:-1, 1:-1] for t in memory[2:]])  # noqa: E731
+    return PagedKVCache.from_tensors(*inside(codes + scales), dtype=dtype), codes + scales, inside
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("ps,block", [(16, 16), (64, 16), (64, 32), (64, 64), (128, 64)])
+@pytest.mark.parametrize("S", [1, 4, 5, 16, 17, 70])
+def test_nothing_beside_a_calls_tokens_changes(dtype, D, ps, block, S):
+    """Codes and scales of every page, block and head, and of the memory around them, are known and compared, those that no call comes to among them."""
+    from pbs_attn_b200.decode import paged_kv_append
+    H = 3
+    starts = [0, 1, block - 1, block, ps - 1, ps, 2 * ps + 3]
+    new = [S, 0, S, max(1, S // 2), S, 1, S]
+    lens = [a + m for a, m in zip(starts, new)]
+    cache, memory, inside = _guarded(pages_for(lens, ps), ps, H, D, dtype, block, S + D)
+    want = [t.clone() for t in memory]
+    wk, wv, wks, wvs = inside(want)
+    table = make_table(cache, lens, S)
+    cos, sin = rope_tables(max(lens), D, dtype)
+    k, v, q = _data(lens, S, H, D, dtype, S, 2.0)
+    room = torch.full((len(lens), S + 2, 2 * H + 2, D), 7.0, dtype=dtype, device="cuda")
+    out = room[:, 1:-1, 1:-1].transpose(1, 2)
+    paged_kv_append(cache, k, v, table, ints(*lens), new_lens=ints(*new), cos=cos, sin=sin, query_states=q, query_out=out)
+    cache.check_status()
+    pos = torch.stack([(a + torch.arange(S, device="cuda")).clamp(max=max(lens) - 1) for a in starts])
+    c, s = cos[pos].float()[:, None], sin[pos].float()[:, None]
+    append8(cache, wk, wks, rotate(k.float(), c, s), table, lens, new)
+    append8(cache, wv, wvs, v.float(), table, lens, new)
+    for got, x in zip(memory, want):
+        assert torch.equal(got, x)
+    there = torch.arange(S, device="cuda") < ints(*new)[:, None]
+    assert torch.equal(out, torch.where(there[:, None, :, None], rotate(q.float(), c, s).to(dtype), 0))
+    out.fill_(7.0)
+    assert (room == 7).all()
+
+
+@pytest.mark.parametrize("growth", [1.0, 1.25, 1.5, 2.0, 3.0])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_tokens_error_is_half_of_each_step_that_it_was_rounded_to(dtype, growth):
+    """A token is off by half a step when it is written, and by half a step of then each time that its block's scale grows, no more.  Reciprocals and
+    ratios that codes up to 127 are multiplied by are rounded: 127 * 2^-24 of a step each time, taken as 2^-16.  Where the scale doubles with every
+    token these halves come to less than one step of the last."""
+    from pbs_attn_b200.decode import paged_kv_append
+    H, D, n = 4, 256, 16 if growth <= 2 else 7             # (3^6 is a number of eight bits times a power of 2, to within the type's rounding)
+    cache = make_cache8(1, 16, H, D, dtype, 16)
+    g = torch.Generator(device="cuda").manual_seed(int(growth * 8))
+    x = torch.rand(H, n, D, generator=g, device="cuda") * 2 - 1
+    x[..., 7] = 1.0
+    x = (x * (2.0 ** -6 * growth ** torch.arange(n, device="cuda", dtype=torch.float64))[:, None]).to(dtype)
+    steps = torch.zeros(H, n, dtype=torch.float64, device="cuda")
+    off = torch.zeros(H, n, dtype=torch.float64, device="cuda")                   # what each token may be off by
+    for t in range(n):
+        row = x[:, t][None, :, None]
+        paged_kv_append(cache, row, row, ints(0)[None], ints(t + 1))
+        steps[:, t] = cache.k_params[0, :, 0].double()
+        grown = torch.ones(H, dtype=torch.bool, device="cuda") if t == 0 else steps[:, t] > steps[:, t - 1]
+        off[:, :t] += torch.where(grown, steps[:, t], 0)[:, None] * (0.5 + 2.0 ** -16)
+        off[:, t] += steps[:, t] * (0.5 + 2.0 ** -16)
+    for codes, scales in ((cache.k, cache.k_params), (cache.v, cache.v_params)):
+        held = values8(cache, codes, scales, ints(0)[None], 0, n)[0]
+        assert ((held - x.double()).abs() <= off[..., None]).all()
+    if growth == 2.0:
+        assert (off < steps[:, -1:] * (1 + 2.0 ** -12)).all()
