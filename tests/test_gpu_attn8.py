@@ -311,3 +311,29 @@ def test_written_rows_attended_rows_and_rows_behind_them():
         x = torch.randn(3, 2, 2, 1, 128, generator=g, device="cuda").mul(1 + step / 3).bfloat16()
         paged_kv_append(cache, x[0], x[1], table, ints(*lens))
         _run(q, cache, table, lens)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [2, 11, 200, 3000])
+def test_channels_in_which_the_token_that_weighs_most_is_zero(dtype, n):
+    """What is left there is small, beside sums of codes plus 128, up to 255 of a weight times its scale.  These run over up to eight tiles of up to two
+    products of 17 terms, each of which is cut below 2^-23 of the largest, and what they are less is summed up the same: 2 * 16 * 17 * 255 * 2^-23 of the
+    weighted scale at most, below 2^-5, beside the other bounds.  (Half a step of it is what a value lost when it was written.)"""
+    from pbs_attn_b200.decode import paged_attn_fwd, paged_kv_append
+    D, ps = 128, 64
+    pages = -(-n // ps)
+    for at in (0, n // 2, n - 1):
+        g = torch.Generator(device="cuda").manual_seed(n + at)
+        cache = make_cache8(pages, ps, 1, D, dtype, 64)
+        k, v, q = (torch.randn(1, 1, s, D, generator=g, device="cuda") for s in (n, n, 1))
+        k[0, 0, at] = 12 * q[0, 0, 0] / q.norm() * D ** 0.5 / q.norm() * D ** 0.5
+        v[0, 0, at, :D // 2] = 0
+        table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+        paged_kv_append(cache, k.to(dtype), v.to(dtype), table, ints(n))
+        q = q.expand(1, 8, 1, D).to(dtype)
+        got = paged_attn_fwd(q, cache, table, ints(n))
+        cache.check_status()
+        want, bound = attention8(q, cache, table, [n])
+        scale = cache.v_params.abs().max().double()
+        assert_within(got, want, bound + scale * 2.0 ** -5)
+        assert (want[..., :D // 2].abs() < 1e-2 * want[..., D // 2:].abs().max()).all()
