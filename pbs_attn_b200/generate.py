@@ -11,6 +11,7 @@ reference patches prompts only and leaves single tokens to the model's own forwa
 from __future__ import annotations
 
 import copy
+import math
 from typing import Optional, Sequence, Union
 
 import torch
@@ -130,7 +131,8 @@ class _Beams:
         self.rows = torch.arange(B, device=device)[:, None] * beams
         self.scores = torch.full((B, beams), float("-inf"), device=device)
         self.scores[:, 0] = 0.0                            # (all rows are the prompt still)
-        self.done_scores = torch.full((B, beams), float("-inf"), device=device)
+        # (in 64 bits: 32 do not hold large powers of a length)
+        self.done_scores = torch.full((B, beams), float("-inf"), dtype=torch.double, device=device)
         self.done_tokens = torch.full((B, beams, steps), self.pad, dtype=torch.long, device=device)
 
     def choose(self, logits: torch.Tensor, cache: PagedModelCache) -> torch.Tensor:
@@ -141,7 +143,7 @@ class _Beams:
             ended = (tokens[..., None] == self.ends).any(-1)
             count = cache.seq_lens[0] - (self.S - 1)       # tokens written, this one among them
             # of the N best alone: one that comes after them is not a beam
-            final = torch.where(ended[:, :self.N], scores[:, :self.N] / count ** self.power, float("-inf"))
+            final = torch.where(ended[:, :self.N], scores[:, :self.N].double() / count.double() ** self.power, float("-inf"))
             texts = written[self.rows + beams[:, :self.N]]                            # (B, N, steps)
             texts = texts.scatter(2, (count - 1).long().expand(*texts.shape[:2], 1), tokens[:, :self.N, None])
             after = torch.arange(texts.shape[2], device=texts.device) >= count
@@ -164,7 +166,7 @@ class _Beams:
     def best(self, input_ids: torch.Tensor) -> torch.Tensor:
         """The best of each sequence, those that have not ended among them: (B, S + steps)."""
         steps = self.done_tokens.shape[2]
-        self._enter(self.scores / steps ** self.power, self.history[:, self.S:].unflatten(0, (-1, self.N)))
+        self._enter(self.scores.double() / steps ** self.power, self.history[:, self.S:].unflatten(0, (-1, self.N)))
         return torch.cat([input_ids, self.done_tokens[:, 0]], 1)
 
 
@@ -204,6 +206,8 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, bits: int =
         raise ValueError(f"num_beams={num_beams} with {len(ends)} end tokens: at most {MAX_BEAMS}, and {MAX_KEEP} continuations a step")
     if ends and num_beams == 1:
         raise ValueError("eos_token_id is for beams (num_beams > 1): a greedy sequence goes on for max_new_tokens")
+    if num_beams > 1 and not (math.isfinite(length_penalty) and abs(length_penalty) * math.log(max_new_tokens) < 600):
+        raise ValueError(f"length_penalty={length_penalty}: {max_new_tokens} to the power of it is beyond 64 bits")
     with torch.cuda.device(input_ids.device):              # (graphs, streams and events belong to the current one)
         cache = PagedModelCache(model, B, S + max_new_tokens, bits, page_size, group_size, block_size, num_beams, S)
         beams = _Beams(input_ids, max_new_tokens, num_beams, ends, length_penalty) if num_beams > 1 else None

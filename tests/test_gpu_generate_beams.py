@@ -226,3 +226,24 @@ def test_calls_that_follow_one_another_see_what_the_one_before_wrote(captured):
         cache.check_status()
         results.append([x.clone() for x in (back, last, scores, table, lens, cache.k, cache.v, cache.k_params)])
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("power", [30.0, 60.0, -30.0])
+def test_length_penalties_whose_powers_32_bits_do_not_hold(power):
+    """24 tokens to the power of 30 are more than 2^128: texts are told apart all the same."""
+    from pbs_attn_b200.generate import generate
+    model, new, ends = _model(), 24, tuple(range(0, 60, 6))
+    ids = torch.randint(0, 300, (3, 40), device="cuda")
+    steps = []
+    out = generate(_patched(model), ids, new, cuda_graph=False, step_logits=steps, num_beams=4, length_penalty=power, eos_token_id=ends)
+    assert out[:, 40:].tolist() == _plain_search(steps, 3, 4, new, ends, power)[0]
+    assert torch.equal(out, generate(model, ids, new, num_beams=4, length_penalty=power, eos_token_id=ends))
+
+
+def test_length_penalties_that_are_no_numbers_to_count_with():
+    from pbs_attn_b200.generate import generate
+    model = _patched(_model())
+    ids = torch.zeros(1, 4, dtype=torch.long, device="cuda")
+    for power in (math.inf, -math.inf, math.nan, 1e4, -1e4):
+        with pytest.raises(ValueError, match="length_penalty"):
+            generate(model, ids, 3, num_beams=2, length_penalty=power)
