@@ -357,10 +357,10 @@ int pbs_paged_gather(const pbs_paged_cache_t* cache, const pbs_paged_batch_t* ba
 /* Causal attention of the new tokens' queries, q (B, q_heads, S, D), over the cache: token i sees the positions up to its own.
  * out has q's shape; rows that see nothing, or scores of -infinity alone, are 0.  Softmax and sums are held in 32 bits.
  * Range for 16 bits: that of the type (bf16 values below 2^-90 may count as 0).  For 8 bits: |v| from 2^-66 to 2^100 in bf16 (what scales below
- * 2^-70 stand for loses bits); queries are rounded to 2^-15 of the largest of their row, weights times scales to fp16, and a result is off by up to
- * 2^-12 of the weighted mean of the scales besides (sums of codes plus 128; half a scale is what a value lost when it was written).  For 4 bits: in bf16 |q| up to 2^100 (what is 2^29 below
- * the largest of a query's row counts as 0) and |v| from 2^-80 to 2^100; in both types, a group of channels whose steps are 2^20 below
- * those of another group of the head loses bits, and one 2^30 below it counts as its minima.
+ * 2^-70 stand for loses bits); queries are rounded to 2^-15 of the largest of their row, weights times scales to 11 bits in bf16 and to 22 in fp16,
+ * and a result is off by up to 2^-12 of the weighted mean of the scales besides (sums of codes plus 128; half a scale is what a value lost when it
+ * was written).  For 4 bits: in bf16 |q| up to 2^100 (what is 2^29 below the largest of a query's row counts as 0) and |v| from 2^-80 to 2^100; in
+ * both types, a group of channels whose steps are 2^20 below those of another group of the head loses bits, and one 2^30 below it counts as its minima.
  * What a row does not see does not reach it, infinities and NaNs included: its bits do not change with the values of tokens behind it or
  * of other sequences (8 bits: as the cache holds them; appending a token behind it may change the scale of a block that it sees).  They may with the batch, the lengths in it, the table's width, the number of new tokens and the GPU, which decide
  * where a sequence is cut and in what order its sums are added; with all of these alike they are the same every time.

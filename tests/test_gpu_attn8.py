@@ -337,3 +337,17 @@ def test_channels_in_which_the_token_that_weighs_most_is_zero(dtype, n):
         scale = cache.v_params.abs().max().double()
         assert_within(got, want, bound + scale * 2.0 ** -5)
         assert (want[..., :D // 2].abs() < 1e-2 * want[..., D // 2:].abs().max()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,Hq,Hkv,S", [(128, 8, 2, 1), (128, 20, 1, 1), (64, 16, 2, 2), (256, 8, 1, 1)])
+def test_a_results_own_rounding_is_the_largest_of_its_errors(dtype, D, Hq, Hkv, S):
+    """Over a whole result what the kernel adds to rounding it once to its type stays below half of that rounding: sqrt(1 + 1 / 4) of it together."""
+    from pbs_attn_b200.decode import paged_attn_fwd
+    lens = [40, 300, 1200, 3000]
+    for spread in (0.0, 1.0):
+        q, cache, table = _case(lens, Hq, Hkv, S, D, dtype, spread=spread, seed=3)
+        want, _ = attention8(q, cache, table, lens)
+        got = paged_attn_fwd(q, cache, table, ints(*lens))
+        off, own = (got.double() - want).norm(), (want.to(dtype).double() - want).norm()
+        assert off <= math.sqrt(1.25) * own, (float(off / want.norm()), float(own / want.norm()))
