@@ -10,10 +10,10 @@
 // cut down to K now and then, the CTA's warps waited for one another and branched: 76 us for 512 rows of 152064 in fp32.)
 // The CTA that finishes an entry last merges the sorted lists of its segments in the same way, by score.
 //
-// Measured (B200, GPU time): 512 rows of 152064 in fp32, 64 entries of eight beams, 64 us, 74 % of the copy rate: streaming runs at it, the segments'
-// ends and the merges (5 us each) behind it do not overlap much, as all rows end at once; in bf16 50 us, 47 %: 23 us of instruction issue and 20 of
-// exponentials where an SM has four rows.  64 rows of 128256 in bf16 17 us, four 11, one 10: latency of 20000 cycles, of which the meeting of
-// the segments (fence, count, loads, ranks) is more than half.
+// Measured (B200, GPU time): 512 rows of 152064 in fp32, 64 entries of eight beams, 61 to 64 us, 74 to 78 % of the copy rate: streaming runs at it, the
+// segments' ends and the merges (5 us each) behind it do not overlap much, as all rows end at once; in bf16 50 us, 47 %: 23 us of instruction issue
+// and 20 of exponentials, which come one after the other in every warp.  64 rows of 128256 in bf16 17 us, four 11, one 10: latency of 20000 cycles, of
+// which the meeting of the segments (fence, count, loads, ranks) is more than half.
 #include <climits>
 
 #include "pbs_paged.cuh"

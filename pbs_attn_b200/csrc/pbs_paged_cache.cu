@@ -1,14 +1,14 @@
 // New keys and values into a paged cache, rotated and quantised on the way, and back.
 //
 // D / 8 neighbouring lanes hold a row of D channels, eight each: a lane's channels are 16 bytes of the input and, in 4 bits, one word of the
-// cache.  The other half of a row, for the rotation, is D / 16 lanes away, and a group's extremes meet over G / 8 lanes, so no shared memory
-// is needed and every byte is read and written once.  A CTA's groups of lanes take neighbouring tokens and the same heads, of the queries, the
-// keys or the values, so nothing branches within a warp and codes of neighbouring tokens are written together.
+// cache.  The other half of a row, for the rotation, is D / 16 lanes away, and a group's extremes (4 bits) meet over G / 8 lanes, so 16 and 4 bits
+// need no shared memory, and every byte is read and written once.  A CTA's groups of lanes take neighbouring tokens and the same heads, of the
+// queries, the keys or the values, so nothing branches within a warp and codes of neighbouring tokens are written together.  8 bits: see below.
 //
 // HBM bounds prompts, latency and the launch single tokens.  8191 tokens of 8 KV heads into 4 bits: 15 us (33.5 MB read, 9.4 MB written, 2.9
-// TB/s; 75 % of the issue slots are taken: some 170 instructions for eight channels), back out 11 us; 64 sequences' next tokens, 32 query
-// heads rotated, 2.5 us.  Into 8 bits 11.5 us (50 MB, 4.4 TB/s, 67 %: instruction issue and the last CTAs) and back 9.0 (86 %); one token 2.6 us,
-// 64 sequences' 3.0, with drafts of up to four 3.2.
+// TB/s; 75 % of the issue slots are taken: some 170 instructions for eight channels), back out 8.9 us; 64 sequences' next tokens, 32 query
+// heads rotated, 2.3 us.  Into 8 bits 11.2 us (50 MB, 4.5 TB/s, 68 %; 64 % of the issue slots: a warp's loads, maximum, scale and stores come one
+// after another, and nothing of a next block is under way) and back 8.9 (86 %); one token 2.5 us, 64 sequences' 3.0, with drafts of up to four 3.1.
 #include <climits>
 #include <type_traits>
 
@@ -331,7 +331,7 @@ __device__ __forceinline__ uint2 scaled8(const uint2& w, float ratio) {
 
 constexpr int kPrompt = 128;
 
-// Prompts: a warp takes 16 tokens of a block, blocks of 32 and 64 are several warps'.  Four warps a CTA, ten CTAs a SM: 11.5 us for 8191 tokens, 11.1 in
+// Prompts: a warp takes 16 tokens of a block, blocks of 32 and 64 are several warps'.  Four warps a CTA, ten CTAs a SM: 11.2 us for 8191 tokens, 11.1 in
 // blocks of 64, 12.3 of 64 channels (eight warps, four CTAs: 11.7, 12.7 and 13.5; twelve CTAs, spilling: 14.3, 12.7 and 11.8).
 template <int DT, int D, int W, bool ROPE>
 __global__ void __launch_bounds__(kPrompt, D == 256 ? ROPE ? 2 : 4 : ROPE ? 4 : 10) paged_append8_kernel(const __grid_constant__ AppendArgs p, int blocks, int units) {

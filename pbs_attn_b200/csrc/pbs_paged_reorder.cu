@@ -6,9 +6,10 @@
 //
 // Bound by HBM: what moves is read once and written once.  One launch for up to kLayers layers; a CTA takes a group's keys or values of one head
 // in some of them, and looks up once what moves.  32 layers of 8 KV heads of 128, pages of 64 tokens half full, half of the rows moving: 8 groups of
-// four in 16 bits 26.4 us for 134 MB (77 % of the copy rate), 32 of eight 156 us; one of four in 8 bits 4.9 us.  (Divisions by the units of a page and
+// four in 16 bits 25.7 us for 134 MB (80 % of the copy rate), 32 of eight 156 us; one of four in 8 bits 4.6 us.  (Divisions by the units of a page and
 // four rows' pieces in registers whatever the number that moves, one CTA a SM: 65 us.  72 registers, three CTAs a SM, each taking twice as much:
-// 27.6, 166 and 7.0; 48 registers, five: 32, 156 and 6.3.)
+// 27.6, 166 and 7.0; 48 registers, five: 32, 156 and 6.3.)  A group's table is one CTA's, 256 columns at a time: four rows of 1024 full pages 6.0 us, of
+// 2048 8.3, of 8192 (131072 tokens in pages of 16) 21.4.
 #include <climits>
 
 #include "pbs_paged.cuh"
