@@ -415,7 +415,8 @@ int pbs_process_logits(const pbs_logits_t* args, void* stream);
  * the `keep` largest, larger ones first: scores, beams and tokens.  Of equal scores the lower beam comes first, within a beam the larger logit,
  * of equal ones the lower token.  A NaN counts as -infinity, a logit of +infinity as the largest number of 32 bits.  Beams whose score is
  * -infinity are not alive (their tokens come in their order, with -infinity, where there is nothing else).  Scores are formed in 64 bits from sums
- * in 32 and rounded once.
+ * in 32 and rounded once.  The logits of beams that are not alive are not looked at; rows with more than 1024 equal logits among their largest (not
+ * -infinity) take a few times as long.
  * workspace: pbs_beam_select_workspace bytes; its first PBS_PAGED_COUNTER_BYTES are 0 before the first call and each call leaves them so.
  * Calls that share one come after one another. */
 typedef struct {

@@ -192,7 +192,7 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, bits: int =
 
     With ``num_beams`` N > 1 the N best continuations of each sequence go on instead: by the sum of their tokens' log-probabilities after penalties,
     biases and mask.  One of the N best that ends in ``eos_token_id`` (one or a few) leaves them, with its sum divided by its number of new tokens
-    to the power of ``length_penalty``.  After ``max_new_tokens`` steps the best of those that ended and of those that run is returned, filled up with the
+    to the power of ``length_penalty`` (a power that 64 bits hold).  After ``max_new_tokens`` steps the best of those that ended and of those that run is returned, filled up with the
     (first) end token.  What is given by the sequence holds for its beams; ``step_logits`` has a row for each."""
     if not is_model_supported(model) or any("original_forward" not in layer.self_attn.__dict__ for layer in model.model.layers):
         raise ValueError("generate needs a model whose layers are all patched (apply_patch_with_prefill)")
